@@ -4,6 +4,10 @@
 returns the context ``[B, S, A*64]`` -- the layouts on both sides of BERT's attention, so nothing is
 transposed or copied around the kernels.  Head dim 64, S in {128, 256, 384, 512}, optional key-padding lengths, no dropout;
 anything else goes through ``F.scaled_dot_product_attention`` (also the oracle of the kernel tests).
+
+``attention(q, k, v)`` (kernel K22, ``csrc/attn_general_kernels.hip``) is the general form: any lengths (one query token
+included), head dims that are multiples of 8 to 128, fewer key than query heads, causal or with key lengths, strided
+operands; bf16 on the GPU.  CPU tensors take :func:`attention_general_reference`.
 """
 from __future__ import annotations
 
@@ -13,6 +17,7 @@ import os
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -97,3 +102,129 @@ def attention_reference(qkv, kv_len=None):
     if kv_len is not None:
         mask = (torch.arange(S, device=qkv.device)[None, :] < kv_len.to(qkv.device)[:, None])[:, None, None, :]
     return F.scaled_dot_product_attention(q, k, v, attn_mask=mask).transpose(1, 2).reshape(B, S, A * D)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# K22: any lengths, grouped heads, causal
+# ---------------------------------------------------------------------------------------------------------------------
+_general = None
+
+
+def _general_kernels():
+    global _general
+    if _general is None:
+        P, I, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+        _general = (hip.declare("dtf_attn_general_fwd", [P] * 6 + [I] * 7 + [Fl, P, P]),
+                    hip.declare("dtf_attn_general_bwd", [P] * 11 + [I] * 7 + [Fl, P, P]))
+    return _general
+
+
+def _operand(t):
+    """As it is where the kernels can address it (dense head dimension, 16-B aligned rows), else a contiguous copy."""
+    st = t.stride()
+    if st[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _general_strides(*tensors):
+    return (ctypes.c_int64 * (3 * len(tensors)))(*(0 if n == 1 else s for t in tensors for n, s in zip(t.shape[:3], t.stride())))
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_len, causal, scale):
+        q, k, v = _operand(q), _operand(k), _operand(v)
+        B, Sq, Hq, D = q.shape
+        Sk, Hk = k.shape[1], k.shape[2]
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, Hq, Sq, dtype=torch.float32, device=q.device)
+        with hip.on_device(q):
+            rc = _general_kernels()[0](q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                                       _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len),
+                                       hip.stream())
+        hip.check(rc, "dtf_attn_general_fwd")
+        ctx.save_for_backward(q, k, v, o, lse, kv_len)
+        ctx.how = causal, scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, kv_len = ctx.saved_tensors
+        B, Sq, Hq, D = q.shape
+        Sk, Hk = k.shape[1], k.shape[2]
+        if not do.is_contiguous() or do.data_ptr() % 16:
+            do = do.clone(memory_format=torch.contiguous_format)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dsum = torch.empty(B, Hq, Sq, dtype=torch.float32, device=q.device)
+        with hip.on_device(q):
+            rc = _general_kernels()[1](q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                                       dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _general_strides(q, k, v),
+                                       B, Sq, Sk, Hq, Hk, D, *ctx.how, hip.ptr(kv_len), hip.stream())
+        hip.check(rc, "dtf_attn_general_bwd")
+        return dq, dk, dv, None, None, None
+
+
+def _check_general(q, k, v, kv_len, scale):
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError("attention: %s is [B, S, heads, D], got %s" % (n, tuple(t.shape)))
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("attention: q, k and v must share dtype and device")
+    B, Sq, Hq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("attention: q %s, k %s and v %s do not fit together" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if min(q.shape) < 1 or min(k.shape) < 1:
+        raise ValueError("attention: no dimension may be empty, got q %s and k %s" % (tuple(q.shape), tuple(k.shape)))
+    if Hq % k.shape[2]:
+        raise ValueError("attention: %d query heads do not divide over %d key heads" % (Hq, k.shape[2]))
+    if D % 8 or D > 128:
+        raise ValueError("attention: the head dimension must be a multiple of 8 up to 128, got %d" % D)
+    if max(Sq, k.shape[1]) > 1 << 30:
+        raise ValueError("attention: sequences are at most 2**30 tokens long")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("attention: scale must be positive and finite, got %r" % (scale,))
+    if kv_len is not None and (tuple(kv_len.shape) != (B,) or kv_len.is_floating_point() or kv_len.dtype == torch.bool):
+        raise ValueError("attention: kv_len holds one integer for each of the %d sequences" % B)
+
+
+def attention(q, k, v, causal=False, kv_len=None, scale=None):
+    """``softmax(scale q k^T) v`` per head: ``q`` ``[B, Sq, Hq, D]``, ``k`` and ``v`` ``[B, Sk, Hk, D]`` -> ``[B, Sq, Hq, D]``;
+    query head h reads key head ``h // (Hq / Hk)``, ``scale`` is ``1 / sqrt(D)`` by default.  ``causal``: query i sees the keys
+    ``j <= i + Sk - Sq`` (the last query sees all).  ``kv_len`` (integers ``[B]``, values taken to ``[0, Sk]``): keys at or past
+    it are padding and never read.  A query that sees no key gets zeros, and passes no gradient on."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    _check_general(q, k, v, kv_len, scale)
+    if not q.is_cuda:
+        return attention_general_reference(q, k, v, causal, kv_len, scale)
+    if q.dtype != torch.bfloat16:
+        raise TypeError("attention: the GPU kernels take bfloat16, got %s" % q.dtype)
+    if kv_len is not None:
+        if kv_len.dtype != torch.int32:
+            kv_len = kv_len.clamp(0, k.shape[1])
+        kv_len = kv_len.to(device=q.device, dtype=torch.int32).contiguous()
+    return _Attention.apply(q, k, v, kv_len, int(bool(causal)), scale)
+
+
+def attention_general_reference(q, k, v, causal=False, kv_len=None, scale=None):
+    """The definition in elementary operations (fp32, fp64 for fp64 operands)."""
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    at = torch.arange(Sk, device=q.device)
+    seen = torch.ones(B, 1, 1, Sk, dtype=torch.bool, device=q.device)
+    if kv_len is not None:
+        seen = (at < kv_len.to(q.device)[:, None])[:, None, None, :]
+        pad = ~seen.view(B, Sk, 1, 1)
+        k, v = k.masked_fill(pad, 0), v.masked_fill(pad, 0)               # whatever padding holds takes no part
+    if causal:
+        seen = seen & (at <= torch.arange(Sq, device=q.device)[:, None] + (Sk - Sq))
+    qt, kt, vt = (t.to(dt).transpose(1, 2) for t in (q, k, v))
+    kt, vt = (t.repeat_interleave(Hq // Hk, dim=1) for t in (kt, vt))
+    s = (torch.matmul(qt, kt.transpose(2, 3).contiguous()) * scale).masked_fill(~seen, -math.inf)
+    e = torch.exp(s - s.detach().amax(-1, keepdim=True).clamp_min(-1e30))
+    z = e.sum(-1, keepdim=True)
+    p = e / torch.where(z == 0, torch.ones_like(z), z)
+    return torch.matmul(p, vt).transpose(1, 2).to(q.dtype).contiguous()

@@ -1,0 +1,510 @@
+// K22: attention of any length on gfx950 -- bf16, head dims to 128, grouped heads, causal or with key lengths, strided
+// operands; forward and the backward that recomputes the probabilities.
+//
+//   vis(i) = number of keys that query i sees (always a prefix): min(kv_len[b], causal ? i + 1 + Sk - Sq : Sk), >= 0
+//   S = c Q K^T,  P = softmax over the vis(i) keys (no key: P = 0),  O = P V
+//   D = rowsum(dO o O),  dP = dO V^T,  dS = P o (dP - D),  dQ = c dS K,  dK = c dS^T Q,  dV = P^T dO
+//
+// One online-softmax pass over the keys, 32x32x16 MFMA tiles:
+//   S^T = K . Q^T      a lane owns ONE query (column lane & 31) and 16 of a tile's 32 keys, so the running maximum and
+//                      sum are register reductions plus one exchange with lane ^ 32
+//   O^T = V^T . P^T    the score accumulator, rounded to bf16, IS the B operand: registers 8s .. 8s+7 of a lane hold the
+//                      keys 16s + 8 (j >> 2) + 4 g + (j & 3), j = 0..7, g = lane >> 5; the A operand V^T comes in that
+//                      key order from two ds_read_b64_tr_b16
+// P and dS are rounded to bf16 for the second products (their operands' type: half a step, 2^-9 of each term, random in
+// sign, so the sums keep the accuracy of the bf16 results); scores, maxima, sums, L, D and all accumulators are fp32.
+#include "dtf_common.h"
+
+typedef __attribute__((ext_vector_type(4))) short ag_s16x4;
+typedef __attribute__((address_space(3))) void ag_lds_void;
+typedef unsigned short u16;
+
+#define AG_NEG (-__builtin_inff())
+
+struct AgArgs {
+    const u16 *q, *k, *v;                 // element (b, s, h, d) of T at T + b*T_bs + s*T_ss + h*T_hs + d
+    int64_t q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs;
+    const u16 *o, *dO;                    // contiguous [B, Sq, Hq, D]
+    u16 *out, *dq, *dk, *dv;              // contiguous [B, Sq, Hq, D] (dk, dv: [B, Sk, Hk, D])
+    float *lse, *dsum;                    // [B, Hq, Sq]; lse in the log2 domain, +inf for a query that sees no key
+    const int* kv_len;                    // [B] or null
+    int B, Sq, Sk, Hq, Hk, D, group, causal, ntiles;
+    float scale, scale_log2e;
+};
+
+// LDS image of a [rows][DP] bf16 tile, 16-B chunk c of row r.  Conflict-free (256 B of banks) both for ds_read_b128 of
+// 16 rows at one chunk and for ds_read_b64_tr_b16 of 8 rows x 32 columns.
+template <int DP>
+__device__ __forceinline__ int ag_off(int row, int c) {
+    if constexpr (DP == 128) return row * 256 + ((((c >> 1) ^ (row & 7)) << 5) | (((c ^ (row >> 3)) & 1) << 4));
+    else return row * 128 + ((((c >> 1) ^ ((row >> 1) & 3)) << 5) | (((c ^ (row >> 3)) & 1) << 4));
+}
+
+__device__ __forceinline__ f32x16 ag_zero() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+__device__ __forceinline__ f32x16 ag_mfma(s16x8 a, s16x8 b, f32x16 c) {
+    typedef __attribute__((ext_vector_type(8))) __bf16 bf8;
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+// registers 8s .. 8s+7 of an accumulator as a bf16 operand
+__device__ __forceinline__ s16x8 ag_pack(const f32x16& x, int s) {
+    const u32x4 p = {pack_bf16x2(x[8 * s], x[8 * s + 1]), pack_bf16x2(x[8 * s + 2], x[8 * s + 3]),
+                     pack_bf16x2(x[8 * s + 4], x[8 * s + 5]), pack_bf16x2(x[8 * s + 6], x[8 * s + 7])};
+    return __builtin_bit_cast(s16x8, p);
+}
+
+// transposed A operand from an image: 32 columns d0 .. d0+31 as rows, 16 image rows row0 .. row0+15 as k in the
+// accumulators' key order.  The 16 lanes of a group read a 4-row x 16-column block, lane 4 q + p its row q, columns 4 p.
+template <int DP>
+__device__ __forceinline__ s16x8 ag_tr(const unsigned char* img, int row0, int d0, int lane) {
+    const int g = lane >> 5, row = row0 + 4 * g + ((lane >> 2) & 3), col = d0 + (lane & 16) + 4 * (lane & 3);
+    const unsigned char* p0 = img + ag_off<DP>(row, col >> 3) + (col & 7) * 2;
+    const unsigned char* p1 = img + ag_off<DP>(row + 8, col >> 3) + (col & 7) * 2;
+    typedef __attribute__((address_space(3))) ag_s16x4* lp;
+    const ag_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p0);
+    const ag_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p1);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <int DP>
+__device__ __forceinline__ s16x8 ag_row(const unsigned char* img, int row, int c) {
+    return *reinterpret_cast<const s16x8*>(img + ag_off<DP>(row, c));
+}
+
+// A tile of ROWS rows in flight from memory to an image through registers; rows at or past `limit` and columns past D
+// are zeros (never read), so nothing masked reaches a product.
+template <int DP, int ROWS, int NT>
+struct AgTile {
+    static constexpr int CPR = DP / 8, N = ROWS * CPR / NT;
+    u32x4 r[N];
+    __device__ __forceinline__ void load(const u16* base, int64_t rs, int row0, int limit, int D, int tid) {
+        const int c = tid % CPR;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = row0 + tid / CPR + i * (NT / CPR);
+            r[i] = (u32x4){0u, 0u, 0u, 0u};
+            if (row < limit && c * 8 < D) r[i] = *reinterpret_cast<const u32x4*>(base + row * rs + c * 8);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* img, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            *reinterpret_cast<u32x4*>(img + ag_off<DP>(tid / CPR + i * (NT / CPR), tid % CPR)) = r[i];
+    }
+};
+
+// workgroups of one head land on one XCD (ids go round the 8 XCDs), so its keys and values are read into one L2
+__device__ __forceinline__ int ag_xcd(int id, int n) {
+    const int q = n >> 3, r = n & 7, x = id & 7, i = id >> 3;
+    return x * q + (x < r ? x : r) + i;
+}
+
+__device__ __forceinline__ int ag_vis(const AgArgs& a, int i, int klen) {
+    int n = a.causal ? min(klen, i + 1 + a.Sk - a.Sq) : klen;
+    return max(n, 0);
+}
+
+__device__ __forceinline__ int ag_klen(const AgArgs& a, int b) { return a.kv_len ? max(0, min(a.kv_len[b], a.Sk)) : a.Sk; }
+
+template <int DP>
+__device__ __forceinline__ void ag_frags(s16x8 (&f)[DP / 16], const u16* row, int g, int D) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        f[ks] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+        if (16 * ks + 8 * g < D) f[ks] = *reinterpret_cast<const s16x8*>(row + 16 * ks + 8 * g);
+    }
+}
+
+// accumulator tiles [32 d][this lane's row] -> 4 bf16 at a time
+template <int DP>
+__device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DP / 32], float f, int g, int D) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+            const int d = 32 * dt + 8 * rq + 4 * g;
+            if (d < D) {
+                const u32x2 p = {pack_bf16x2(acc[dt][4 * rq] * f, acc[dt][4 * rq + 1] * f),
+                                 pack_bf16x2(acc[dt][4 * rq + 2] * f, acc[dt][4 * rq + 3] * f)};
+                *reinterpret_cast<u32x2*>(row + d) = p;
+            }
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Forward: 4 waves x 32 queries, 64 keys a step.  PACK: the rows of a workgroup run over the `group` query heads of one
+// key head and their Sq queries, so a few queries with many heads still fill the matrix tile and read K, V once.
+// ---------------------------------------------------------------------------
+template <int DP, bool PACK>
+__global__ __launch_bounds__(256) void ag_fwd_kernel(AgArgs a) {
+    constexpr int KS = DP / 16, DT = DP / 32, BN = 64, BM = 128;
+    __shared__ __attribute__((aligned(16))) unsigned char Kimg[BN * DP * 2];
+    __shared__ __attribute__((aligned(16))) unsigned char Vimg[BN * DP * 2];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = ag_xcd(blockIdx.x, gridDim.x);
+    const int t = a.ntiles - 1 - id % a.ntiles, hb = id / a.ntiles;        // long causal tiles first
+    const int H = PACK ? a.Hk : a.Hq, b = hb / H, h = hb - b * H;
+    const int hk = PACK ? h : h / a.group, rows = PACK ? a.group * a.Sq : a.Sq;
+    const int klen = ag_klen(a, b);
+    const int r = min(t * BM + wave * 32 + (lane & 31), rows - 1);
+    const int i = PACK ? r % a.Sq : r, head = PACK ? h * a.group + r / a.Sq : h;
+    const int vis = ag_vis(a, i, klen);
+    const int end = PACK ? ag_vis(a, a.Sq - 1, klen) : ag_vis(a, min(t * BM + BM, a.Sq) - 1, klen);
+    int lo = vis, hi = vis;                                                // of this wave's queries
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        lo = min(lo, __shfl_xor(lo, o, 64));
+        hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+
+    const u16* Kh = a.k + b * a.k_bs + hk * a.k_hs;
+    const u16* Vh = a.v + b * a.v_bs + hk * a.v_hs;
+    s16x8 qf[KS];
+    ag_frags<DP>(qf, a.q + b * a.q_bs + i * a.q_ss + head * a.q_hs, g, a.D);
+
+    f32x16 oacc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_zero();
+    float m = AG_NEG, l = 0.f;
+    AgTile<DP, BN, 256> kr, vr;
+    if (end > 0) {
+        kr.load(Kh, a.k_ss, 0, klen, a.D, tid);
+        vr.load(Vh, a.v_ss, 0, klen, a.D, tid);
+    }
+    for (int k0 = 0; k0 < end; k0 += BN) {
+        __syncthreads();
+        kr.store(Kimg, tid);
+        vr.store(Vimg, tid);
+        __syncthreads();
+        if (k0 + BN < end) {
+            kr.load(Kh, a.k_ss, k0 + BN, klen, a.D, tid);
+            vr.load(Vh, a.v_ss, k0 + BN, klen, a.D, tid);
+        }
+        if (k0 >= hi) continue;                                            // (uniform in the wave; barriers stay matched)
+        f32x16 s[BN / 32];
+#pragma unroll
+        for (int u = 0; u < BN / 32; ++u) {
+            s[u] = ag_zero();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[u] = ag_mfma(ag_row<DP>(Kimg, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s[u]);
+        }
+        if (k0 + BN > lo) {
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (k0 + 32 * u + 8 * (e >> 2) + 4 * g + (e & 3) >= vis) s[u][e] = AG_NEG;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[u][e]);
+        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
+        const float mn = __builtin_elementwise_maximum(m, mx * a.scale_log2e);
+        const float mu = mn == AG_NEG ? 0.f : mn;                          // nothing seen yet: every p is exp2(-inf) = 0
+        const float alpha = __builtin_amdgcn_exp2f(m - mu);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
+#pragma unroll
+        for (int u = 0; u < BN / 32; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], a.scale_log2e, -mu));
+                l += s[u][e];
+            }
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+                const s16x8 pf = ag_pack(s[u], h2);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_mfma(ag_tr<DP>(Vimg, 32 * u + 16 * h2, 32 * dt, lane), pf, oacc[dt]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (t * BM + wave * 32 + (lane & 31) < rows) {
+        ag_store_row<DP>(a.out + (((int64_t)b * a.Sq + i) * a.Hq + head) * a.D, oacc, l == 0.f ? 0.f : 1.f / l, g, a.D);
+        if (g == 0) a.lse[((int64_t)b * a.Hq + head) * a.Sq + i] = l == 0.f ? __builtin_inff() : m + log2f(l);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Backward, dQ: 4 waves x 32 queries, 64 keys a step.  D comes from the matrix instruction too (the diagonal of O . dO^T,
+// summed over d in the order of dP = V . dO^T), so that a query with ONE key, whose O is that V row, has dS = 0 exactly.
+// ---------------------------------------------------------------------------
+template <int DP>
+__global__ __launch_bounds__(256) void ag_dq_kernel(AgArgs a) {
+    constexpr int KS = DP / 16, DT = DP / 32, BN = 64, BM = 128;
+    __shared__ __attribute__((aligned(16))) unsigned char Kimg[BN * DP * 2];
+    __shared__ __attribute__((aligned(16))) unsigned char Vimg[BN * DP * 2];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = ag_xcd(blockIdx.x, gridDim.x);
+    const int t = a.ntiles - 1 - id % a.ntiles, hb = id / a.ntiles;
+    const int b = hb / a.Hq, h = hb - b * a.Hq, hk = h / a.group;
+    const int klen = ag_klen(a, b);
+    const int i = min(t * BM + wave * 32 + (lane & 31), a.Sq - 1);
+    const int vis = ag_vis(a, i, klen), end = ag_vis(a, min(t * BM + BM, a.Sq) - 1, klen);
+    const int lo = ag_vis(a, min(t * BM + wave * 32, a.Sq - 1), klen), hi = ag_vis(a, min(t * BM + wave * 32 + 32, a.Sq) - 1, klen);
+
+    const u16* Kh = a.k + b * a.k_bs + hk * a.k_hs;
+    const u16* Vh = a.v + b * a.v_bs + hk * a.v_hs;
+    const int64_t row = ((int64_t)b * a.Sq + i) * a.Hq + h, li = ((int64_t)b * a.Hq + h) * a.Sq + i;
+    s16x8 qf[KS], gf[KS];
+    ag_frags<DP>(qf, a.q + b * a.q_bs + i * a.q_ss + h * a.q_hs, g, a.D);
+    ag_frags<DP>(gf, a.dO + row * a.D, g, a.D);
+    float dsum = 0.f;
+    {
+        s16x8 of[KS];
+        ag_frags<DP>(of, a.o + row * a.D, g, a.D);
+        f32x16 x = ag_zero();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x = ag_mfma(of[ks], gf[ks], x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (8 * (e >> 2) + 4 * g + (e & 3) == (lane & 31)) dsum = x[e];
+        dsum += __shfl_xor(dsum, 32, 64);
+    }
+    const float lse = a.lse[li];
+    const bool valid = t * BM + wave * 32 + (lane & 31) < a.Sq;
+    if (valid && g == 0) a.dsum[li] = dsum;
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_zero();
+    AgTile<DP, BN, 256> kr, vr;
+    if (end > 0) {
+        kr.load(Kh, a.k_ss, 0, klen, a.D, tid);
+        vr.load(Vh, a.v_ss, 0, klen, a.D, tid);
+    }
+    for (int k0 = 0; k0 < end; k0 += BN) {
+        __syncthreads();
+        kr.store(Kimg, tid);
+        vr.store(Vimg, tid);
+        __syncthreads();
+        if (k0 + BN < end) {
+            kr.load(Kh, a.k_ss, k0 + BN, klen, a.D, tid);
+            vr.load(Vh, a.v_ss, k0 + BN, klen, a.D, tid);
+        }
+        if (k0 >= hi) continue;
+#pragma unroll
+        for (int u = 0; u < BN / 32; ++u) {
+            f32x16 s = ag_zero(), dp = ag_zero();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = ag_mfma(ag_row<DP>(Kimg, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s);
+                dp = ag_mfma(ag_row<DP>(Vimg, 32 * u + (lane & 31), 2 * ks + g), gf[ks], dp);
+            }
+            const bool edge = k0 + 32 * u + 32 > lo;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse));
+                float ds = p * (dp[e] - dsum);
+                if (edge) ds = k0 + 32 * u + 8 * (e >> 2) + 4 * g + (e & 3) < vis ? ds : 0.f;
+                s[e] = ds;
+            }
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+                const s16x8 f = ag_pack(s, h2);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_mfma(ag_tr<DP>(Kimg, 32 * u + 16 * h2, 32 * dt, lane), f, acc[dt]);
+            }
+        }
+    }
+    if (valid) ag_store_row<DP>(a.dq + row * a.D, acc, a.scale, g, a.D);
+}
+
+// ---------------------------------------------------------------------------
+// Backward, dK and dV: 4 waves x 32 keys, 32 queries a step, over all query heads of the key head's group (so shared
+// heads' gradients are one fixed-order sum: no atomics).  S = Q . K^T, dP = dO . V^T (a lane owns one key),
+// dV^T += dO^T . P, dK^T += Q^T . dS.
+// ---------------------------------------------------------------------------
+template <int DP>
+__global__ __launch_bounds__(256) void ag_dkv_kernel(AgArgs a) {
+    constexpr int KS = DP / 16, DT = DP / 32, BQ = 32, BM = 128;
+    __shared__ __attribute__((aligned(16))) unsigned char Qimg[BQ * DP * 2];
+    __shared__ __attribute__((aligned(16))) unsigned char Gimg[BQ * DP * 2];
+    __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = ag_xcd(blockIdx.x, gridDim.x);
+    const int t = id % a.ntiles, hb = id / a.ntiles;                       // low keys are seen by the most queries
+    const int b = hb / a.Hk, hk = hb - b * a.Hk;
+    const int klen = ag_klen(a, b);
+    const int j = t * BM + wave * 32 + (lane & 31), jc = min(j, a.Sk - 1), jw = t * BM + wave * 32;
+    // first query that sees key j: i + 1 + Sk - Sq > j
+    const int off = a.Sk - a.Sq;
+    const int first = a.causal ? max(0, t * BM - off) : 0;
+    const int begin = first / BQ * BQ;
+    const int64_t go_ss = (int64_t)a.Hq * a.D;
+
+    s16x8 kf[KS], vf[KS];
+    ag_frags<DP>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
+    ag_frags<DP>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, a.D);
+    const bool seen = j < klen;
+    if (!seen) {                                       // padded keys: whatever they hold takes no part
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            kf[ks] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+            vf[ks] = kf[ks];
+        }
+    }
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        dk[dt] = ag_zero();
+        dv[dt] = ag_zero();
+    }
+    const int steps = t * BM < klen && begin < a.Sq ? (a.Sq - begin + BQ - 1) / BQ : 0, total = steps * a.group;
+    AgTile<DP, BQ, 256> qr, gr;
+    float lr = 0.f, dr = 0.f;
+    auto load = [&](int n) {
+        const int h = hk * a.group + n / steps, q0 = begin + n % steps * BQ;
+        qr.load(a.q + b * a.q_bs + h * a.q_hs, a.q_ss, q0, a.Sq, a.D, tid);
+        gr.load(a.dO + ((int64_t)b * a.Sq * a.Hq + h) * a.D, go_ss, q0, a.Sq, a.D, tid);
+        if (tid < BQ) {
+            const int64_t li = ((int64_t)b * a.Hq + h) * a.Sq + q0 + tid;
+            lr = q0 + tid < a.Sq ? a.lse[li] : __builtin_inff();
+            dr = q0 + tid < a.Sq ? a.dsum[li] : 0.f;
+        }
+    };
+    if (total > 0) load(0);
+    for (int n = 0; n < total; ++n) {
+        const int q0 = begin + n % steps * BQ;
+        __syncthreads();
+        qr.store(Qimg, tid);
+        gr.store(Gimg, tid);
+        if (tid < BQ) {
+            Ls[tid] = lr;
+            Ds[tid] = dr;
+        }
+        __syncthreads();
+        if (n + 1 < total) load(n + 1);
+        if (a.causal && q0 + BQ - 1 + off < jw) continue;                  // no query of the step sees this wave's keys
+        f32x16 s = ag_zero(), dp = ag_zero();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            s = ag_mfma(ag_row<DP>(Qimg, lane & 31, 2 * ks + g), kf[ks], s);
+            dp = ag_mfma(ag_row<DP>(Gimg, lane & 31, 2 * ks + g), vf[ks], dp);
+        }
+        const bool edge = (a.causal && q0 + off < jw + 31) || jw + 32 > klen;
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + 8 * rq + 4 * g);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(Ds + 8 * rq + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int x = 4 * rq + e;
+                float p = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale_log2e, -l4[e]));
+                if (edge) p = seen && (!a.causal || q0 + 8 * rq + 4 * g + e + off >= j) ? p : 0.f;
+                s[x] = p;
+                dp[x] = p * (dp[x] - d4[e]);
+            }
+        }
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {
+            const s16x8 pf = ag_pack(s, h2), df = ag_pack(dp, h2);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                dv[dt] = ag_mfma(ag_tr<DP>(Gimg, 16 * h2, 32 * dt, lane), pf, dv[dt]);
+                dk[dt] = ag_mfma(ag_tr<DP>(Qimg, 16 * h2, 32 * dt, lane), df, dk[dt]);
+            }
+        }
+    }
+    if (j < a.Sk) {
+        const int64_t o = (((int64_t)b * a.Sk + j) * a.Hk + hk) * a.D;
+        ag_store_row<DP>(a.dk + o, dk, a.scale, g, a.D);
+        ag_store_row<DP>(a.dv + o, dv, 1.f, g, a.D);
+    }
+}
+
+// ---------------------------------------------------------------------------
+static int ag_check(const AgArgs& a, const int64_t* st, int nst) {
+    if (a.B <= 0 || a.Sq <= 0 || a.Sk <= 0 || a.Hq <= 0 || a.Hk <= 0 || a.Hq % a.Hk) return -70;
+    if (a.D < 8 || a.D > 128 || a.D % 8) return -70;
+    for (int i = 0; i < nst; ++i)
+        if (st[i] & 7) return -17;
+    return 0;
+}
+
+static int ag_grid(int64_t n, int* out) {
+    if (n > 0x7fffffff) return -72;
+    *out = (int)n;
+    return 0;
+}
+
+extern "C" {
+
+// st: the nine element strides (batch, token, head) of q, k, v
+int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* st, int B, int Sq,
+                         int Sk, int Hq, int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
+    DTF_CLEAR_ERRORS();
+    AgArgs a{};
+    a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.out = (u16*)o; a.lse = lse;
+    a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
+    a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
+    a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
+    a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
+    int rc = ag_check(a, st, 9), grid = 0;
+    if (rc) return rc;
+    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o)) & 15) return -16;
+    a.group = Hq / Hk;
+    const bool pack = a.group > 1 && Sq < 128;         // a 128-row tile of one head would be part empty
+    const int64_t rows = pack ? (int64_t)a.group * Sq : Sq;
+    a.ntiles = (int)((rows + 127) / 128);
+    if ((rc = ag_grid((int64_t)B * (pack ? Hk : Hq) * a.ntiles, &grid))) return rc;
+    if (D > 64) {
+        if (pack) hipLaunchKernelGGL((ag_fwd_kernel<128, true>), dim3(grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((ag_fwd_kernel<128, false>), dim3(grid), dim3(256), 0, stream, a);
+    } else {
+        if (pack) hipLaunchKernelGGL((ag_fwd_kernel<64, true>), dim3(grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((ag_fwd_kernel<64, false>), dim3(grid), dim3(256), 0, stream, a);
+    }
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+// o, do_: contiguous [B, Sq, Hq, D]; dsum: workspace [B, Hq, Sq]; dq like o, dk / dv contiguous [B, Sk, Hk, D]
+int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
+                         float* dsum, void* dq, void* dk, void* dv, const int64_t* st, int B, int Sq, int Sk, int Hq, int Hk,
+                         int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
+    DTF_CLEAR_ERRORS();
+    AgArgs a{};
+    a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.o = (const u16*)o; a.dO = (const u16*)do_;
+    a.lse = const_cast<float*>(lse); a.dsum = dsum; a.dq = (u16*)dq; a.dk = (u16*)dk; a.dv = (u16*)dv;
+    a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
+    a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
+    a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
+    a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
+    int rc = ag_check(a, st, 9), grid = 0;
+    if (rc) return rc;
+    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)do_) | ((uintptr_t)dq) |
+         ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) return -16;
+    a.group = Hq / Hk;
+    a.ntiles = (Sq - 1) / 128 + 1;
+    if ((rc = ag_grid((int64_t)B * Hq * a.ntiles, &grid))) return rc;
+    if (D > 64) hipLaunchKernelGGL((ag_dq_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((ag_dq_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
+    DTF_CHECK_LAUNCH();
+    a.ntiles = (Sk - 1) / 128 + 1;
+    if ((rc = ag_grid((int64_t)B * Hk * a.ntiles, &grid))) return rc;
+    if (D > 64) hipLaunchKernelGGL((ag_dkv_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((ag_dkv_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,483 @@
+// K24: the boundary between two transformer blocks in one pass (bf16 / fp32 activations):
+//
+//   n = post(h)   r = x + scale * gate * n   y = pre(r)        post, gate optional; h absent: y = pre(x)
+//
+// post and pre are RMS norms  v / sqrt(mean(v^2) + eps) * w  or layer norms  (v - mean) / sqrt(var + eps) * w + b.
+// The gate is one row per `rpg` rows of x (1: per element, S: per sequence, M: per channel).
+//
+// Forward: a row is held in the registers of TPR threads between its two norms, so x and h are read and r and y written
+// once.  y is the norm of the unrounded r.  Backward recomputes n and r from x and h (the same bytes as reading r, and no
+// rounding in between):
+//   dr = dr_in + rstd (a - rhat mean(a rhat) [- mean(a)]),  a = dy w;   dx = dr;   dn = scale gate dr;   dgate = scale n dr
+//   dh = rstd_h (c - hhat mean(c hhat) [- mean(c)]),  c = dn w_post
+// The sums over rows (dw, db, dgate of a shared gate) run in registers over a workgroup's rows, one fp32 partial row per
+// workgroup, and a second kernel adds the partials in a fixed order: no atomics.  Both directions are HBM-bound.
+#include "dtf_common.h"
+
+struct RnArgs {
+    const void *x, *h, *gate, *w, *b, *pw, *pb;
+    void *y, *r;
+    float* stats;                         // [4][M]: mean, rstd of pre; mean, rstd of post
+    const void *dy, *dr;                  // each may be null (no gradient arrives there)
+    void *dx, *dh, *dgate;                // dh null: not wanted (or equal to dx); dgate: per element only
+    float* part;                          // [parts][narr][H]
+    int64_t M, rpg;
+    int H, wdt, layer, nbx, narr;         // workgroup id = group * nbx + bx
+    int s_w, s_b, s_pw, s_pb, s_g;        // slot of each sum in a partial row, -1: none
+    int64_t group_rows;                   // rows of one group of workgroups (a shared gate's rows, or M)
+    float scale, eps;
+};
+
+// element e of thread l's share of a row: vectors of V when rows allow 16-B access, else every TPR-th element
+template <int DT, bool VEC, int TPR, int NE>
+struct RnRow {
+    static constexpr int V = DT == DTF_BF16 ? 8 : 4;
+    static __device__ __forceinline__ int col(int l, int e) { return VEC ? ((e / V) * TPR + l) * V + e % V : e * TPR + l; }
+    static __device__ __forceinline__ void load(const void* base, int64_t off, int H, int l, float (&v)[NE]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < NE / V; ++c) {
+                const int at = (c * TPR + l) * V;
+                u32x4 q = {0u, 0u, 0u, 0u};
+                if (at < H) q = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + (off + at) * (16 / V));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == DTF_BF16) {
+                        v[c * V + 2 * k] = __uint_as_float(q[k] << 16);
+                        v[c * V + 2 * k + 1] = __uint_as_float(q[k] & 0xffff0000u);
+                    } else v[c * V + k] = __uint_as_float(q[k]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) v[e] = e * TPR + l < H ? load1<DT>(base, off + e * TPR + l) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ void store(void* base, int64_t off, int H, int l, const float (&v)[NE]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < NE / V; ++c) {
+                const int at = (c * TPR + l) * V;
+                u32x4 q;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == DTF_BF16) q[k] = pack_bf16x2(v[c * V + 2 * k], v[c * V + 2 * k + 1]);
+                    else q[k] = __float_as_uint(v[c * V + k]);
+                }
+                if (at < H) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(base) + (off + at) * (16 / V)) = q;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+                if (e * TPR + l < H) store1<DT>(base, off + e * TPR + l, v[e]);
+        }
+    }
+    // a parameter row of type wdt (the activations' type or fp32); absent: `missing`
+    static __device__ __forceinline__ void param(const void* p, int wdt, int H, int l, float missing, float (&v)[NE]) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = missing;
+        if (!p) return;
+        if (wdt == DT) load(p, 0, H, l, v);
+        else {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) v[e] = col(l, e) < H ? reinterpret_cast<const float*>(p)[col(l, e)] : 0.f;
+        }
+    }
+};
+
+// sums of a and b over the TPR threads of a row; `red` alternates between two halves, one barrier a call
+template <int TPR>
+__device__ __forceinline__ void rn_sum2(float& a, float& b, float (*red)[2][16], int& flip) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (TPR > 64) {
+        const int wave = threadIdx.x >> 6, w0 = wave & ~(TPR / 64 - 1);
+        if ((threadIdx.x & 63) == 0) {
+            red[flip][0][wave] = a;
+            red[flip][1][wave] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) {
+            a += red[flip][0][w0 + i];
+            b += red[flip][1][w0 + i];
+        }
+        flip ^= 1;
+    }
+}
+
+// v -> (v - mean) * rstd in place; columns past H stay 0
+template <class R, int TPR, int NE>
+__device__ __forceinline__ void rn_normalise(float (&v)[NE], int H, int l, float eps, int layer, float (*red)[2][16], int& flip,
+                                             float& mean, float& rstd) {
+    const float inv = 1.f / (float)H;
+    float s = 0.f, z = 0.f;
+    mean = 0.f;
+    if (layer) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) s += v[e];
+        rn_sum2<TPR>(s, z, red, flip);
+        mean = s * inv;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = R::col(l, e) < H ? v[e] - mean : 0.f;
+    }
+    s = z = 0.f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s = fmaf(v[e], v[e], s);
+    rn_sum2<TPR>(s, z, red, flip);
+    rstd = 1.f / sqrtf(s * inv + eps);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) v[e] *= rstd;
+}
+
+template <int DT, bool VEC, int TPR, int NE>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(RnArgs a) {
+    typedef RnRow<DT, VEC, TPR, NE> R;
+    constexpr int RB = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[2][2][16];
+    const int l = threadIdx.x % TPR, H = a.H;
+    const int64_t want = (int64_t)blockIdx.x * RB + threadIdx.x / TPR;
+    const int64_t row = want < a.M ? want : a.M - 1;           // spare rows of the last workgroup redo its last, unstored
+    int flip = 0;
+    float v[NE], p[NE], mean, rstd;
+    R::load(a.x, row * H, H, l, v);
+    if (a.h) {
+        float n[NE];
+        R::load(a.h, row * H, H, l, n);
+        if (a.pw) {
+            rn_normalise<R, TPR, NE>(n, H, l, a.eps, a.layer, red, flip, mean, rstd);
+            if (l == 0 && want < a.M) {
+                a.stats[2 * a.M + row] = mean;
+                a.stats[3 * a.M + row] = rstd;
+            }
+            R::param(a.pw, a.wdt, H, l, 1.f, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) n[e] *= p[e];
+            if (a.pb) {
+                R::param(a.pb, a.wdt, H, l, 0.f, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) n[e] += p[e];
+            }
+        }
+        if (a.gate) {
+            R::load(a.gate, row / a.rpg * H, H, l, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) n[e] *= p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, n[e], v[e]);
+        if (want < a.M) R::store(a.r, row * H, H, l, v);
+    }
+    rn_normalise<R, TPR, NE>(v, H, l, a.eps, a.layer, red, flip, mean, rstd);
+    if (l == 0 && want < a.M) {
+        a.stats[row] = mean;
+        a.stats[a.M + row] = rstd;
+    }
+    R::param(a.w, a.wdt, H, l, 1.f, p);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) v[e] *= p[e];
+    if (a.b) {
+        R::param(a.b, a.wdt, H, l, 0.f, p);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] += p[e];
+    }
+    if (want < a.M) R::store(a.y, row * H, H, l, v);
+}
+
+template <int DT, bool VEC, int TPR, int NE, bool LAYER>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a) {
+    typedef RnRow<DT, VEC, TPR, NE> R;
+    constexpr int NT = TPR < 256 ? 256 : TPR, RB = NT / TPR;
+    __shared__ float red[2][2][16];
+    __shared__ float comb[RB > 1 ? NT * NE : 1];
+    const int l = threadIdx.x % TPR, slot = threadIdx.x / TPR, H = a.H;
+    const int64_t group = blockIdx.x / a.nbx;
+    const int bx = blockIdx.x - (int)group * a.nbx;
+    const int64_t r0 = group * a.group_rows;
+    const int64_t r1 = r0 + a.group_rows < a.M ? r0 + a.group_rows : a.M;
+    const float inv = 1.f / (float)H;
+    int flip = 0;
+    float sw[NE], sb[LAYER ? NE : 1], spw[NE], spb[LAYER ? NE : 1], sg[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) sw[e] = spw[e] = sg[e] = 0.f;
+    if constexpr (LAYER) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) sb[e] = spb[e] = 0.f;
+    }
+    for (int64_t base = r0 + (int64_t)bx * RB; base < r1; base += (int64_t)a.nbx * RB) {     // (uniform in the workgroup)
+        const bool valid = base + slot < r1;
+        const int64_t row = valid ? base + slot : r1 - 1;
+        const float live = valid ? 1.f : 0.f;
+        float v[NE], n[NE], dr[NE], t[NE], p[NE];
+        R::load(a.x, row * H, H, l, v);
+        const float mean = LAYER ? a.stats[row] : 0.f, rstd = a.stats[a.M + row];
+        float pmean = 0.f, prstd = 1.f;
+        if (a.h) {
+            R::load(a.h, row * H, H, l, n);                    // n: hhat with a post norm, h without
+            if (a.pw) {
+                if (LAYER) pmean = a.stats[2 * a.M + row];
+                prstd = a.stats[3 * a.M + row];
+#pragma unroll
+                for (int e = 0; e < NE; ++e) n[e] = R::col(l, e) < H ? (n[e] - pmean) * prstd : 0.f;
+                R::param(a.pw, a.wdt, H, l, 1.f, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) t[e] = n[e] * p[e];
+                if (a.pb) {
+                    R::param(a.pb, a.wdt, H, l, 0.f, p);
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) t[e] += p[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) t[e] = n[e];
+            }
+            if (a.gate) {
+                R::load(a.gate, row / a.rpg * H, H, l, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, t[e] * p[e], v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, t[e], v[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            v[e] = R::col(l, e) < H ? (v[e] - mean) * rstd : 0.f;        // rhat
+            dr[e] = 0.f;
+        }
+        if (a.dr) R::load(a.dr, row * H, H, l, dr);
+        if (a.dy) {
+            float dy[NE], c1 = 0.f, c2 = 0.f;
+            R::load(a.dy, row * H, H, l, dy);
+            R::param(a.w, a.wdt, H, l, 1.f, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                sw[e] = fmaf(live * dy[e], v[e], sw[e]);
+                if constexpr (LAYER) sb[e] = fmaf(live, dy[e], sb[e]);
+                dy[e] *= p[e];
+                c1 = fmaf(dy[e], v[e], c1);
+                if constexpr (LAYER) c2 += dy[e];
+            }
+            rn_sum2<TPR>(c1, c2, red, flip);
+            c1 *= inv;
+            c2 *= inv;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) dr[e] = fmaf(rstd, dy[e] - v[e] * c1 - c2, dr[e]);
+        }
+        if (valid) R::store(a.dx, row * H, H, l, dr);
+        if (!a.h) continue;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) dr[e] *= a.scale;
+        if (a.gate) {
+            // t: n of the forward; p: gate (both again, after the registers served dy)
+#pragma unroll
+            for (int e = 0; e < NE; ++e) t[e] *= dr[e];
+            if (a.dgate) {
+                if (valid) R::store(a.dgate, row * H, H, l, t);
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) sg[e] = fmaf(live, t[e], sg[e]);
+            }
+            R::load(a.gate, row / a.rpg * H, H, l, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) dr[e] *= p[e];                  // dn
+        }
+        if (a.pw) {
+            float c1 = 0.f, c2 = 0.f;
+            R::param(a.pw, a.wdt, H, l, 1.f, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                if (R::col(l, e) >= H) dr[e] = 0.f;
+                spw[e] = fmaf(live * dr[e], n[e], spw[e]);
+                if constexpr (LAYER) spb[e] = fmaf(live, dr[e], spb[e]);
+                dr[e] *= p[e];
+                c1 = fmaf(dr[e], n[e], c1);
+                if constexpr (LAYER) c2 += dr[e];
+            }
+            rn_sum2<TPR>(c1, c2, red, flip);
+            c1 *= inv;
+            c2 *= inv;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) dr[e] = prstd * (dr[e] - n[e] * c1 - c2);
+        }
+        if (a.dh && valid) R::store(a.dh, row * H, H, l, dr);
+    }
+    float* out = a.part + (int64_t)blockIdx.x * a.narr * H;
+    auto flush = [&](const float* s, int at) {
+        if (at < 0) return;
+        if constexpr (RB > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < NE; ++e) comb[(slot * NE + e) * TPR + l] = s[e];
+            __syncthreads();
+            if (slot == 0) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    float z = 0.f;
+#pragma unroll
+                    for (int k = 0; k < RB; ++k) z += comb[(k * NE + e) * TPR + l];
+                    if (R::col(l, e) < H) out[(int64_t)at * H + R::col(l, e)] = z;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+                if (R::col(l, e) < H) out[(int64_t)at * H + R::col(l, e)] = s[e];
+        }
+    };
+    flush(sw, a.s_w);
+    if constexpr (LAYER) flush(sb, a.s_b);
+    flush(spw, a.s_pw);
+    if constexpr (LAYER) flush(spb, a.s_pb);
+    flush(sg, a.s_g);
+}
+
+struct RnSumArgs {
+    const float* part;
+    void* out[5];
+    int dt[5];
+    int64_t first[5], count[5], parts[5];   // slot, output rows, partial rows summed into each output row
+    int n, H, narr;
+};
+
+// one output row (a parameter's gradient, or one row of a shared gate's) per blockIdx.y: 64 columns, 16 waves share the parts
+__global__ __launch_bounds__(1024) void rn_sum_kernel(RnSumArgs a) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = a.H;
+    const int nc = (H + 63) / 64, c = (int)(blockIdx.x % nc) * 64 + lane;
+    int64_t o = blockIdx.x / nc;
+    int k = 0;
+    while (k < a.n - 1 && o >= a.count[k]) o -= a.count[k++];
+    const int64_t parts = a.parts[k];
+    const float* p = a.part + (o * parts * a.narr + a.first[k]) * H + c;
+    float s = 0.f;
+    if (c < H) {
+#pragma unroll 8
+        for (int64_t i = wave; i < parts; i += 16) s += p[i * a.narr * H];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < H) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += red[i][lane];
+        if (a.dt[k] == DTF_BF16) store1<DTF_BF16>(a.out[k], o * H + c, s);
+        else store1<DTF_F32>(a.out[k], o * H + c, s);
+    }
+}
+
+static int rn_tpr(int H) { return H <= 1024 ? 64 : H <= 2048 ? 128 : H <= 4096 ? 256 : H <= 8192 ? 512 : 1024; }
+
+static int rn_blocks(int64_t rows, int H, int64_t groups) {
+    const int tpr = rn_tpr(H), rb = tpr < 256 ? 256 / tpr : 1;
+    const int64_t target = tpr <= 256 ? 512 : 256;
+    int64_t n = target / groups, most = (rows + rb - 1) / rb;
+    if (n > most) n = most;
+    return n < 1 ? 1 : (int)n;
+}
+
+extern "C" {
+
+// fp32 workspace of the backward: groups = rows of a shared gate (1 without)
+int64_t dtf_residual_norm_ws(int64_t M, int H, int64_t groups, int narr) {
+    return groups * rn_blocks((M + groups - 1) / groups, H, groups) * narr * H;
+}
+
+#define RN_BY_SHAPE(X, DTY, VECT)                                                                 \
+    if (H <= 512) { X(DTY, VECT, 64, 8) } else if (H <= 1024) { X(DTY, VECT, 64, 16) }            \
+    else if (H <= 2048) { X(DTY, VECT, 128, 16) } else if (H <= 4096) { X(DTY, VECT, 256, 16) }   \
+    else if (H <= 8192) { X(DTY, VECT, 512, 16) } else { X(DTY, VECT, 1024, 16) }
+#define RN_DISPATCH(X)                                                        \
+    if (dt == DTF_BF16) {                                                     \
+        if (vec) { RN_BY_SHAPE(X, DTF_BF16, true) } else { RN_BY_SHAPE(X, DTF_BF16, false) } \
+    } else {                                                                  \
+        if (vec) { RN_BY_SHAPE(X, DTF_F32, true) } else { RN_BY_SHAPE(X, DTF_F32, false) }   \
+    }
+
+static int rn_check(int dt, int wdt, int64_t M, int H, int64_t rpg) {
+    if (dt != DTF_F32 && dt != DTF_BF16) return -90;
+    if (wdt != dt && wdt != DTF_F32) return -90;
+    if (M <= 0 || H <= 0 || H > 16384 || rpg <= 0) return -91;
+    return 0;
+}
+
+// rows [M, H] contiguous; gate [M / rpg, H] or null; w, b, pw, pb of type wdt (dt or fp32)
+int dtf_residual_norm_fwd(const void* x, const void* h, const void* gate, const void* w, const void* b, const void* pw,
+                          const void* pb, void* y, void* r, float* stats, int dt, int wdt, int layer, int64_t M, int H,
+                          int64_t rpg, float scale, float eps, hipStream_t stream) {
+    DTF_CLEAR_ERRORS();
+    int rc = rn_check(dt, wdt, M, H, rpg);
+    if (rc) return rc;
+    RnArgs a{};
+    a.x = x; a.h = h; a.gate = gate; a.w = w; a.b = b; a.pw = pw; a.pb = pb; a.y = y; a.r = r; a.stats = stats;
+    a.M = M; a.rpg = rpg; a.H = H; a.wdt = wdt; a.layer = layer; a.scale = scale; a.eps = eps;
+    const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)b | (uintptr_t)pw |
+                         (uintptr_t)pb | (uintptr_t)y | (uintptr_t)r;
+    const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
+    const int tpr = rn_tpr(H), nt = tpr < 256 ? 256 : tpr, rb = nt / tpr;
+    const int64_t grid = (M + rb - 1) / rb;
+    if (grid > 0x7fffffff) return -92;
+#define RN_FWD(DTY, VECT, TPR, NE) \
+    hipLaunchKernelGGL((rn_fwd_kernel<DTY, VECT, TPR, NE>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
+    RN_DISPATCH(RN_FWD)
+#undef RN_FWD
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+// dgate [M, H] for a gate per element, else [M / rpg, H] through the partials; dw, db, dpw, dpb of type wdt; any of them
+// null where there is no such operand.  ws: dtf_residual_norm_ws(M, H, groups, narr) floats, groups = M / rpg for a shared
+// gate and 1 otherwise, narr = number of sums (dw, db, dpw, dpb, dgate of a shared gate).
+int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const void* w, const void* pw, const void* pb,
+                          const float* stats, const void* dy, const void* dr, void* dx, void* dh, void* dgate, void* dw,
+                          void* db, void* dpw, void* dpb, float* ws, int dt, int wdt, int layer, int64_t M, int H, int64_t rpg,
+                          float scale, hipStream_t stream) {
+    DTF_CLEAR_ERRORS();
+    int rc = rn_check(dt, wdt, M, H, rpg);
+    if (rc) return rc;
+    RnArgs a{};
+    a.x = x; a.h = h; a.gate = gate; a.w = w; a.pw = pw; a.pb = pb; a.stats = const_cast<float*>(stats); a.dy = dy; a.dr = dr;
+    a.dx = dx; a.dh = dh; a.part = ws; a.M = M; a.rpg = rpg; a.H = H; a.wdt = wdt; a.layer = layer; a.scale = scale;
+    const bool shared = gate && rpg > 1;
+    a.dgate = gate && !shared ? dgate : nullptr;
+    const int64_t groups = shared ? (M + rpg - 1) / rpg : 1;
+    a.group_rows = shared ? rpg : M;
+    a.nbx = rn_blocks((M + groups - 1) / groups, H, groups);
+    RnSumArgs s{};
+    auto sum = [&](void* out, int type, bool on, int64_t rows) {
+        if (!on || !out) return -1;
+        s.out[s.n] = out; s.dt[s.n] = type; s.first[s.n] = s.n; s.count[s.n] = rows;
+        s.parts[s.n] = rows > 1 ? a.nbx : groups * a.nbx;
+        return s.n++;
+    };
+    a.s_w = sum(dw, wdt, true, 1);
+    a.s_b = sum(db, wdt, layer, 1);
+    a.s_pw = sum(dpw, wdt, pw != nullptr, 1);
+    a.s_pb = sum(dpb, wdt, layer && pw, 1);
+    a.s_g = sum(dgate, dt, shared, groups);
+    a.narr = s.n;
+    const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)pw | (uintptr_t)pb |
+                         (uintptr_t)dy | (uintptr_t)dr | (uintptr_t)dx | (uintptr_t)dh | (uintptr_t)a.dgate;
+    const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
+    const int tpr = rn_tpr(H), nt = tpr < 256 ? 256 : tpr;
+    const int64_t grid = groups * a.nbx;
+    if (grid > 0x7fffffff) return -92;
+#define RN_BWD(DTY, VECT, TPR, NE)                                                                                              \
+    if (layer) hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, true>), dim3((unsigned)grid), dim3(nt), 0, stream, a);     \
+    else hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, false>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
+    RN_DISPATCH(RN_BWD)
+#undef RN_BWD
+    DTF_CHECK_LAUNCH();
+    if (s.n == 0) return 0;
+    s.part = ws; s.H = H; s.narr = s.n;
+    int64_t rows = 0;
+    for (int i = 0; i < s.n; ++i) rows += s.count[i];
+    rows *= (H + 63) / 64;
+    if (rows > 0x7fffffff) return -92;
+    hipLaunchKernelGGL(rn_sum_kernel, dim3((unsigned)rows), dim3(1024), 0, stream, s);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+}  // extern "C"

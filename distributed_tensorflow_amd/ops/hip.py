@@ -86,6 +86,28 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+class _OnDevice:
+    """Makes a tensor's device the current one for a launch (nothing happens where it is already)."""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.index != self.back:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.back:
+            torch.cuda.set_device(self.back)
+
+
+def on_device(t):
+    return _OnDevice(t.device.index)
+
+
 def check(rc, what):
     if rc != 0:
         if rc == -16:

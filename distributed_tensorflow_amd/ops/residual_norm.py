@@ -1,0 +1,180 @@
+"""The boundary between two transformer blocks in one pass (kernel K24, ``csrc/residual_norm_kernels.hip``):
+
+    n = post(h);   r = x + scale * gate * n;   y = pre(r)
+
+``x`` is the residual stream, ``h`` a block's output, ``post`` an optional norm behind the block, ``gate`` an optional factor
+per element, per sequence or per channel, ``pre`` the norm in front of the next block.  Norms are RMS norms or layer norms.
+bf16 or fp32, any width to 16384; parameters in the activations' type or fp32.  CPU tensors take
+:func:`residual_norm_reference`, the oracle of the kernel tests.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import hip
+
+MAX_WIDTH = 16384
+_fns = None
+
+
+def _kernels():
+    global _fns
+    if _fns is None:
+        P, I, L, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+        _fns = (hip.declare("dtf_residual_norm_fwd", [P] * 10 + [I, I, I, L, I, L, Fl, Fl, P]),
+                hip.declare("dtf_residual_norm_bwd", [P] * 17 + [I, I, I, L, I, L, Fl, P]),
+                hip.declare("dtf_residual_norm_ws", [L, I, L, I], L))
+    return _fns
+
+
+def _normed(v, weight, bias, kind, eps):
+    if kind == "layer":
+        v = v - v.mean(-1, keepdim=True)
+    v = v / torch.sqrt((v * v).mean(-1, keepdim=True) + eps) * weight.float()
+    return v if bias is None else v + bias.float()
+
+
+def residual_norm_reference(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=None, post_bias=None, kind="rms",
+                            eps=1e-6):
+    """The definition in elementary fp32 operations, rounded once at the end."""
+    n = h.float() if post_weight is None else _normed(h.float(), post_weight, post_bias, kind, eps)
+    r = x.float() + scale * (n if gate is None else n * gate.float())
+    return _normed(r, weight, bias, kind, eps).to(x.dtype), r.to(x.dtype)
+
+
+def _rows_per_gate(x, gate):
+    """Rows of x that share a row of the gate: the gate's leading dimensions are x's up to some axis and 1 from there on."""
+    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
+    if len(shape) == x.dim() and shape[-1] == x.shape[-1]:
+        lead = tuple(x.shape[:-1])
+        for cut in range(len(lead), -1, -1):
+            if shape[:-1] == lead[:cut] + (1,) * (len(lead) - cut):
+                rows = 1
+                for n in lead[cut:]:
+                    rows *= n
+                return rows
+    raise ValueError("residual_norm: a gate for x %s is x's own shape, or that with 1 for its last leading dimensions (one row a "
+                     "sequence), or [%d]; got %s" % (tuple(x.shape), x.shape[-1], tuple(gate.shape)))
+
+
+def _checked(x, h, weight, bias, gate, post_weight, post_bias, kind):
+    if kind not in ("rms", "layer"):
+        raise ValueError("residual_norm: kind is 'rms' or 'layer', got %r" % (kind,))
+    hip.dt(x)
+    if x.dim() < 1 or x.numel() == 0 or x.shape[-1] > MAX_WIDTH:
+        raise ValueError("residual_norm: x is [..., H] with 1 <= H <= %d and at least one row, got %s" % (MAX_WIDTH, tuple(x.shape)))
+    if h is not None and (h.shape != x.shape or h.dtype != x.dtype or h.device != x.device):
+        raise ValueError("residual_norm: h must match x in shape, dtype and device")
+    if gate is not None and (gate.dtype != x.dtype or gate.device != x.device):
+        raise ValueError("residual_norm: the gate must match x in dtype and device")
+    if post_bias is not None and post_weight is None:
+        raise ValueError("residual_norm: post_bias without post_weight")
+    if kind == "rms" and (bias is not None or post_bias is not None):
+        raise ValueError("residual_norm: an RMS norm has no bias")
+    for p in (weight, bias, post_weight, post_bias):
+        if p is None:
+            continue
+        if tuple(p.shape) != (x.shape[-1],) or p.device != x.device:
+            raise ValueError("residual_norm: parameters are [%d] on x's device, got %s" % (x.shape[-1], tuple(p.shape)))
+        if p.dtype not in (x.dtype, torch.float32) or p.dtype != weight.dtype:
+            raise ValueError("residual_norm: parameters share one dtype, x's or float32")
+    return None if gate is None else _rows_per_gate(x, gate)
+
+
+def _rows(t, H):
+    return None if t is None else t.reshape(-1, H).contiguous()
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, h, weight, bias, gate, post_weight, post_bias, rpg, scale, layer, eps):
+        H = x.shape[-1]
+        x2, h2, g2 = _rows(x, H), _rows(h, H), _rows(gate, H)
+        weight, bias, post_weight, post_bias = (None if p is None else p.contiguous() for p in (weight, bias, post_weight, post_bias))
+        M = x2.shape[0]
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        r = None if h is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty(4, M, dtype=torch.float32, device=x.device)
+        with hip.on_device(x):
+            rc = _kernels()[0](x2.data_ptr(), hip.ptr(h2), hip.ptr(g2), weight.data_ptr(), hip.ptr(bias), hip.ptr(post_weight),
+                               hip.ptr(post_bias), y.data_ptr(), hip.ptr(r), stats.data_ptr(), hip.dt(x), hip.dt(weight),
+                               int(layer), M, H, rpg, scale, eps, hip.stream())
+        hip.check(rc, "dtf_residual_norm_fwd")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x2, h2, g2, weight, bias, post_weight, post_bias, stats)
+        ctx.how = x.shape, None if gate is None else gate.shape, rpg, scale, layer
+        return y, r
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dr):
+        x2, h2, g2, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
+        shape, gate_shape, rpg, scale, layer = ctx.how
+        if dy is None and dr is None:
+            return (None,) * 11
+        M, H = x2.shape
+        dy2, dr2 = _rows(dy, H), _rows(dr, H)
+        dev = x2.device
+
+        def like(t):
+            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+
+        dx = torch.empty(shape, dtype=x2.dtype, device=dev)
+        same = post_weight is None and g2 is None and scale == 1.0        # then dh = dx, written once
+        dh = None if h2 is None or same else torch.empty(shape, dtype=x2.dtype, device=dev)
+        dgate, dw, db, dpw, dpb = like(g2), like(weight), like(bias), like(post_weight), like(post_bias)
+        shared = g2 is not None and rpg > 1
+        groups = g2.shape[0] if shared else 1
+        narr = sum(t is not None for t in (dw, db, dpw, dpb)) + int(shared)
+        fwd, bwd, ws_floats = _kernels()
+        ws = torch.empty(ws_floats(M, H, groups, narr), dtype=torch.float32, device=dev)
+        with hip.on_device(x2):
+            rc = bwd(x2.data_ptr(), hip.ptr(h2), hip.ptr(g2), weight.data_ptr(), hip.ptr(post_weight), hip.ptr(post_bias),
+                     stats.data_ptr(), hip.ptr(dy2), hip.ptr(dr2), dx.data_ptr(), hip.ptr(dh), hip.ptr(dgate), dw.data_ptr(),
+                     hip.ptr(db), hip.ptr(dpw), hip.ptr(dpb), ws.data_ptr(), hip.dt(x2), hip.dt(weight), int(layer), M, H, rpg,
+                     scale, hip.stream())
+        hip.check(rc, "dtf_residual_norm_bwd")
+        if h2 is not None and same:
+            dh = dx
+        return dx, dh, dw, db, None if dgate is None else dgate.view(gate_shape), dpw, dpb, None, None, None, None
+
+
+def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=None, post_bias=None, kind="rms", eps=1e-6):
+    """-> (y, r): ``r = x + scale * gate * post(h)`` and ``y = pre(r)``.  ``x``, ``h`` ``[..., H]``; ``weight`` / ``bias`` are
+    pre's, ``post_weight`` / ``post_bias`` post's (without ``post_weight``, h itself is added).  ``gate``: x's shape, or
+    ``[B, 1, H]`` (one row a sequence), or ``[H]``; its gradient is summed over the rows that share it.  ``kind``: ``"rms"``, or
+    ``"layer"`` (biases optional).  y is the norm of r before r is rounded to x's type."""
+    rpg = _checked(x, h, weight, bias, gate, post_weight, post_bias, kind)
+    if h is None:
+        raise ValueError("residual_norm: h is missing (rms_norm has no residual)")
+    scale, eps = float(scale), float(eps)
+    if not x.is_cuda:
+        return residual_norm_reference(x, h, weight, bias, gate=gate, scale=scale, post_weight=post_weight, post_bias=post_bias,
+                                       kind=kind, eps=eps)
+    return _ResidualNorm.apply(x, h, weight, bias, gate, post_weight, post_bias, rpg or 1, scale, kind == "layer", eps)
+
+
+def rms_norm(x, weight, eps=1e-6):
+    """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension: the norm in front of a first block."""
+    _checked(x, None, weight, None, None, None, None, "rms")
+    if not x.is_cuda:
+        return _normed(x.float(), weight, None, "rms", eps).to(x.dtype)
+    return _ResidualNorm.apply(x, None, weight, None, None, None, None, 1, 1.0, False, float(eps))[0]
+
+
+class FusedRMSNorm(nn.Module):
+    """RMS norm over the last dimension.  ``norm(x)``, or ``norm(x, h, ...)`` -> (y, r) for the boundary between two blocks."""
+
+    def __init__(self, hidden, eps=1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(hidden))
+        self.eps = eps
+
+    def forward(self, x, h=None, **kw):
+        if h is None:
+            return rms_norm(x, self.weight, self.eps)
+        return residual_norm(x, h, self.weight, eps=self.eps, **kw)

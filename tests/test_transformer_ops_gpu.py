@@ -1,0 +1,276 @@
+"""The transformer-block kernels (K22 attention of any length, K23 rotary positions, K24 block boundary) against their
+definitions in 64 bits, with tolerances derived in ``transformer_oracles``."""
+import pytest
+import torch
+
+import transformer_oracles as oracle
+
+pytestmark = pytest.mark.gpu
+
+from distributed_tensorflow_amd.ops import hip  # noqa: E402
+from distributed_tensorflow_amd.ops.attention import attention  # noqa: E402
+from distributed_tensorflow_amd.ops.residual_norm import FusedRMSNorm, residual_norm, rms_norm  # noqa: E402
+from distributed_tensorflow_amd.ops.rotary import rotary, rotary_frequencies  # noqa: E402
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a visible MI355X"
+    hip.lib()
+    return torch.device("cuda", 0)
+
+
+def _randn(dev, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return lambda *s: torch.randn(*s, generator=g, device=dev)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+ATT = [
+    # B, Sq, Sk, Hq, Hk, D, causal, lens
+    (1, 1, 1, 1, 1, 64, False, None), (2, 1, 1, 2, 1, 128, True, None), (1, 2, 2, 3, 3, 64, True, None),
+    (2, 37, 37, 12, 12, 64, False, (18, 37)), (3, 33, 33, 4, 2, 64, True, (0, 1, 33)),
+    (1, 64, 64, 2, 2, 128, True, None), (1, 65, 65, 2, 1, 128, True, None), (2, 129, 129, 4, 1, 64, True, (129, 70)),
+    (1, 300, 300, 2, 2, 80, True, None), (1, 257, 257, 6, 2, 96, False, (200,)), (1, 200, 200, 1, 1, 8, True, None),
+    (1, 130, 130, 2, 2, 32, False, None), (1, 1000, 1000, 2, 1, 64, True, None), (1, 640, 640, 5, 1, 128, True, (513,)),
+    # queries and keys of different lengths; causal ones end together; the third leaves 60 rows empty
+    (2, 1, 300, 8, 2, 128, False, (300, 5)), (2, 7, 515, 8, 1, 128, True, None), (1, 100, 40, 2, 2, 64, True, None),
+    (2, 140, 1, 3, 1, 64, True, None), (1, 257, 1100, 4, 4, 64, True, (900,)), (4, 1, 129, 4, 4, 64, False, (0, 1, 64, 129)),
+    (1, 31, 2000, 40, 8, 128, True, None), (1, 513, 65, 2, 1, 128, False, None),
+]
+
+
+def _att_inputs(dev, B, Sq, Sk, Hq, Hk, D, packed):
+    r = _randn(dev, Sq * 1000 + Sk + D)
+    if packed and Sq == Sk:
+        q, k, v = r(B, Sq, Hq + 2 * Hk, D).to(BF).split([Hq, Hk, Hk], 2)
+    else:
+        q, k, v = r(B, Sq, Hq, D).to(BF), r(B, Sk, Hk, D).to(BF), r(B, Sk, Hk, D).to(BF)
+    return q, k, v, r(B, Sq, Hq, D).to(BF)
+
+
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D,causal,lens", ATT)
+def test_attention_matches_the_definition(dev, B, Sq, Sk, Hq, Hk, D, causal, lens):
+    q, k, v, do = _att_inputs(dev, B, Sq, Sk, Hq, Hk, D, True)
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*leaves, causal=causal, kv_len=n)
+    grads = torch.autograd.grad(out, leaves, do)
+    want, tol = oracle.attention(q, k, v, do, causal, lens)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+        oracle.close(got.detach(), want[name], tol[name], name)
+    again = attention(q, k, v, causal=causal, kv_len=n)
+    assert torch.equal(again, out)                                     # without gradients, and again: the same bits
+    if Sk == 1:
+        assert not grads[0].any() and not grads[1].any()               # one key: the probabilities are constant
+
+
+@pytest.mark.parametrize("scale", [0.01, 1.0])
+def test_attention_scale_and_large_scores(dev, scale):
+    q, k, v, do = _att_inputs(dev, 1, 150, 150, 2, 2, 64, False)
+    q = (q.float() * 8).to(BF)                                         # scores of standard deviation 64 at scale 1
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*leaves, causal=True, scale=scale)
+    grads = torch.autograd.grad(out, leaves, do)
+    want, tol = oracle.attention(q, k, v, do, True, scale=scale)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+        oracle.close(got.detach(), want[name], tol[name], name)
+
+
+def test_attention_padding_is_never_read(dev):
+    B, S, H, D = 3, 200, 2, 64
+    q, k, v, do = _att_inputs(dev, B, S, S, H, H, D, False)
+    lens = (200, 77, 0)
+    n = torch.tensor(lens, dtype=torch.int64, device=dev)
+    got = []
+    for poison in (0.0, float("nan"), float("inf")):
+        kk, vv = k.clone(), v.clone()
+        for b, m in enumerate(lens):
+            kk[b, m:], vv[b, m:] = poison, poison
+        leaves = [t.detach().requires_grad_() for t in (q, kk, vv)]
+        out = attention(*leaves, kv_len=n)
+        got.append((out.detach(),) + torch.autograd.grad(out, leaves, do))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+    assert not got[0][0][2].any() and not got[0][1][2].any()            # no key: zeros, and no gradient
+    for g in got[0][2:]:
+        for b, m in enumerate(lens):
+            assert not g[b, m:].any()
+
+
+def test_attention_key_lengths_outside_the_range(dev):
+    q, k, v, _ = _att_inputs(dev, 3, 70, 70, 2, 2, 64, False)
+    a = attention(q, k, v, kv_len=torch.tensor([-5, 70, 2 ** 40], device=dev))
+    b = attention(q, k, v, kv_len=torch.tensor([0, 70, 70], dtype=torch.int32))
+    c = attention(q, k, v, kv_len=torch.tensor([-1, 1000, 70], dtype=torch.int32, device=dev))
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_attention_other_strides_and_orders(dev):
+    B, S, H, D = 2, 90, 4, 64
+    q, k, v, do = _att_inputs(dev, B, S, S, H, H, D, False)
+    plain = attention(q, k, v, causal=True)
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]              # [B, H, S, D] memory
+    assert torch.equal(attention(*heads_first, causal=True), plain)
+    last = [t.transpose(2, 3).contiguous().transpose(2, 3) for t in (q, k, v)]                     # D not dense: copied
+    assert torch.equal(attention(*last, causal=True), plain)
+    odd = [torch.cat([t.new_zeros(3), t.reshape(-1)])[3:].view(t.shape) for t in (q, k, v)]        # not 16-B aligned: copied
+    assert torch.equal(attention(*odd, causal=True), plain)
+    one = k[:, :, :1].expand(B, S, H, D)                                                           # a broadcast key head
+    leaf = k[:, :, :1].detach().clone().requires_grad_()
+    out = attention(q, leaf.expand(B, S, H, D), v, causal=True)
+    assert torch.equal(out, attention(q, one.contiguous(), v, causal=True))
+    dk, = torch.autograd.grad(out, leaf, do)
+    full = one.contiguous().requires_grad_()
+    want, = torch.autograd.grad(attention(q, full, v, causal=True), full, do)
+    assert torch.equal(dk, want.sum(2, keepdim=True))
+    wide = q.detach().requires_grad_()
+    g1, = torch.autograd.grad(attention(wide, k, v).sum(), wide)                                   # an expanded gradient
+    g2, = torch.autograd.grad(attention(wide, k, v), wide, torch.ones_like(q))
+    assert torch.equal(g1, g2)
+
+
+def test_attention_nan_reaches_its_query(dev):
+    q, k, v, _ = _att_inputs(dev, 1, 70, 70, 1, 1, 64, False)
+    clean = attention(q, k, v, causal=True)
+    q[0, 40, 0, 3] = float("nan")
+    out = attention(q, k, v, causal=True)
+    assert bool(out[0, 40].isnan().all())
+    keep = [i for i in range(70) if i != 40]
+    assert torch.equal(out[:, keep], clean[:, keep])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# rotary
+# ---------------------------------------------------------------------------------------------------------------------
+ROT = [
+    # B, S, Hq, Hk, D, pairs, dtype
+    (1, 1, 1, 1, 2, 1, F32), (8, 1, 32, 8, 128, 64, BF), (2, 37, 12, 12, 64, 32, BF), (3, 50, 4, 2, 96, 32, F32),
+    (2, 33, 3, 1, 128, 7, BF), (1, 129, 2, 2, 80, 40, BF), (1, 65, 2, 1, 64, 8, BF), (2, 17, 5, 5, 10, 3, F32), (1, 300, 40, 8, 128, 64, BF),
+    (1, 70, 2, 1, 256, 128, F32), (2, 19, 2, 2, 2048, 1024, BF), (1, 21, 4, 4, 128, 38, BF),
+]
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,S,Hq,Hk,D,m,dt", ROT)
+def test_rotary_matches_the_definition(dev, B, S, Hq, Hk, D, m, dt, interleaved):
+    r = _randn(dev, S * 100 + D)
+    q, k, _ = r(B, S, Hq + 2 * Hk, D).to(dt).split([Hq, Hk, Hk], 2)
+    gq, gk = r(B, S, Hq, D).to(dt), r(B, S, Hk, D).to(dt)
+    f, amp = rotary_frequencies(2 * m, scaling="by_parts", factor=4.0, original_length=2048, device=dev)
+    pos = torch.randint(0, 1 << 20, (B, 1), device=dev, generator=torch.Generator(dev).manual_seed(S)) + torch.arange(S, device=dev)
+    leaves = [t.detach().requires_grad_() for t in (q, k)]
+    outs = rotary(*leaves, f, pos, interleaved=interleaved, amplitude=amp)
+    grads = torch.autograd.grad(outs, leaves, (gq, gk))
+    for name, x, got, inv in (("q", q, outs[0], False), ("k", k, outs[1], False), ("dq", gq, grads[0], True), ("dk", gk, grads[1], True)):
+        want, tol = oracle.rotary(x, f, pos, interleaved, amp, inv)
+        oracle.close(got.detach(), want, tol, name)
+    assert torch.equal(outs[0][..., 2 * m:], q[..., 2 * m:]) and torch.equal(grads[1][..., 2 * m:], gk[..., 2 * m:])
+
+
+def test_rotary_positions(dev):
+    r = _randn(dev, 5)
+    q, k = r(2, 40, 4, 64).to(BF), r(2, 40, 2, 64).to(BF)
+    f, _ = rotary_frequencies(64, device=dev)
+    at = torch.arange(40, device=dev)
+    base = rotary(q, k, f, offset=7)
+    for pos in (at + 7, (at + 7).int(), (at + 7).expand(2, 40), (at + 7)[None], torch.stack([at + 7, at + 7], 1).t()):
+        for a, b in zip(base, rotary(q, k, f, pos)):
+            assert torch.equal(a, b)
+    alone = rotary(q, None, f, offset=7)
+    assert alone[1] is None and torch.equal(alone[0], base[0])
+    zero = rotary(q, k, f, torch.zeros(40, dtype=torch.int64, device=dev))
+    assert torch.equal(zero[0], q) and torch.equal(zero[1], k)
+    far = torch.tensor([[-3, 0, 1 << 40, 2 ** 31 + 11]], device=dev)                  # negative, and past 32 bits
+    y, _ = rotary(q[:1, :4].float(), None, f, far)
+    want, tol = oracle.rotary(q[:1, :4].float(), f, far, False, 1.0)
+    # (position 2^40: position * frequency carries 2^40 * 2^-53 = 1.3e-4 in the angle, on both sides)
+    oracle.close(y, want, tol + 2 * 2 ** -13 * torch.tensor([0, 0, 1.0, 0], device=dev).view(1, 4, 1, 1) * q[:1, :4].abs().amax() * 2, "far")
+    leaf = q.detach().requires_grad_()
+    g, = torch.autograd.grad(rotary(leaf, None, f, offset=7)[0].sum(), leaf)          # an expanded gradient
+    assert torch.equal(g, rotary(torch.ones_like(q), None, f, -(at + 7))[0])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# block boundary
+# ---------------------------------------------------------------------------------------------------------------------
+NORM = [
+    # shape, kind, post, gate, scale, dtype, parameter dtype
+    ((1, 1, 1), "rms", False, "none", 1.0, F32, F32), ((8, 1, 4096), "rms", True, "none", 0.5, BF, BF),
+    ((2, 100, 768), "layer", False, "channel", 1.0, BF, BF), ((3, 37, 768), "layer", True, "sequence", 0.3, BF, F32),
+    ((2, 65, 1024), "rms", True, "full", 0.25, BF, BF), ((3, 33, 1001), "rms", False, "full", 0.7, F32, F32),
+    ((2, 20, 1001), "layer", True, "channel", 0.7, BF, BF), ((1, 50, 2000), "rms", True, "sequence", 1.0, BF, BF),
+    ((2, 9, 4100), "layer", True, "sequence", 2.0, F32, F32), ((1, 6, 8192), "rms", True, "channel", 0.1, BF, BF),
+    ((2, 3, 16384), "layer", True, "full", 0.1, BF, BF), ((2, 3, 16381), "layer", True, "sequence", 0.1, F32, F32),
+    ((5, 40, 16), "rms", False, "none", 1.0, BF, BF), ((3, 11, 520), "layer", True, "none", 1.0, F32, F32),
+    ((700, 128), "rms", True, "channel", 0.5, BF, BF), ((6, 3, 5, 256), "rms", True, "sequence", 0.5, BF, BF),
+    ((1500, 2, 64), "layer", False, "sequence", 1.0, BF, BF), ((2, 17, 5000), "rms", False, "channel", 1.0, BF, F32),
+]
+
+
+def _norm_inputs(dev, shape, kind, post, gate, dt, pdt):
+    r = _randn(dev, shape[-1] + len(shape))
+    H = shape[-1]
+    x, h = (r(*shape) * torch.exp(r(H))).to(dt), (r(*shape) * 1.5 + 0.3).to(dt)
+    w, b = (1 + 0.2 * r(H)).to(pdt), (0.1 * r(H)).to(pdt) if kind == "layer" else None
+    pw = (1 + 0.2 * r(H)).to(pdt) if post else None
+    pb = (0.1 * r(H)).to(pdt) if post and kind == "layer" else None
+    gs = {"none": None, "channel": (H,), "sequence": shape[:1] + (1,) * (len(shape) - 2) + (H,), "full": shape}[gate]
+    return dict(x=x, h=h, w=w, b=b, gate=None if gs is None else (0.3 + 0.5 * r(*gs)).to(dt), pw=pw, pb=pb), r(*shape).to(dt), (0.5 * r(*shape)).to(dt)
+
+
+@pytest.mark.parametrize("grads", ["both", "y", "r"])
+@pytest.mark.parametrize("shape,kind,post,gate,scale,dt,pdt", NORM)
+def test_residual_norm_matches_the_definition(dev, shape, kind, post, gate, scale, dt, pdt, grads):
+    t, dy, dr = _norm_inputs(dev, shape, kind, post, gate, dt, pdt)
+    leaf = {n: None if v is None else v.detach().requires_grad_() for n, v in t.items()}
+    y, r = residual_norm(leaf["x"], leaf["h"], leaf["w"], leaf["b"], gate=leaf["gate"], scale=scale, post_weight=leaf["pw"],
+                         post_bias=leaf["pb"], kind=kind)
+    dy, dr = dy if grads != "r" else None, dr if grads != "y" else None
+    names = [n for n, v in leaf.items() if v is not None]
+    outs = [(o, g) for o, g in ((y, dy), (r, dr)) if g is not None]
+    got = torch.autograd.grad([o for o, _ in outs], [leaf[n] for n in names], [g for _, g in outs], allow_unused=True)
+    want, tol = oracle.residual_norm(**t, scale=scale, kind=kind, dy=dy, dr=dr)
+    oracle.close(y.detach(), want["y"], tol["y"], "y")
+    oracle.close(r.detach(), want["r"], tol["r"], "r")
+    for n, g in zip(names, got):
+        if g is None:
+            assert grads == "r" and n in ("w", "b"), n
+            continue
+        assert g.dtype == leaf[n].dtype and g.shape == leaf[n].shape
+        oracle.close(g, want["d" + n], tol["d" + n], "d" + n)
+
+
+def test_rms_norm_and_module(dev):
+    r = _randn(dev, 3)
+    x, w, dy = r(3, 50, 768).to(BF), (1 + 0.2 * r(768)).to(BF), r(3, 50, 768).to(BF)
+    lx, lw = x.detach().requires_grad_(), w.detach().requires_grad_()
+    y = rms_norm(lx, lw, 1e-5)
+    dx, dw = torch.autograd.grad(y, (lx, lw), dy)
+    zero = torch.zeros_like(x)
+    want, tol = oracle.residual_norm(x, zero, w, dy=dy, eps=1e-5)
+    for n, got in (("y", y), ("dx", dx), ("dw", dw)):
+        oracle.close(got.detach(), want[n], tol[n], n)
+    m = FusedRMSNorm(768, eps=1e-5).to(dev, BF)
+    assert torch.equal(m(x), rms_norm(x, m.weight, 1e-5))
+    a, b = m(x, dy, scale=0.5), residual_norm(x, dy, m.weight, scale=0.5, eps=1e-5)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_residual_norm_unaligned_rows_equal_aligned_ones(dev):
+    t, dy, dr = _norm_inputs(dev, (2, 21, 768), "rms", True, "full", BF, BF)
+    res = []
+    for off in (0, 1):
+        v = {n: None if u is None else torch.cat([u.new_zeros(off), u.reshape(-1)])[off:].view(u.shape).requires_grad_() for n, u in t.items()}
+        y, r = residual_norm(v["x"], v["h"], v["w"], gate=v["gate"], scale=0.5, post_weight=v["pw"])
+        g = torch.autograd.grad((y, r), [u for u in v.values() if u is not None], (dy, dr))
+        res.append((y.detach(), r.detach()) + g)
+    want, tol = oracle.residual_norm(**t, scale=0.5, dy=dy, dr=dr)
+    for got in res:
+        for n, g in zip(("y", "r", "dx", "dh", "dw", "dgate", "dpw"), got):
+            oracle.close(g, want[n], tol[n], n)

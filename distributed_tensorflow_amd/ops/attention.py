@@ -17,7 +17,6 @@ import os
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -137,31 +136,23 @@ class _Attention(torch.autograd.Function):
         q, k, v = _operand(q), _operand(k), _operand(v)
         B, Sq, Hq, D = q.shape
         Sk, Hk = k.shape[1], k.shape[2]
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(B, Hq, Sq, dtype=torch.float32, device=q.device)
-        with hip.on_device(q):
-            rc = _general_kernels()[0](q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-                                       _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len),
-                                       hip.stream())
+        o = q.new_empty(q.shape)
+        lse = q.new_empty((B, Hq, Sq), dtype=torch.float32)
+        ctx.how = _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
+        rc = hip.launch(q, _general_kernels()[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), *ctx.how)
         hip.check(rc, "dtf_attn_general_fwd")
         ctx.save_for_backward(q, k, v, o, lse, kv_len)
-        ctx.how = causal, scale
         return o
 
     @staticmethod
-    @once_differentiable
+    @hip.first_order
     def backward(ctx, do):
-        q, k, v, o, lse, kv_len = ctx.saved_tensors
-        B, Sq, Hq, D = q.shape
-        Sk, Hk = k.shape[1], k.shape[2]
+        q, k, v, o, lse, _ = ctx.saved_tensors
         if not do.is_contiguous() or do.data_ptr() % 16:
             do = do.clone(memory_format=torch.contiguous_format)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dsum = torch.empty(B, Hq, Sq, dtype=torch.float32, device=q.device)
-        with hip.on_device(q):
-            rc = _general_kernels()[1](q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                                       dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _general_strides(q, k, v),
-                                       B, Sq, Sk, Hq, Hk, D, *ctx.how, hip.ptr(kv_len), hip.stream())
+        dq, dk, dv, dsum = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape), lse.new_empty(lse.shape)
+        rc = hip.launch(q, _general_kernels()[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(),
+                        lse.data_ptr(), dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ctx.how)
         hip.check(rc, "dtf_attn_general_bwd")
         return dq, dk, dv, None, None, None
 

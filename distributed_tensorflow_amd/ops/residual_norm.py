@@ -13,7 +13,6 @@ import ctypes
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -85,62 +84,52 @@ def _checked(x, h, weight, bias, gate, post_weight, post_bias, kind):
     return None if gate is None else _rows_per_gate(x, gate)
 
 
-def _rows(t, H):
-    return None if t is None else t.reshape(-1, H).contiguous()
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _like(t):
+    return None if t is None else t.new_empty(t.shape)
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, weight, bias, gate, post_weight, post_bias, rpg, scale, layer, eps):
+        x, h, weight, bias, gate, post_weight, post_bias = map(_dense, (x, h, weight, bias, gate, post_weight, post_bias))
         H = x.shape[-1]
-        x2, h2, g2 = _rows(x, H), _rows(h, H), _rows(gate, H)
-        weight, bias, post_weight, post_bias = (None if p is None else p.contiguous() for p in (weight, bias, post_weight, post_bias))
-        M = x2.shape[0]
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        r = None if h is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty(4, M, dtype=torch.float32, device=x.device)
-        with hip.on_device(x):
-            rc = _kernels()[0](x2.data_ptr(), hip.ptr(h2), hip.ptr(g2), weight.data_ptr(), hip.ptr(bias), hip.ptr(post_weight),
-                               hip.ptr(post_bias), y.data_ptr(), hip.ptr(r), stats.data_ptr(), hip.dt(x), hip.dt(weight),
-                               int(layer), M, H, rpg, scale, eps, hip.stream())
+        M = x.numel() // H
+        y, r = x.new_empty(x.shape), _like(h)
+        stats = x.new_empty(4 * M, dtype=torch.float32)
+        how = hip.dt(x), hip.dt(weight), layer, M, H, rpg, scale
+        rc = hip.launch(x, _kernels()[0], x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(bias),
+                        hip.ptr(post_weight), hip.ptr(post_bias), y.data_ptr(), hip.ptr(r), stats.data_ptr(), *how, eps)
         hip.check(rc, "dtf_residual_norm_fwd")
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x2, h2, g2, weight, bias, post_weight, post_bias, stats)
-        ctx.how = x.shape, None if gate is None else gate.shape, rpg, scale, layer
+        ctx.save_for_backward(x, h, weight, bias, gate, post_weight, post_bias, stats)
+        ctx.how = how
         return y, r
 
     @staticmethod
-    @once_differentiable
+    @hip.first_order
     def backward(ctx, dy, dr):
-        x2, h2, g2, weight, bias, post_weight, post_bias, stats = ctx.saved_tensors
-        shape, gate_shape, rpg, scale, layer = ctx.how
         if dy is None and dr is None:
             return (None,) * 11
-        M, H = x2.shape
-        dy2, dr2 = _rows(dy, H), _rows(dr, H)
-        dev = x2.device
-
-        def like(t):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
-
-        dx = torch.empty(shape, dtype=x2.dtype, device=dev)
-        same = post_weight is None and g2 is None and scale == 1.0        # then dh = dx, written once
-        dh = None if h2 is None or same else torch.empty(shape, dtype=x2.dtype, device=dev)
-        dgate, dw, db, dpw, dpb = like(g2), like(weight), like(bias), like(post_weight), like(post_bias)
-        shared = g2 is not None and rpg > 1
-        groups = g2.shape[0] if shared else 1
-        narr = sum(t is not None for t in (dw, db, dpw, dpb)) + int(shared)
-        fwd, bwd, ws_floats = _kernels()
-        ws = torch.empty(ws_floats(M, H, groups, narr), dtype=torch.float32, device=dev)
-        with hip.on_device(x2):
-            rc = bwd(x2.data_ptr(), hip.ptr(h2), hip.ptr(g2), weight.data_ptr(), hip.ptr(post_weight), hip.ptr(post_bias),
-                     stats.data_ptr(), hip.ptr(dy2), hip.ptr(dr2), dx.data_ptr(), hip.ptr(dh), hip.ptr(dgate), dw.data_ptr(),
-                     hip.ptr(db), hip.ptr(dpw), hip.ptr(dpb), ws.data_ptr(), hip.dt(x2), hip.dt(weight), int(layer), M, H, rpg,
-                     scale, hip.stream())
+        x, h, weight, bias, gate, post_weight, post_bias, stats = ctx.saved_tensors
+        _, _, _, M, H, rpg, scale = how = ctx.how
+        dy, dr = _dense(dy), _dense(dr)
+        dx = x.new_empty(x.shape)
+        same = post_weight is None and gate is None and scale == 1.0      # then dh = dx, written once
+        dh = None if same else _like(h)
+        dw, db, dgate, dpw, dpb = _like(weight), _like(bias), _like(gate), _like(post_weight), _like(post_bias)
+        groups = M // rpg if gate is not None and rpg > 1 else 0          # rows of a gate that is shared
+        narr = 1 + (bias is not None) + (post_weight is not None) + (post_bias is not None) + (groups > 0)
+        _, bwd, ws_floats = _kernels()
+        ws = stats.new_empty(ws_floats(M, H, groups or 1, narr))
+        rc = hip.launch(x, bwd, x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(post_weight),
+                        hip.ptr(post_bias), stats.data_ptr(), hip.ptr(dy), hip.ptr(dr), dx.data_ptr(), hip.ptr(dh), hip.ptr(dgate),
+                        dw.data_ptr(), hip.ptr(db), hip.ptr(dpw), hip.ptr(dpb), ws.data_ptr(), *how)
         hip.check(rc, "dtf_residual_norm_bwd")
-        if h2 is not None and same:
-            dh = dx
-        return dx, dh, dw, db, None if dgate is None else dgate.view(gate_shape), dpw, dpb, None, None, None, None
+        return dx, dx if same and h is not None else dh, dw, db, dgate, dpw, dpb, None, None, None, None
 
 
 def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=None, post_bias=None, kind="rms", eps=1e-6):
@@ -155,7 +144,7 @@ def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=
     if not x.is_cuda:
         return residual_norm_reference(x, h, weight, bias, gate=gate, scale=scale, post_weight=post_weight, post_bias=post_bias,
                                        kind=kind, eps=eps)
-    return _ResidualNorm.apply(x, h, weight, bias, gate, post_weight, post_bias, rpg or 1, scale, kind == "layer", eps)
+    return _ResidualNorm.apply(x, h, weight, bias, gate, post_weight, post_bias, rpg or 1, scale, int(kind == "layer"), eps)
 
 
 def rms_norm(x, weight, eps=1e-6):
@@ -163,7 +152,7 @@ def rms_norm(x, weight, eps=1e-6):
     _checked(x, None, weight, None, None, None, None, "rms")
     if not x.is_cuda:
         return _normed(x.float(), weight, None, "rms", eps).to(x.dtype)
-    return _ResidualNorm.apply(x, None, weight, None, None, None, None, 1, 1.0, False, float(eps))[0]
+    return _ResidualNorm.apply(x, None, weight, None, None, None, None, 1, 1.0, 0, float(eps))[0]
 
 
 class FusedRMSNorm(nn.Module):

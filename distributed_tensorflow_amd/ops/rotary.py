@@ -11,7 +11,6 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -107,18 +106,16 @@ def _dense_heads(t):
 def _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, sign):
     q, k = _dense_heads(q), _dense_heads(k)
     B, S, Hq, D = q.shape
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo = q.new_empty(q.shape)
+    ko = None if k is None else k.new_empty(k.shape)
     st = (ctypes.c_int64 * 6)(*q.stride()[:3], *((0, 0, 0) if k is None else k.stride()[:3]))
     p_bs = p_ss = 0
     if positions is not None:
         p_ss = positions.stride(-1)
         p_bs = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    with hip.on_device(q):
-        rc = _kernel()(q.data_ptr(), hip.ptr(k), qo.data_ptr(), hip.ptr(ko), hip.dt(q), st, hip.ptr(positions),
-                       int(positions is not None and positions.dtype == torch.int64), p_bs, p_ss, offset, inv_freq.data_ptr(),
-                       B, S, Hq, 0 if k is None else k.shape[2], D, inv_freq.numel(), int(interleaved), amplitude, sign,
-                       hip.stream())
+    rc = hip.launch(q, _kernel(), q.data_ptr(), hip.ptr(k), qo.data_ptr(), hip.ptr(ko), hip.dt(q), st, hip.ptr(positions),
+                    int(positions is not None and positions.dtype == torch.int64), p_bs, p_ss, offset, inv_freq.data_ptr(), B, S,
+                    Hq, 0 if k is None else k.shape[2], D, inv_freq.numel(), interleaved, amplitude, sign)
     hip.check(rc, "dtf_rotary")
     return qo, ko
 
@@ -131,7 +128,7 @@ class _Rotary(torch.autograd.Function):
         return _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, 1.0)
 
     @staticmethod
-    @once_differentiable
+    @hip.first_order
     def backward(ctx, dq, dk):
         inv_freq, positions = ctx.saved_tensors
         # the transpose of a rotation is the rotation by the negative angle
@@ -144,7 +141,7 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved=False, amplitude=1.0, 
     ``None``; ``positions`` int32 / int64 ``[S]`` or ``[B, S]`` (default ``offset + arange(S)``); ``interleaved``: pairs are
     neighbours ``(x[2j], x[2j+1])`` instead of the two halves ``(x[j], x[j + m])``.  Gradients flow to q and k."""
     _checked(q, k, inv_freq, positions)
-    interleaved, amplitude, offset = bool(interleaved), float(amplitude), int(offset)
+    interleaved, amplitude, offset = int(bool(interleaved)), float(amplitude), int(offset)
     if not q.is_cuda:
         return rotary_reference(q, k, inv_freq, positions, interleaved=interleaved, amplitude=amplitude, offset=offset)
     if q.numel() == 0 or (k is not None and k.numel() == 0):

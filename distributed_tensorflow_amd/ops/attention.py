@@ -113,8 +113,10 @@ def _general_kernels():
     global _general
     if _general is None:
         P, I, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
-        _general = (hip.declare("dtf_attn_general_fwd", [P] * 6 + [I] * 7 + [Fl, P, P]),
-                    hip.declare("dtf_attn_general_bwd", [P] * 11 + [I] * 7 + [Fl, P, P]))
+        L = ctypes.c_int64
+        _general = (hip.declare("dtf_attn_general_fwd", [P] * 7 + [I] * 7 + [Fl, P, P]),
+                    hip.declare("dtf_attn_general_bwd", [P] * 12 + [I] * 7 + [Fl, P, P]),
+                    hip.declare("dtf_attn_general_fwd_ws", [I] * 6, L), hip.declare("dtf_attn_general_bwd_ws", [I] * 6, L))
     return _general
 
 
@@ -124,6 +126,10 @@ def _operand(t):
     if st[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _workspace(like, floats):
+    return like.new_empty(floats, dtype=torch.float32) if floats else None
 
 
 def _general_strides(*tensors):
@@ -138,8 +144,10 @@ class _Attention(torch.autograd.Function):
         Sk, Hk = k.shape[1], k.shape[2]
         o = q.new_empty(q.shape)
         lse = q.new_empty((B, Hq, Sq), dtype=torch.float32)
+        fwd, _, ws_floats, _ = _general_kernels()
+        ws = _workspace(q, ws_floats(B, Sq, Sk, Hq, Hk, D))
         ctx.how = _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
-        rc = hip.launch(q, _general_kernels()[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), *ctx.how)
+        rc = hip.launch(q, fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), hip.ptr(ws), *ctx.how)
         hip.check(rc, "dtf_attn_general_fwd")
         ctx.save_for_backward(q, k, v, o, lse, kv_len)
         return o
@@ -151,8 +159,10 @@ class _Attention(torch.autograd.Function):
         if not do.is_contiguous() or do.data_ptr() % 16:
             do = do.clone(memory_format=torch.contiguous_format)
         dq, dk, dv, dsum = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape), lse.new_empty(lse.shape)
-        rc = hip.launch(q, _general_kernels()[1], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(),
-                        lse.data_ptr(), dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *ctx.how)
+        _, bwd, _, ws_floats = _general_kernels()
+        ws = _workspace(q, ws_floats(*ctx.how[1:7]))
+        rc = hip.launch(q, bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                        dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), hip.ptr(ws), *ctx.how)
         hip.check(rc, "dtf_attn_general_bwd")
         return dq, dk, dv, None, None, None
 

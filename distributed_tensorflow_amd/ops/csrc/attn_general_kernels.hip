@@ -28,7 +28,8 @@ struct AgArgs {
     u16 *out, *dq, *dk, *dv;              // contiguous [B, Sq, Hq, D] (dk, dv: [B, Sk, Hk, D])
     float *lse, *dsum;                    // [B, Hq, Sq]; lse in the log2 domain, +inf for a query that sees no key
     const int* kv_len;                    // [B] or null
-    int B, Sq, Sk, Hq, Hk, D, group, causal, ntiles;
+    float* ws;                            // partial results of `nsplit` workgroups that share a tile; unused for nsplit = 1
+    int B, Sq, Sk, Hq, Hk, D, group, causal, ntiles, nsplit;
     float scale, scale_log2e;
 };
 
@@ -77,25 +78,38 @@ __device__ __forceinline__ s16x8 ag_row(const unsigned char* img, int row, int c
     return *reinterpret_cast<const s16x8*>(img + ag_off<DP>(row, c));
 }
 
-// A tile of ROWS rows in flight from memory to an image through registers; rows at or past `limit` and columns past D
-// are zeros (never read), so nothing masked reaches a product.
+// A tile of ROWS rows from memory to an image by LDS-DMA (global_load_lds, 16 B a lane: no staging registers, no ds_write
+// pass).  One wave instruction fills 1 KB = 1024 / (2 DP) image rows, so the chunk that a lane fetches is the one whose
+// swizzled place it fills.  Rows at or past `limit` and columns past D come from a page of zeros: whatever padding holds is
+// never read, and nothing masked reaches a product.
+__device__ const u32x4 ag_zeros = {0u, 0u, 0u, 0u};
+
 template <int DP, int ROWS, int NT>
 struct AgTile {
-    static constexpr int CPR = DP / 8, N = ROWS * CPR / NT;
-    u32x4 r[N];
-    __device__ __forceinline__ void load(const u16* base, int64_t rs, int row0, int limit, int D, int tid) {
-        const int c = tid % CPR;
+    typedef __attribute__((address_space(1))) const void glb;
+    static constexpr int RPI = 1024 / (2 * DP), N = ROWS / RPI / (NT / 64), STEP = RPI * (NT / 64);
+    const u16* src;          // this lane's chunk of tile row `row` at tile 0
+    int row;
+    bool col;
+    int64_t rs;
+    __device__ __forceinline__ void init(const u16* base, int64_t rs_, int D, int wave, int lane) {
+        row = wave * RPI + lane / (DP / 8);
+        const int p = lane % (DP / 8);
+        const int x = DP == 128 ? row & 7 : (row >> 1) & 3;
+        const int c = (((p >> 1) ^ x) << 1) | ((p ^ (row >> 3)) & 1);      // STEP is a multiple of 16: the same for every row of a lane
+        col = c * 8 < D;
+        rs = rs_;
+        src = base + row * rs + c * 8;
+    }
+    // rows row0 .. row0 + ROWS - 1 of the matrix; `full`: all of them are below limit and D == DP (uniform)
+    __device__ __forceinline__ void load(unsigned char* img, int row0, int limit, bool full, int wave) const {
+        const u16* p = src + row0 * rs;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = row0 + tid / CPR + i * (NT / CPR);
-            r[i] = (u32x4){0u, 0u, 0u, 0u};
-            if (row < limit && c * 8 < D) r[i] = *reinterpret_cast<const u32x4*>(base + row * rs + c * 8);
+            const void* from = p + (int64_t)(i * STEP) * rs;
+            if (!full && !(col && row0 + row + i * STEP < limit)) from = &ag_zeros;
+            __builtin_amdgcn_global_load_lds((glb*)from, (ag_lds_void*)(img + (i * (NT / 64) + wave) * 1024), 16, 0, 0);
         }
-    }
-    __device__ __forceinline__ void store(unsigned char* img, int tid) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            *reinterpret_cast<u32x4*>(img + ag_off<DP>(tid / CPR + i * (NT / CPR), tid % CPR)) = r[i];
     }
 };
 
@@ -137,27 +151,34 @@ __device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DP / 
         }
 }
 
+#define AG_LANDED() asm volatile("s_waitcnt vmcnt(0)" ::: "memory")      // this wave's LDS-DMA has arrived
+
 // ---------------------------------------------------------------------------
-// Forward: 4 waves x 32 queries, 64 keys a step.  PACK: the rows of a workgroup run over the `group` query heads of one
-// key head and their Sq queries, so a few queries with many heads still fill the matrix tile and read K, V once.
+// Forward: 4 waves x 32 queries, 64 keys a step, K and V double-buffered (the DMA of a step's successor runs under its
+// products; one barrier a step).  The running maximum moves, and O is rescaled, only when a query's scores pass it by 2^8.
+// PACK: the rows of a workgroup run over the `group` query heads of one key head and their Sq queries, so a few queries with
+// many heads still fill the matrix tile and read K, V once.  nsplit > 1: that many workgroups share a tile's keys, each
+// writes its (O, m, l), and ag_join_kernel adds them.
 // ---------------------------------------------------------------------------
 template <int DP, bool PACK>
-__global__ __launch_bounds__(256) void ag_fwd_kernel(AgArgs a) {
+__global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, BN = 64, BM = 128;
-    __shared__ __attribute__((aligned(16))) unsigned char Kimg[BN * DP * 2];
-    __shared__ __attribute__((aligned(16))) unsigned char Vimg[BN * DP * 2];
+    __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int id = ag_xcd(blockIdx.x, gridDim.x);
+    int id = ag_xcd(blockIdx.x, gridDim.x);
+    const int sp = id % a.nsplit;
+    id /= a.nsplit;
     const int t = a.ntiles - 1 - id % a.ntiles, hb = id / a.ntiles;        // long causal tiles first
     const int H = PACK ? a.Hk : a.Hq, b = hb / H, h = hb - b * H;
     const int hk = PACK ? h : h / a.group, rows = PACK ? a.group * a.Sq : a.Sq;
     const int klen = ag_klen(a, b);
-    const int r = min(t * BM + wave * 32 + (lane & 31), rows - 1);
+    const int rw = t * BM + wave * 32, r = min(rw + (lane & 31), rows - 1);
     const int i = PACK ? r % a.Sq : r, head = PACK ? h * a.group + r / a.Sq : h;
     const int vis = ag_vis(a, i, klen);
-    const int end = PACK ? ag_vis(a, a.Sq - 1, klen) : ag_vis(a, min(t * BM + BM, a.Sq) - 1, klen);
-    int lo = vis, hi = vis;                                                // of this wave's queries
+    const int r0 = t * BM, r1 = min(t * BM + BM, rows) - 1;
+    const int end = ag_vis(a, PACK ? (r0 / a.Sq == r1 / a.Sq ? r1 % a.Sq : a.Sq - 1) : r1, klen);
+    int lo = vis, hi = rw < rows ? vis : 0;                                // of this wave's queries
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         lo = min(lo, __shfl_xor(lo, o, 64));
@@ -165,37 +186,31 @@ __global__ __launch_bounds__(256) void ag_fwd_kernel(AgArgs a) {
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
+    const int steps = (end + BN - 1) / BN;
+    const int kbeg = (int)((int64_t)steps * sp / a.nsplit) * BN, kend = min((int)((int64_t)steps * (sp + 1) / a.nsplit) * BN, end);
 
-    const u16* Kh = a.k + b * a.k_bs + hk * a.k_hs;
-    const u16* Vh = a.v + b * a.v_bs + hk * a.v_hs;
     s16x8 qf[KS];
     ag_frags<DP>(qf, a.q + b * a.q_bs + i * a.q_ss + head * a.q_hs, g, a.D);
+    AgTile<DP, BN, 256> kt, vt;
+    kt.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ss, a.D, wave, lane);
+    vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, a.D, wave, lane);
+    auto fetch = [&](unsigned char* K, unsigned char* V, int k0) {
+        const bool full = a.D == DP && k0 + BN <= klen;
+        kt.load(K, k0, klen, full, wave);
+        vt.load(V, k0, klen, full, wave);
+    };
 
     f32x16 oacc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_zero();
     float m = AG_NEG, l = 0.f;
-    AgTile<DP, BN, 256> kr, vr;
-    if (end > 0) {
-        kr.load(Kh, a.k_ss, 0, klen, a.D, tid);
-        vr.load(Vh, a.v_ss, 0, klen, a.D, tid);
-    }
-    for (int k0 = 0; k0 < end; k0 += BN) {
-        __syncthreads();
-        kr.store(Kimg, tid);
-        vr.store(Vimg, tid);
-        __syncthreads();
-        if (k0 + BN < end) {
-            kr.load(Kh, a.k_ss, k0 + BN, klen, a.D, tid);
-            vr.load(Vh, a.v_ss, k0 + BN, klen, a.D, tid);
-        }
-        if (k0 >= hi) continue;                                            // (uniform in the wave; barriers stay matched)
+    auto step = [&](const unsigned char* K, const unsigned char* V, int k0) {
         f32x16 s[BN / 32];
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
             s[u] = ag_zero();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[u] = ag_mfma(ag_row<DP>(Kimg, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s[u]);
+            for (int ks = 0; ks < KS; ++ks) s[u] = ag_mfma(ag_row<DP>(K, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s[u]);
         }
         if (k0 + BN > lo) {
 #pragma unroll
@@ -209,16 +224,18 @@ __global__ __launch_bounds__(256) void ag_fwd_kernel(AgArgs a) {
         for (int u = 0; u < BN / 32; ++u)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[u][e]);
-        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
-        const float mn = __builtin_elementwise_maximum(m, mx * a.scale_log2e);
-        const float mu = mn == AG_NEG ? 0.f : mn;                          // nothing seen yet: every p is exp2(-inf) = 0
-        const float alpha = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
-        l *= alpha;
+        mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
+        if (__any(!(mx <= m + 8.f))) {
+            const float mn = __builtin_elementwise_maximum(m, mx);
+            const float alpha = mn == AG_NEG ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
+                for (int e = 0; e < 16; ++e) oacc[dt][e] *= alpha;
+        }
+        const float mu = m == AG_NEG ? 0.f : m;                            // nothing seen yet: every p is exp2(-inf) = 0
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
 #pragma unroll
@@ -230,14 +247,74 @@ __global__ __launch_bounds__(256) void ag_fwd_kernel(AgArgs a) {
             for (int h2 = 0; h2 < 2; ++h2) {
                 const s16x8 pf = ag_pack(s[u], h2);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_mfma(ag_tr<DP>(Vimg, 32 * u + 16 * h2, 32 * dt, lane), pf, oacc[dt]);
+                for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_mfma(ag_tr<DP>(V, 32 * u + 16 * h2, 32 * dt, lane), pf, oacc[dt]);
             }
         }
+    };
+    if (kbeg < kend) fetch(K0, V0, kbeg);
+    AG_LANDED();
+    __syncthreads();
+    for (int k0 = kbeg; k0 < kend; k0 += 2 * BN) {
+        if (k0 + BN < kend) fetch(K1, V1, k0 + BN);
+        if (k0 < hi) step(K0, V0, k0);
+        AG_LANDED();
+        __syncthreads();
+        if (k0 + BN >= kend) break;
+        if (k0 + 2 * BN < kend) fetch(K0, V0, k0 + 2 * BN);
+        if (k0 + BN < hi) step(K1, V1, k0 + BN);
+        AG_LANDED();
+        __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
-    if (t * BM + wave * 32 + (lane & 31) < rows) {
-        ag_store_row<DP>(a.out + (((int64_t)b * a.Sq + i) * a.Hq + head) * a.D, oacc, l == 0.f ? 0.f : 1.f / l, g, a.D);
+    if (rw + (lane & 31) >= rows) return;
+    const int64_t row = ((int64_t)b * a.Sq + i) * a.Hq + head;
+    if (a.nsplit == 1) {
+        ag_store_row<DP>(a.out + row * a.D, oacc, l == 0.f ? 0.f : 1.f / l, g, a.D);
         if (g == 0) a.lse[((int64_t)b * a.Hq + head) * a.Sq + i] = l == 0.f ? __builtin_inff() : m + log2f(l);
+        return;
+    }
+    const int64_t n = (int64_t)a.B * a.Sq * a.Hq;
+    float* po = a.ws + (sp * n + row) * a.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+            const int d = 32 * dt + 8 * rq + 4 * g;
+            if (d < a.D) *reinterpret_cast<f32x4*>(po + d) = (f32x4){oacc[dt][4 * rq], oacc[dt][4 * rq + 1], oacc[dt][4 * rq + 2], oacc[dt][4 * rq + 3]};
+        }
+    if (g == 0) {
+        float* ml = a.ws + (int64_t)a.nsplit * n * a.D + (sp * n + row) * 2;
+        ml[0] = m;
+        ml[1] = l;
+    }
+}
+
+// O = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M): 32 lanes a row, 4 columns a lane
+__global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
+    const int64_t n = (int64_t)a.B * a.Sq * a.Hq, row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const int d = threadIdx.x % 32 * 4;
+    if (row >= n) return;
+    const float* ml = a.ws + (int64_t)a.nsplit * n * a.D + row * 2;
+    float M = AG_NEG, l = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) M = __builtin_elementwise_maximum(M, ml[s * n * 2]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float ms = ml[s * n * 2], w = ms == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
+        l = fmaf(ml[s * n * 2 + 1], w, l);
+        if (d < a.D) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.ws + (s * n + row) * a.D + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], w, o[e]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (d < a.D) {
+        const u32x2 p = {pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+        *reinterpret_cast<u32x2*>(a.out + row * a.D + d) = p;
+    }
+    if (d == 0) {
+        const int64_t b = row / ((int64_t)a.Sq * a.Hq), ih = row - b * a.Sq * a.Hq, i = ih / a.Hq, h = ih - i * a.Hq;
+        a.lse[(b * a.Hq + h) * a.Sq + i] = l == 0.f ? __builtin_inff() : M + log2f(l);
     }
 }
 
@@ -246,26 +323,32 @@ __global__ __launch_bounds__(256) void ag_fwd_kernel(AgArgs a) {
 // summed over d in the order of dP = V . dO^T), so that a query with ONE key, whose O is that V row, has dS = 0 exactly.
 // ---------------------------------------------------------------------------
 template <int DP>
-__global__ __launch_bounds__(256) void ag_dq_kernel(AgArgs a) {
+__global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, BN = 64, BM = 128;
-    __shared__ __attribute__((aligned(16))) unsigned char Kimg[BN * DP * 2];
-    __shared__ __attribute__((aligned(16))) unsigned char Vimg[BN * DP * 2];
+    __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int id = ag_xcd(blockIdx.x, gridDim.x);
     const int t = a.ntiles - 1 - id % a.ntiles, hb = id / a.ntiles;
     const int b = hb / a.Hq, h = hb - b * a.Hq, hk = h / a.group;
     const int klen = ag_klen(a, b);
-    const int i = min(t * BM + wave * 32 + (lane & 31), a.Sq - 1);
+    const int rw = t * BM + wave * 32, i = min(rw + (lane & 31), a.Sq - 1);
     const int vis = ag_vis(a, i, klen), end = ag_vis(a, min(t * BM + BM, a.Sq) - 1, klen);
-    const int lo = ag_vis(a, min(t * BM + wave * 32, a.Sq - 1), klen), hi = ag_vis(a, min(t * BM + wave * 32 + 32, a.Sq) - 1, klen);
+    const int lo = ag_vis(a, min(rw, a.Sq - 1), klen), hi = rw < a.Sq ? ag_vis(a, min(rw + 32, a.Sq) - 1, klen) : 0;
 
-    const u16* Kh = a.k + b * a.k_bs + hk * a.k_hs;
-    const u16* Vh = a.v + b * a.v_bs + hk * a.v_hs;
     const int64_t row = ((int64_t)b * a.Sq + i) * a.Hq + h, li = ((int64_t)b * a.Hq + h) * a.Sq + i;
     s16x8 qf[KS], gf[KS];
     ag_frags<DP>(qf, a.q + b * a.q_bs + i * a.q_ss + h * a.q_hs, g, a.D);
     ag_frags<DP>(gf, a.dO + row * a.D, g, a.D);
+    AgTile<DP, BN, 256> kt, vt;
+    kt.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ss, a.D, wave, lane);
+    vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, a.D, wave, lane);
+    auto fetch = [&](unsigned char* K, unsigned char* V, int k0) {
+        const bool full = a.D == DP && k0 + BN <= klen;
+        kt.load(K, k0, klen, full, wave);
+        vt.load(V, k0, klen, full, wave);
+    };
+    if (end > 0) fetch(K0, V0, 0);
     float dsum = 0.f;
     {
         s16x8 of[KS];
@@ -279,40 +362,25 @@ __global__ __launch_bounds__(256) void ag_dq_kernel(AgArgs a) {
         dsum += __shfl_xor(dsum, 32, 64);
     }
     const float lse = a.lse[li];
-    const bool valid = t * BM + wave * 32 + (lane & 31) < a.Sq;
+    const bool valid = rw + (lane & 31) < a.Sq;
     if (valid && g == 0) a.dsum[li] = dsum;
 
     f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_zero();
-    AgTile<DP, BN, 256> kr, vr;
-    if (end > 0) {
-        kr.load(Kh, a.k_ss, 0, klen, a.D, tid);
-        vr.load(Vh, a.v_ss, 0, klen, a.D, tid);
-    }
-    for (int k0 = 0; k0 < end; k0 += BN) {
-        __syncthreads();
-        kr.store(Kimg, tid);
-        vr.store(Vimg, tid);
-        __syncthreads();
-        if (k0 + BN < end) {
-            kr.load(Kh, a.k_ss, k0 + BN, klen, a.D, tid);
-            vr.load(Vh, a.v_ss, k0 + BN, klen, a.D, tid);
-        }
-        if (k0 >= hi) continue;
+    auto step = [&](const unsigned char* K, const unsigned char* V, int k0) {
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
             f32x16 s = ag_zero(), dp = ag_zero();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                s = ag_mfma(ag_row<DP>(Kimg, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s);
-                dp = ag_mfma(ag_row<DP>(Vimg, 32 * u + (lane & 31), 2 * ks + g), gf[ks], dp);
+                s = ag_mfma(ag_row<DP>(K, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s);
+                dp = ag_mfma(ag_row<DP>(V, 32 * u + (lane & 31), 2 * ks + g), gf[ks], dp);
             }
             const bool edge = k0 + 32 * u + 32 > lo;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse));
-                float ds = p * (dp[e] - dsum);
+                float ds = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (dp[e] - dsum);
                 if (edge) ds = k0 + 32 * u + 8 * (e >> 2) + 4 * g + (e & 3) < vis ? ds : 0.f;
                 s[e] = ds;
             }
@@ -320,9 +388,22 @@ __global__ __launch_bounds__(256) void ag_dq_kernel(AgArgs a) {
             for (int h2 = 0; h2 < 2; ++h2) {
                 const s16x8 f = ag_pack(s, h2);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_mfma(ag_tr<DP>(Kimg, 32 * u + 16 * h2, 32 * dt, lane), f, acc[dt]);
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_mfma(ag_tr<DP>(K, 32 * u + 16 * h2, 32 * dt, lane), f, acc[dt]);
             }
         }
+    };
+    AG_LANDED();
+    __syncthreads();
+    for (int k0 = 0; k0 < end; k0 += 2 * BN) {
+        if (k0 + BN < end) fetch(K1, V1, k0 + BN);
+        if (k0 < hi) step(K0, V0, k0);
+        AG_LANDED();
+        __syncthreads();
+        if (k0 + BN >= end) break;
+        if (k0 + 2 * BN < end) fetch(K0, V0, k0 + 2 * BN);
+        if (k0 + BN < hi) step(K1, V1, k0 + BN);
+        AG_LANDED();
+        __syncthreads();
     }
     if (valid) ag_store_row<DP>(a.dq + row * a.D, acc, a.scale, g, a.D);
 }
@@ -330,26 +411,26 @@ __global__ __launch_bounds__(256) void ag_dq_kernel(AgArgs a) {
 // ---------------------------------------------------------------------------
 // Backward, dK and dV: 4 waves x 32 keys, 32 queries a step, over all query heads of the key head's group (so shared
 // heads' gradients are one fixed-order sum: no atomics).  S = Q . K^T, dP = dO . V^T (a lane owns one key),
-// dV^T += dO^T . P, dK^T += Q^T . dS.
+// dV^T += dO^T . P, dK^T += Q^T . dS.  nsplit > 1: that many workgroups share a tile's (head, query) steps, each writes
+// fp32 sums, and ag_add_kernel adds them in order.
 // ---------------------------------------------------------------------------
 template <int DP>
-__global__ __launch_bounds__(256) void ag_dkv_kernel(AgArgs a) {
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void ag_dkv_kernel(AgArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, BQ = 32, BM = 128;
-    __shared__ __attribute__((aligned(16))) unsigned char Qimg[BQ * DP * 2];
-    __shared__ __attribute__((aligned(16))) unsigned char Gimg[BQ * DP * 2];
-    __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+    __shared__ __attribute__((aligned(16))) unsigned char Q0[BQ * DP * 2], Q1[BQ * DP * 2], G0[BQ * DP * 2], G1[BQ * DP * 2];
+    __shared__ __attribute__((aligned(16))) float L0[BQ], L1[BQ], D0[BQ], D1[BQ];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int id = ag_xcd(blockIdx.x, gridDim.x);
+    int id = ag_xcd(blockIdx.x, gridDim.x);
+    const int sp = id % a.nsplit;
+    id /= a.nsplit;
     const int t = id % a.ntiles, hb = id / a.ntiles;                       // low keys are seen by the most queries
     const int b = hb / a.Hk, hk = hb - b * a.Hk;
     const int klen = ag_klen(a, b);
-    const int j = t * BM + wave * 32 + (lane & 31), jc = min(j, a.Sk - 1), jw = t * BM + wave * 32;
+    const int jw = t * BM + wave * 32, j = jw + (lane & 31), jc = min(j, a.Sk - 1);
     // first query that sees key j: i + 1 + Sk - Sq > j
     const int off = a.Sk - a.Sq;
-    const int first = a.causal ? max(0, t * BM - off) : 0;
-    const int begin = first / BQ * BQ;
-    const int64_t go_ss = (int64_t)a.Hq * a.D;
+    const int begin = a.causal ? max(0, t * BM - off) / BQ * BQ : 0;
 
     s16x8 kf[KS], vf[KS];
     ag_frags<DP>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
@@ -368,43 +449,41 @@ __global__ __launch_bounds__(256) void ag_dkv_kernel(AgArgs a) {
         dk[dt] = ag_zero();
         dv[dt] = ag_zero();
     }
-    const int steps = t * BM < klen && begin < a.Sq ? (a.Sq - begin + BQ - 1) / BQ : 0, total = steps * a.group;
-    AgTile<DP, BQ, 256> qr, gr;
-    float lr = 0.f, dr = 0.f;
-    auto load = [&](int n) {
+    const int steps = t * BM < klen && begin < a.Sq ? (a.Sq - begin + BQ - 1) / BQ : 0;
+    const int64_t total = (int64_t)steps * a.group;
+    const int n0 = (int)(total * sp / a.nsplit), n1 = (int)(total * (sp + 1) / a.nsplit);
+    AgTile<DP, BQ, 256> qt, gt;
+    qt.init(a.q + b * a.q_bs, a.q_ss, a.D, wave, lane);
+    gt.init(a.dO + (int64_t)b * a.Sq * a.Hq * a.D, (int64_t)a.Hq * a.D, a.D, wave, lane);
+    const u16 *qs = qt.src, *gs = gt.src;
+    auto fetch = [&](unsigned char* Q, unsigned char* G, float* L, float* Dm, int n) {
         const int h = hk * a.group + n / steps, q0 = begin + n % steps * BQ;
-        qr.load(a.q + b * a.q_bs + h * a.q_hs, a.q_ss, q0, a.Sq, a.D, tid);
-        gr.load(a.dO + ((int64_t)b * a.Sq * a.Hq + h) * a.D, go_ss, q0, a.Sq, a.D, tid);
+        const bool full = a.D == DP && q0 + BQ <= a.Sq;
+        qt.src = qs + h * a.q_hs;
+        gt.src = gs + (int64_t)h * a.D;
+        qt.load(Q, q0, a.Sq, full, wave);
+        gt.load(G, q0, a.Sq, full, wave);
         if (tid < BQ) {
             const int64_t li = ((int64_t)b * a.Hq + h) * a.Sq + q0 + tid;
-            lr = q0 + tid < a.Sq ? a.lse[li] : __builtin_inff();
-            dr = q0 + tid < a.Sq ? a.dsum[li] : 0.f;
+            const bool in = q0 + tid < a.Sq;
+            L[tid] = in ? a.lse[li] : __builtin_inff();
+            Dm[tid] = in ? a.dsum[li] : 0.f;
         }
     };
-    if (total > 0) load(0);
-    for (int n = 0; n < total; ++n) {
+    auto step = [&](const unsigned char* Q, const unsigned char* G, const float* L, const float* Dm, int n) {
         const int q0 = begin + n % steps * BQ;
-        __syncthreads();
-        qr.store(Qimg, tid);
-        gr.store(Gimg, tid);
-        if (tid < BQ) {
-            Ls[tid] = lr;
-            Ds[tid] = dr;
-        }
-        __syncthreads();
-        if (n + 1 < total) load(n + 1);
-        if (a.causal && q0 + BQ - 1 + off < jw) continue;                  // no query of the step sees this wave's keys
+        if (a.causal && q0 + BQ - 1 + off < jw) return;                    // no query of the step sees this wave's keys
         f32x16 s = ag_zero(), dp = ag_zero();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            s = ag_mfma(ag_row<DP>(Qimg, lane & 31, 2 * ks + g), kf[ks], s);
-            dp = ag_mfma(ag_row<DP>(Gimg, lane & 31, 2 * ks + g), vf[ks], dp);
+            s = ag_mfma(ag_row<DP>(Q, lane & 31, 2 * ks + g), kf[ks], s);
+            dp = ag_mfma(ag_row<DP>(G, lane & 31, 2 * ks + g), vf[ks], dp);
         }
         const bool edge = (a.causal && q0 + off < jw + 31) || jw + 32 > klen;
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(Ls + 8 * rq + 4 * g);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(Ds + 8 * rq + 4 * g);
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(L + 8 * rq + 4 * g);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(Dm + 8 * rq + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int x = 4 * rq + e;
@@ -419,16 +498,56 @@ __global__ __launch_bounds__(256) void ag_dkv_kernel(AgArgs a) {
             const s16x8 pf = ag_pack(s, h2), df = ag_pack(dp, h2);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                dv[dt] = ag_mfma(ag_tr<DP>(Gimg, 16 * h2, 32 * dt, lane), pf, dv[dt]);
-                dk[dt] = ag_mfma(ag_tr<DP>(Qimg, 16 * h2, 32 * dt, lane), df, dk[dt]);
+                dv[dt] = ag_mfma(ag_tr<DP>(G, 16 * h2, 32 * dt, lane), pf, dv[dt]);
+                dk[dt] = ag_mfma(ag_tr<DP>(Q, 16 * h2, 32 * dt, lane), df, dk[dt]);
             }
         }
+    };
+    if (n0 < n1) fetch(Q0, G0, L0, D0, n0);
+    AG_LANDED();
+    __syncthreads();
+    for (int n = n0; n < n1; n += 2) {
+        if (n + 1 < n1) fetch(Q1, G1, L1, D1, n + 1);
+        step(Q0, G0, L0, D0, n);
+        AG_LANDED();
+        __syncthreads();
+        if (n + 1 >= n1) break;
+        if (n + 2 < n1) fetch(Q0, G0, L0, D0, n + 2);
+        step(Q1, G1, L1, D1, n + 1);
+        AG_LANDED();
+        __syncthreads();
     }
-    if (j < a.Sk) {
-        const int64_t o = (((int64_t)b * a.Sk + j) * a.Hk + hk) * a.D;
+    if (j >= a.Sk) return;
+    const int64_t o = (((int64_t)b * a.Sk + j) * a.Hk + hk) * a.D;
+    if (a.nsplit == 1) {
         ag_store_row<DP>(a.dk + o, dk, a.scale, g, a.D);
         ag_store_row<DP>(a.dv + o, dv, 1.f, g, a.D);
+        return;
     }
+    const int64_t n = (int64_t)a.B * a.Sk * a.Hk * a.D;
+    float* pk = a.ws + sp * 2 * n + o;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+            const int d = 32 * dt + 8 * rq + 4 * g;
+            if (d < a.D) {
+                *reinterpret_cast<f32x4*>(pk + d) = (f32x4){dk[dt][4 * rq], dk[dt][4 * rq + 1], dk[dt][4 * rq + 2], dk[dt][4 * rq + 3]};
+                *reinterpret_cast<f32x4*>(pk + n + d) = (f32x4){dv[dt][4 * rq], dv[dt][4 * rq + 1], dv[dt][4 * rq + 2], dv[dt][4 * rq + 3]};
+            }
+        }
+}
+
+// dK (blockIdx.y 0) and dV (1) from the partial sums, 4 elements a thread
+__global__ __launch_bounds__(256) void ag_add_kernel(AgArgs a) {
+    const int64_t n = (int64_t)a.B * a.Sk * a.Hk * a.D, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    const float* p = a.ws + blockIdx.y * n + i;
+    f32x4 s = *reinterpret_cast<const f32x4*>(p);
+    for (int k = 1; k < a.nsplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * 2 * n);
+    if (blockIdx.y == 0) s *= a.scale;
+    const u32x2 r = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
+    *reinterpret_cast<u32x2*>((blockIdx.y ? a.dv : a.dk) + i) = r;
 }
 
 // ---------------------------------------------------------------------------
@@ -446,26 +565,62 @@ static int ag_grid(int64_t n, int* out) {
     return 0;
 }
 
+// Workgroups that share a tile: enough for AG_FILL workgroups (two a CU), no fewer than `least` steps each.
+#define AG_FILL 512
+static int ag_splits(int64_t grid, int64_t steps, int least) {
+    int64_t n = AG_FILL / grid, most = steps / least;
+    if (n > most) n = most;
+    return n < 1 ? 1 : (int)n;
+}
+
+// PACK where a 128-row tile of one head's queries would be part empty and the group's rows fill fewer tiles
+static bool ag_pack_rows(int Sq, int group) {
+    return group > 1 && Sq <= 512 && ((int64_t)group * Sq + 127) / 128 < (int64_t)group * ((Sq + 127) / 128);
+}
+
+static int ag_fwd_splits(int B, int Sq, int Sk, int Hq, int Hk) {
+    const bool pack = ag_pack_rows(Sq, Hq / Hk);
+    const int64_t rows = pack ? (int64_t)(Hq / Hk) * Sq : Sq;
+    return ag_splits((int64_t)B * (pack ? Hk : Hq) * ((rows + 127) / 128), (Sk + 63) / 64, 4);
+}
+
+static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk) {
+    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), (int64_t)((Sq + 31) / 32) * (Hq / Hk), 8);
+}
+
 extern "C" {
 
-// st: the nine element strides (batch, token, head) of q, k, v
-int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* st, int B, int Sq,
-                         int Sk, int Hq, int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
+// fp32 workspace of the forward / backward, in floats (0: none)
+int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
+    const int64_t n = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
+    return n > 1 ? n * B * Sq * Hq * (D + 2) : 0;
+}
+
+int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
+    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk);
+    return n > 1 ? n * 2 * B * Sk * Hk * D : 0;
+}
+
+// st: the nine element strides (batch, token, head) of q, k, v; ws: dtf_attn_general_fwd_ws floats
+int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, float* lse, float* ws, const int64_t* st, int B,
+                         int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
     AgArgs a{};
-    a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.out = (u16*)o; a.lse = lse;
+    a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.out = (u16*)o; a.lse = lse; a.ws = ws;
     a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
     a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
     a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
     a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
     int rc = ag_check(a, st, 9), grid = 0;
     if (rc) return rc;
-    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o)) & 15) return -16;
+    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)ws)) & 15) return -16;
     a.group = Hq / Hk;
-    const bool pack = a.group > 1 && Sq < 128;         // a 128-row tile of one head would be part empty
+    const bool pack = ag_pack_rows(Sq, a.group);
     const int64_t rows = pack ? (int64_t)a.group * Sq : Sq;
     a.ntiles = (int)((rows + 127) / 128);
-    if ((rc = ag_grid((int64_t)B * (pack ? Hk : Hq) * a.ntiles, &grid))) return rc;
+    a.nsplit = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
+    if (a.nsplit > 1 && !ws) return -73;
+    if ((rc = ag_grid((int64_t)B * (pack ? Hk : Hq) * a.ntiles * a.nsplit, &grid))) return rc;
     if (D > 64) {
         if (pack) hipLaunchKernelGGL((ag_fwd_kernel<128, true>), dim3(grid), dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((ag_fwd_kernel<128, false>), dim3(grid), dim3(256), 0, stream, a);
@@ -474,17 +629,23 @@ int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, f
         else hipLaunchKernelGGL((ag_fwd_kernel<64, false>), dim3(grid), dim3(256), 0, stream, a);
     }
     DTF_CHECK_LAUNCH();
+    if (a.nsplit > 1) {
+        if ((rc = ag_grid(((int64_t)B * Sq * Hq + 7) / 8, &grid))) return rc;
+        hipLaunchKernelGGL(ag_join_kernel, dim3(grid), dim3(256), 0, stream, a);
+        DTF_CHECK_LAUNCH();
+    }
     return 0;
 }
 
-// o, do_: contiguous [B, Sq, Hq, D]; dsum: workspace [B, Hq, Sq]; dq like o, dk / dv contiguous [B, Sk, Hk, D]
+// o, do_: contiguous [B, Sq, Hq, D]; dsum: workspace [B, Hq, Sq]; dq like o, dk / dv contiguous [B, Sk, Hk, D];
+// ws: dtf_attn_general_bwd_ws floats
 int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                         float* dsum, void* dq, void* dk, void* dv, const int64_t* st, int B, int Sq, int Sk, int Hq, int Hk,
-                         int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
+                         float* dsum, void* dq, void* dk, void* dv, float* ws, const int64_t* st, int B, int Sq, int Sk, int Hq,
+                         int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
     AgArgs a{};
     a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.o = (const u16*)o; a.dO = (const u16*)do_;
-    a.lse = const_cast<float*>(lse); a.dsum = dsum; a.dq = (u16*)dq; a.dk = (u16*)dk; a.dv = (u16*)dv;
+    a.lse = const_cast<float*>(lse); a.dsum = dsum; a.dq = (u16*)dq; a.dk = (u16*)dk; a.dv = (u16*)dv; a.ws = ws;
     a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
     a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
     a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
@@ -492,18 +653,28 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     int rc = ag_check(a, st, 9), grid = 0;
     if (rc) return rc;
     if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)do_) | ((uintptr_t)dq) |
-         ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) return -16;
+         ((uintptr_t)dk) | ((uintptr_t)dv) | ((uintptr_t)ws)) & 15) return -16;
     a.group = Hq / Hk;
+    const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk);
+    if (splits > 1 && !ws) return -73;
+    if ((int64_t)((Sq + 31) / 32) * a.group > 0x7fffffff) return -72;
     a.ntiles = (Sq - 1) / 128 + 1;
+    a.nsplit = 1;
     if ((rc = ag_grid((int64_t)B * Hq * a.ntiles, &grid))) return rc;
     if (D > 64) hipLaunchKernelGGL((ag_dq_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((ag_dq_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
     DTF_CHECK_LAUNCH();
     a.ntiles = (Sk - 1) / 128 + 1;
-    if ((rc = ag_grid((int64_t)B * Hk * a.ntiles, &grid))) return rc;
+    a.nsplit = splits;
+    if ((rc = ag_grid((int64_t)B * Hk * a.ntiles * splits, &grid))) return rc;
     if (D > 64) hipLaunchKernelGGL((ag_dkv_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((ag_dkv_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
     DTF_CHECK_LAUNCH();
+    if (splits > 1) {
+        if ((rc = ag_grid(((int64_t)B * Sk * Hk * D + 1023) / 1024, &grid))) return rc;
+        hipLaunchKernelGGL(ag_add_kernel, dim3(grid, 2), dim3(256), 0, stream, a);
+        DTF_CHECK_LAUNCH();
+    }
     return 0;
 }
 

@@ -116,7 +116,7 @@ def _general_kernels():
         L = ctypes.c_int64
         _general = (hip.declare("dtf_attn_general_fwd", [P] * 7 + [I] * 7 + [Fl, P, P]),
                     hip.declare("dtf_attn_general_bwd", [P] * 12 + [I] * 7 + [Fl, P, P]),
-                    hip.declare("dtf_attn_general_fwd_ws", [I] * 6, L), hip.declare("dtf_attn_general_bwd_ws", [I] * 6, L))
+                    hip.declare("dtf_attn_general_fwd_ws", [I] * 6, L), hip.declare("dtf_attn_general_bwd_ws", [I] * 7, L))
     return _general
 
 
@@ -160,7 +160,7 @@ class _Attention(torch.autograd.Function):
             do = do.clone(memory_format=torch.contiguous_format)
         dq, dk, dv, dsum = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape), lse.new_empty(lse.shape)
         _, bwd, _, ws_floats = _general_kernels()
-        ws = _workspace(q, ws_floats(*ctx.how[1:7]))
+        ws = _workspace(q, ws_floats(*ctx.how[1:8]))
         rc = hip.launch(q, bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
                         dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), hip.ptr(ws), *ctx.how)
         hip.check(rc, "dtf_attn_general_bwd")

@@ -60,65 +60,74 @@ __device__ __forceinline__ s16x8 ag_pack(const f32x16& x, int s) {
     return __builtin_bit_cast(s16x8, p);
 }
 
-// transposed A operand from an image: 32 columns d0 .. d0+31 as rows, 16 image rows row0 .. row0+15 as k in the
-// accumulators' key order.  The 16 lanes of a group read a 4-row x 16-column block, lane 4 q + p its row q, columns 4 p.
+// A lane's places in an image.  The swizzle is an XOR, so every other place is (place ^ constant) + constant:
+//   row:   chunk g of row lane & 31; the k-th operand of 16 columns is at row ^ (k << 5), 32 rows further + 32 rows
+//   tr:    the transposed read of rows 4 g + (0..3), columns 0..31 (the 16 lanes of a group read a 4-row x 16-column block,
+//          lane 4 q + p its row q, columns 4 p); columns 32 d .. at tr ^ (d << 6), rows + 8 at (tr ^ 16) + 8 rows
+// keep() makes the compiler derive them where they are used instead of holding 24 addresses over the loop (which spilled).
 template <int DP>
-__device__ __forceinline__ s16x8 ag_tr(const unsigned char* img, int row0, int d0, int lane) {
-    const int g = lane >> 5, row = row0 + 4 * g + ((lane >> 2) & 3), col = d0 + (lane & 16) + 4 * (lane & 3);
-    const unsigned char* p0 = img + ag_off<DP>(row, col >> 3) + (col & 7) * 2;
-    const unsigned char* p1 = img + ag_off<DP>(row + 8, col >> 3) + (col & 7) * 2;
-    typedef __attribute__((address_space(3))) ag_s16x4* lp;
-    const ag_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p0);
-    const ag_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p1);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-template <int DP>
-__device__ __forceinline__ s16x8 ag_row(const unsigned char* img, int row, int c) {
-    return *reinterpret_cast<const s16x8*>(img + ag_off<DP>(row, c));
-}
+struct AgLane {
+    unsigned row, tr;
+    __device__ __forceinline__ void init(int lane) {
+        row = ag_off<DP>(lane & 31, lane >> 5);
+        const int r = 4 * (lane >> 5) + ((lane >> 2) & 3), c = (lane & 16) + 4 * (lane & 3);
+        tr = ag_off<DP>(r, c >> 3) + (c & 7) * 2;
+    }
+    __device__ __forceinline__ void keep() { asm volatile("" : "+v"(row), "+v"(tr)); }
+    // rows r0 + (lane & 31) (r0 a multiple of 32), columns 16 k + 8 g .. + 7
+    __device__ __forceinline__ s16x8 rows(const unsigned char* img, int r0, int k) const {
+        return *reinterpret_cast<const s16x8*>(img + (row ^ (unsigned)(k << 5)) + r0 * DP * 2);
+    }
+    // transposed: columns 32 d .. + 31 as rows, image rows r0 .. r0 + 15 (r0 a multiple of 16) as k in the accumulators' order
+    __device__ __forceinline__ s16x8 cols(const unsigned char* img, int r0, int d) const {
+        typedef __attribute__((address_space(3))) ag_s16x4* lp;
+        const ag_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(img + (tr ^ (unsigned)(d << 6)) + r0 * DP * 2));
+        const ag_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(img + (tr ^ (unsigned)(d << 6 | 16)) + (r0 + 8) * DP * 2));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 
 // A tile of ROWS rows from memory to an image by LDS-DMA (global_load_lds, 16 B a lane: no staging registers, no ds_write
 // pass).  One wave instruction fills 1 KB = 1024 / (2 DP) image rows, so the chunk that a lane fetches is the one whose
 // swizzled place it fills.  Rows at or past `limit` and columns past D come from a page of zeros: whatever padding holds is
 // never read, and nothing masked reaches a product.
 __device__ const u32x4 ag_zeros = {0u, 0u, 0u, 0u};
+__device__ const float ag_inf = __builtin_inff();
+typedef __attribute__((address_space(1))) const void ag_glb_void;
 
 template <int DP, int ROWS, int NT>
 struct AgTile {
-    typedef __attribute__((address_space(1))) const void glb;
     static constexpr int RPI = 1024 / (2 * DP), N = ROWS / RPI / (NT / 64), STEP = RPI * (NT / 64);
-    const u16* src;          // this lane's chunk of tile row `row` at tile 0
+    const char* base;        // of the matrix (uniform)
+    int64_t rs;              // bytes from row to row
+    unsigned off;            // this lane's byte offset from the tile's first row (a token stride is below 2^25 elements)
     int row;
     bool col;
-    int64_t rs;
-    __device__ __forceinline__ void init(const u16* base, int64_t rs_, int D, int wave, int lane) {
+    __device__ __forceinline__ void init(const u16* base_, int64_t rs_, int D, int wave, int lane) {
         row = wave * RPI + lane / (DP / 8);
         const int p = lane % (DP / 8);
         const int x = DP == 128 ? row & 7 : (row >> 1) & 3;
         const int c = (((p >> 1) ^ x) << 1) | ((p ^ (row >> 3)) & 1);      // STEP is a multiple of 16: the same for every row of a lane
         col = c * 8 < D;
-        rs = rs_;
-        src = base + row * rs + c * 8;
+        base = reinterpret_cast<const char*>(base_);
+        rs = rs_ * 2;
+        off = (unsigned)row * (unsigned)rs + c * 16;
     }
     // rows row0 .. row0 + ROWS - 1 of the matrix; `full`: all of them are below limit and D == DP (uniform)
     __device__ __forceinline__ void load(unsigned char* img, int row0, int limit, bool full, int wave) const {
-        const u16* p = src + row0 * rs;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const void* from = p + (int64_t)(i * STEP) * rs;
+            const char* p = base + (row0 + i * STEP) * rs;
+            const void* from = p + off;
             if (!full && !(col && row0 + row + i * STEP < limit)) from = &ag_zeros;
-            __builtin_amdgcn_global_load_lds((glb*)from, (ag_lds_void*)(img + (i * (NT / 64) + wave) * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((ag_glb_void*)from, (ag_lds_void*)(img + (i * (NT / 64) + wave) * 1024), 16, 0, 0);
         }
     }
 };
 
-// workgroups of one head land on one XCD (ids go round the 8 XCDs), so its keys and values are read into one L2
-__device__ __forceinline__ int ag_xcd(int id, int n) {
-    const int q = n >> 3, r = n & 7, x = id & 7, i = id >> 3;
-    return x * q + (x < r ? x : r) + i;
-}
-
+// Workgroup order: the tile is the slow index (causal tiles differ in length: all heads' longest come first, and every XCD
+// gets the same mix), the unit -- (share, head) -- the fast one.  Ids go round the 8 XCDs, so with a multiple of 8 units one
+// head's workgroups stay on one XCD and its keys and values in one L2; so do the query heads of one key head.
 __device__ __forceinline__ int ag_vis(const AgArgs& a, int i, int klen) {
     int n = a.causal ? min(klen, i + 1 + a.Sk - a.Sq) : klen;
     return max(n, 0);
@@ -143,7 +152,7 @@ __device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DP / 
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
             const int d = 32 * dt + 8 * rq + 4 * g;
-            if (d < D) {
+            if (32 * dt + 8 * rq < D) {                                     // (uniform: D is a multiple of 8)
                 const u32x2 p = {pack_bf16x2(acc[dt][4 * rq] * f, acc[dt][4 * rq + 1] * f),
                                  pack_bf16x2(acc[dt][4 * rq + 2] * f, acc[dt][4 * rq + 3] * f)};
                 *reinterpret_cast<u32x2*>(row + d) = p;
@@ -166,12 +175,11 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = ag_xcd(blockIdx.x, gridDim.x);
-    const int sp = id % a.nsplit;
-    id /= a.nsplit;
-    const int t = a.ntiles - 1 - id % a.ntiles, hb = id / a.ntiles;        // long causal tiles first
-    const int H = PACK ? a.Hk : a.Hq, b = hb / H, h = hb - b * H;
-    const int hk = PACK ? h : h / a.group, rows = PACK ? a.group * a.Sq : a.Sq;
+    const int kv = a.B * a.Hk, units = gridDim.x / a.ntiles;               // units: nsplit x (PACK ? 1 : group) x kv
+    const int t = a.ntiles - 1 - blockIdx.x / units, u = blockIdx.x % units;
+    const int b = u % kv / a.Hk, hk = u % kv % a.Hk;
+    const int h = PACK ? hk : hk * a.group + u / kv % a.group, sp = PACK ? u / kv : u / kv / a.group;
+    const int rows = PACK ? a.group * a.Sq : a.Sq;
     const int klen = ag_klen(a, b);
     const int rw = t * BM + wave * 32, r = min(rw + (lane & 31), rows - 1);
     const int i = PACK ? r % a.Sq : r, head = PACK ? h * a.group + r / a.Sq : h;
@@ -204,20 +212,23 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_zero();
     float m = AG_NEG, l = 0.f;
+    AgLane<DP> at;
+    at.init(lane);
     auto step = [&](const unsigned char* K, const unsigned char* V, int k0) {
+        at.keep();
         f32x16 s[BN / 32];
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
             s[u] = ag_zero();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[u] = ag_mfma(ag_row<DP>(K, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s[u]);
+            for (int ks = 0; ks < KS; ++ks) s[u] = ag_mfma(at.rows(K, 32 * u, ks), qf[ks], s[u]);
         }
         if (k0 + BN > lo) {
+            const int left = vis - (k0 + 4 * g);
 #pragma unroll
             for (int u = 0; u < BN / 32; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (k0 + 32 * u + 8 * (e >> 2) + 4 * g + (e & 3) >= vis) s[u][e] = AG_NEG;
+                for (int e = 0; e < 16; ++e) s[u][e] = 32 * u + 8 * (e >> 2) + (e & 3) < left ? s[u][e] : AG_NEG;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -247,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
             for (int h2 = 0; h2 < 2; ++h2) {
                 const s16x8 pf = ag_pack(s[u], h2);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_mfma(ag_tr<DP>(V, 32 * u + 16 * h2, 32 * dt, lane), pf, oacc[dt]);
+                for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_mfma(at.cols(V, 32 * u + 16 * h2, dt), pf, oacc[dt]);
             }
         }
     };
@@ -280,7 +291,7 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
             const int d = 32 * dt + 8 * rq + 4 * g;
-            if (d < a.D) *reinterpret_cast<f32x4*>(po + d) = (f32x4){oacc[dt][4 * rq], oacc[dt][4 * rq + 1], oacc[dt][4 * rq + 2], oacc[dt][4 * rq + 3]};
+            if (32 * dt + 8 * rq < a.D) *reinterpret_cast<f32x4*>(po + d) = (f32x4){oacc[dt][4 * rq], oacc[dt][4 * rq + 1], oacc[dt][4 * rq + 2], oacc[dt][4 * rq + 3]};
         }
     if (g == 0) {
         float* ml = a.ws + (int64_t)a.nsplit * n * a.D + (sp * n + row) * 2;
@@ -289,32 +300,53 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
     }
 }
 
-// O = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M): 32 lanes a row, 4 columns a lane
+// O = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup per row: 32 lanes of 4 columns x 8 threads that share the
+// parts (few rows have many parts, and a chain of dependent reads per part cost more than the attention before it).
 __global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
-    const int64_t n = (int64_t)a.B * a.Sq * a.Hq, row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-    const int d = threadIdx.x % 32 * 4;
-    if (row >= n) return;
+    __shared__ __attribute__((aligned(16))) f32x4 os[8][32];
+    __shared__ float ms[8], ls[8];
+    const int64_t n = (int64_t)a.B * a.Sq * a.Hq, row = blockIdx.x;
+    const int x = threadIdx.x % 32, y = threadIdx.x / 32, d = x * 4;
     const float* ml = a.ws + (int64_t)a.nsplit * n * a.D + row * 2;
-    float M = AG_NEG, l = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) M = __builtin_elementwise_maximum(M, ml[s * n * 2]);
+    float m = AG_NEG, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float ms = ml[s * n * 2], w = ms == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
+    for (int s = y; s < a.nsplit; s += 8) m = __builtin_elementwise_maximum(m, ml[s * n * 2]);
+    for (int s = y; s < a.nsplit; s += 8) {
+        const float mp = ml[s * n * 2], w = mp == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(mp - m);
         l = fmaf(ml[s * n * 2 + 1], w, l);
         if (d < a.D) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(a.ws + (s * n + row) * a.D + d);
+            const f32x4 p = *reinterpret_cast<const f32x4*>(a.ws + (s * n + row) * a.D + d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], w, o[e]);
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(p[e], w, o[e]);
         }
+    }
+    os[y][x] = o;
+    if (x == 0) {
+        ms[y] = m;
+        ls[y] = l;
+    }
+    __syncthreads();
+    if (y > 0) return;
+    m = ms[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = __builtin_elementwise_maximum(m, ms[k]);
+    l = 0.f;
+    o = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float w = ms[k] == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
+        l = fmaf(ls[k], w, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(os[k][x][e], w, o[e]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d < a.D) {
         const u32x2 p = {pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
         *reinterpret_cast<u32x2*>(a.out + row * a.D + d) = p;
     }
-    if (d == 0) {
+    if (x == 0) {
         const int64_t b = row / ((int64_t)a.Sq * a.Hq), ih = row - b * a.Sq * a.Hq, i = ih / a.Hq, h = ih - i * a.Hq;
-        a.lse[(b * a.Hq + h) * a.Sq + i] = l == 0.f ? __builtin_inff() : M + log2f(l);
+        a.lse[(b * a.Hq + h) * a.Sq + i] = l == 0.f ? __builtin_inff() : m + log2f(l);
     }
 }
 
@@ -328,9 +360,9 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int id = ag_xcd(blockIdx.x, gridDim.x);
-    const int t = a.ntiles - 1 - id % a.ntiles, hb = id / a.ntiles;
-    const int b = hb / a.Hq, h = hb - b * a.Hq, hk = h / a.group;
+    const int kv = a.B * a.Hk, units = gridDim.x / a.ntiles;               // units: group x kv
+    const int t = a.ntiles - 1 - blockIdx.x / units, u = blockIdx.x % units;
+    const int b = u % kv / a.Hk, hk = u % kv % a.Hk, h = hk * a.group + u / kv;
     const int klen = ag_klen(a, b);
     const int rw = t * BM + wave * 32, i = min(rw + (lane & 31), a.Sq - 1);
     const int vis = ag_vis(a, i, klen), end = ag_vis(a, min(t * BM + BM, a.Sq) - 1, klen);
@@ -368,27 +400,30 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
     f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_zero();
+    AgLane<DP> at;
+    at.init(lane);
     auto step = [&](const unsigned char* K, const unsigned char* V, int k0) {
+        at.keep();
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
             f32x16 s = ag_zero(), dp = ag_zero();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                s = ag_mfma(ag_row<DP>(K, 32 * u + (lane & 31), 2 * ks + g), qf[ks], s);
-                dp = ag_mfma(ag_row<DP>(V, 32 * u + (lane & 31), 2 * ks + g), gf[ks], dp);
+                s = ag_mfma(at.rows(K, 32 * u, ks), qf[ks], s);
+                dp = ag_mfma(at.rows(V, 32 * u, ks), gf[ks], dp);
             }
-            const bool edge = k0 + 32 * u + 32 > lo;
+            if (k0 + 32 * u + 32 > lo) {
+                const int left = vis - (k0 + 32 * u + 4 * g);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float ds = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (dp[e] - dsum);
-                if (edge) ds = k0 + 32 * u + 8 * (e >> 2) + 4 * g + (e & 3) < vis ? ds : 0.f;
-                s[e] = ds;
+                for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < left ? s[e] : AG_NEG;
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (dp[e] - dsum);
 #pragma unroll
             for (int h2 = 0; h2 < 2; ++h2) {
                 const s16x8 f = ag_pack(s, h2);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_mfma(ag_tr<DP>(K, 32 * u + 16 * h2, 32 * dt, lane), f, acc[dt]);
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_mfma(at.cols(K, 32 * u + 16 * h2, dt), f, acc[dt]);
             }
         }
     };
@@ -415,32 +450,36 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
 // fp32 sums, and ag_add_kernel adds them in order.
 // ---------------------------------------------------------------------------
 template <int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void ag_dkv_kernel(AgArgs a) {
+__global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, BQ = 32, BM = 128;
     __shared__ __attribute__((aligned(16))) unsigned char Q0[BQ * DP * 2], Q1[BQ * DP * 2], G0[BQ * DP * 2], G1[BQ * DP * 2];
-    __shared__ __attribute__((aligned(16))) float L0[BQ], L1[BQ], D0[BQ], D1[BQ];
+    __shared__ __attribute__((aligned(16))) float LD0[128], LD1[128];                 // log-sum-exp (0..), D (64..) of a step's queries
+    __shared__ __attribute__((aligned(16))) unsigned char Vimg[DP == 128 ? BM * DP * 2 : 16];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = ag_xcd(blockIdx.x, gridDim.x);
-    const int sp = id % a.nsplit;
-    id /= a.nsplit;
-    const int t = id % a.ntiles, hb = id / a.ntiles;                       // low keys are seen by the most queries
-    const int b = hb / a.Hk, hk = hb - b * a.Hk;
+    const int kv = a.B * a.Hk, units = gridDim.x / a.ntiles;               // units: nsplit x kv
+    const int t = blockIdx.x / units, u = blockIdx.x % units;              // low keys are seen by the most queries
+    const int b = u % kv / a.Hk, hk = u % kv % a.Hk, sp = u / kv;
     const int klen = ag_klen(a, b);
     const int jw = t * BM + wave * 32, j = jw + (lane & 31), jc = min(j, a.Sk - 1);
     // first query that sees key j: i + 1 + Sk - Sq > j
     const int off = a.Sk - a.Sq;
     const int begin = a.causal ? max(0, t * BM - off) / BQ * BQ : 0;
 
-    s16x8 kf[KS], vf[KS];
-    ag_frags<DP>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
-    ag_frags<DP>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, a.D);
+    // K rows in registers; V rows too for DP = 64, in LDS for DP = 128 (32 registers more would leave one wave a SIMD)
     const bool seen = j < klen;
+    s16x8 kf[KS], vf[DP == 128 ? 1 : KS];
+    ag_frags<DP>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
+    if constexpr (DP == 128) {
+        AgTile<DP, BM, 256> vt;
+        vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, a.D, wave, lane);
+        vt.load(Vimg, t * BM, klen, a.D == DP && t * BM + BM <= klen, wave);
+    } else ag_frags<DP>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, a.D);
     if (!seen) {                                       // padded keys: whatever they hold takes no part
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             kf[ks] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
-            vf[ks] = kf[ks];
+            if constexpr (DP == 64) vf[ks] = kf[ks];
         }
     }
     f32x16 dk[DT], dv[DT];
@@ -455,42 +494,52 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void ag_dkv_kernel(AgArgs a)
     AgTile<DP, BQ, 256> qt, gt;
     qt.init(a.q + b * a.q_bs, a.q_ss, a.D, wave, lane);
     gt.init(a.dO + (int64_t)b * a.Sq * a.Hq * a.D, (int64_t)a.Hq * a.D, a.D, wave, lane);
-    const u16 *qs = qt.src, *gs = gt.src;
-    auto fetch = [&](unsigned char* Q, unsigned char* G, float* L, float* Dm, int n) {
-        const int h = hk * a.group + n / steps, q0 = begin + n % steps * BQ;
+    const char *qs = qt.base, *gs = gt.base;
+    int fh = steps ? n0 / steps : 0, fq = steps ? n0 % steps : 0, sq = fq;      // next step to fetch (head of the group, step), to compute
+    auto fetch = [&](unsigned char* Q, unsigned char* G, float* LD) {
+        const int h = hk * a.group + fh, q0 = begin + fq * BQ;
         const bool full = a.D == DP && q0 + BQ <= a.Sq;
-        qt.src = qs + h * a.q_hs;
-        gt.src = gs + (int64_t)h * a.D;
+        qt.base = qs + h * a.q_hs * 2;
+        gt.base = gs + (int64_t)h * a.D * 2;
         qt.load(Q, q0, a.Sq, full, wave);
         gt.load(G, q0, a.Sq, full, wave);
-        if (tid < BQ) {
-            const int64_t li = ((int64_t)b * a.Hq + h) * a.Sq + q0 + tid;
-            const bool in = q0 + tid < a.Sq;
-            L[tid] = in ? a.lse[li] : __builtin_inff();
-            Dm[tid] = in ? a.dsum[li] : 0.f;
+        if (wave < 2) {                                // no query: log-sum-exp +inf (P = 0) and D 0
+            const float* from = (wave ? a.dsum : a.lse) + ((int64_t)b * a.Hq + h) * a.Sq + q0 + lane;
+            if (q0 + lane >= a.Sq) from = wave ? reinterpret_cast<const float*>(&ag_zeros) : &ag_inf;
+            __builtin_amdgcn_global_load_lds((ag_glb_void*)from, (ag_lds_void*)(LD + wave * 64), 4, 0, 0);
+        }
+        if (++fq == steps) {
+            fq = 0;
+            ++fh;
         }
     };
-    auto step = [&](const unsigned char* Q, const unsigned char* G, const float* L, const float* Dm, int n) {
-        const int q0 = begin + n % steps * BQ;
+    AgLane<DP> at;
+    at.init(lane);
+    auto step = [&](const unsigned char* Q, const unsigned char* G, const float* LD) {
+        at.keep();
+        const int q0 = begin + sq * BQ;
+        if (++sq == steps) sq = 0;
         if (a.causal && q0 + BQ - 1 + off < jw) return;                    // no query of the step sees this wave's keys
         f32x16 s = ag_zero(), dp = ag_zero();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            s = ag_mfma(ag_row<DP>(Q, lane & 31, 2 * ks + g), kf[ks], s);
-            dp = ag_mfma(ag_row<DP>(G, lane & 31, 2 * ks + g), vf[ks], dp);
+            s = ag_mfma(at.rows(Q, 0, ks), kf[ks], s);
+            dp = ag_mfma(at.rows(G, 0, ks), DP == 128 ? at.rows(Vimg, wave * 32, ks) : vf[DP == 128 ? 0 : ks], dp);
         }
-        const bool edge = (a.causal && q0 + off < jw + 31) || jw + 32 > klen;
+        if ((a.causal && q0 + off < jw + 31) || jw + 32 > klen) {          // some (query, key) of the tile is not seen
+            const int from = !seen ? 0x7fffffff : a.causal ? j - off - q0 - 4 * g : -1;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[x] = 8 * (x >> 2) + (x & 3) >= from ? s[x] : AG_NEG;
+        }
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(L + 8 * rq + 4 * g);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(Dm + 8 * rq + 4 * g);
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(LD + 8 * rq + 4 * g);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(LD + 64 + 8 * rq + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int x = 4 * rq + e;
-                float p = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale_log2e, -l4[e]));
-                if (edge) p = seen && (!a.causal || q0 + 8 * rq + 4 * g + e + off >= j) ? p : 0.f;
-                s[x] = p;
-                dp[x] = p * (dp[x] - d4[e]);
+                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale_log2e, -l4[e]));
+                dp[x] = s[x] * (dp[x] - d4[e]);
             }
         }
 #pragma unroll
@@ -498,22 +547,22 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void ag_dkv_kernel(AgArgs a)
             const s16x8 pf = ag_pack(s, h2), df = ag_pack(dp, h2);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                dv[dt] = ag_mfma(ag_tr<DP>(G, 16 * h2, 32 * dt, lane), pf, dv[dt]);
-                dk[dt] = ag_mfma(ag_tr<DP>(Q, 16 * h2, 32 * dt, lane), df, dk[dt]);
+                dv[dt] = ag_mfma(at.cols(G, 16 * h2, dt), pf, dv[dt]);
+                dk[dt] = ag_mfma(at.cols(Q, 16 * h2, dt), df, dk[dt]);
             }
         }
     };
-    if (n0 < n1) fetch(Q0, G0, L0, D0, n0);
+    if (n0 < n1) fetch(Q0, G0, LD0);
     AG_LANDED();
     __syncthreads();
     for (int n = n0; n < n1; n += 2) {
-        if (n + 1 < n1) fetch(Q1, G1, L1, D1, n + 1);
-        step(Q0, G0, L0, D0, n);
+        if (n + 1 < n1) fetch(Q1, G1, LD1);
+        step(Q0, G0, LD0);
         AG_LANDED();
         __syncthreads();
         if (n + 1 >= n1) break;
-        if (n + 2 < n1) fetch(Q0, G0, L0, D0, n + 2);
-        step(Q1, G1, L1, D1, n + 1);
+        if (n + 2 < n1) fetch(Q0, G0, LD0);
+        step(Q1, G1, LD1);
         AG_LANDED();
         __syncthreads();
     }
@@ -531,7 +580,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void ag_dkv_kernel(AgArgs a)
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
             const int d = 32 * dt + 8 * rq + 4 * g;
-            if (d < a.D) {
+            if (32 * dt + 8 * rq < a.D) {
                 *reinterpret_cast<f32x4*>(pk + d) = (f32x4){dk[dt][4 * rq], dk[dt][4 * rq + 1], dk[dt][4 * rq + 2], dk[dt][4 * rq + 3]};
                 *reinterpret_cast<f32x4*>(pk + n + d) = (f32x4){dv[dt][4 * rq], dv[dt][4 * rq + 1], dv[dt][4 * rq + 2], dv[dt][4 * rq + 3]};
             }
@@ -556,6 +605,9 @@ static int ag_check(const AgArgs& a, const int64_t* st, int nst) {
     if (a.D < 8 || a.D > 128 || a.D % 8) return -70;
     for (int i = 0; i < nst; ++i)
         if (st[i] & 7) return -17;
+    for (int i = 1; i < nst; i += 3)
+        if (st[i] < 0 || st[i] >= (1 << 25)) return -74;
+    if ((int64_t)a.Hq * a.D >= (1 << 25)) return -74;
     return 0;
 }
 
@@ -565,10 +617,9 @@ static int ag_grid(int64_t n, int* out) {
     return 0;
 }
 
-// Workgroups that share a tile: enough for AG_FILL workgroups (two a CU), no fewer than `least` steps each.
-#define AG_FILL 512
-static int ag_splits(int64_t grid, int64_t steps, int least) {
-    int64_t n = AG_FILL / grid, most = steps / least;
+// Workgroups that share a tile: enough for `fill` workgroups, no fewer than `least` steps each.
+static int ag_splits(int64_t grid, int64_t steps, int least, int fill) {
+    int64_t n = fill / grid, most = steps / least;
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
@@ -581,11 +632,12 @@ static bool ag_pack_rows(int Sq, int group) {
 static int ag_fwd_splits(int B, int Sq, int Sk, int Hq, int Hk) {
     const bool pack = ag_pack_rows(Sq, Hq / Hk);
     const int64_t rows = pack ? (int64_t)(Hq / Hk) * Sq : Sq;
-    return ag_splits((int64_t)B * (pack ? Hk : Hq) * ((rows + 127) / 128), (Sk + 63) / 64, 4);
+    return ag_splits((int64_t)B * (pack ? Hk : Hq) * ((rows + 127) / 128), (Sk + 63) / 64, 4, 512);
 }
 
-static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk) {
-    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), (int64_t)((Sq + 31) / 32) * (Hq / Hk), 8);
+// (512 workgroups are resident; causal tiles differ in length, so the longest should be no more than what a slot gets in all)
+static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int causal) {
+    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), (int64_t)((Sq + 31) / 32) * (Hq / Hk), 8, causal ? 1024 : 512);
 }
 
 extern "C" {
@@ -596,8 +648,8 @@ int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
     return n > 1 ? n * B * Sq * Hq * (D + 2) : 0;
 }
 
-int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
-    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk);
+int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
+    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, causal);
     return n > 1 ? n * 2 * B * Sk * Hk * D : 0;
 }
 
@@ -630,7 +682,7 @@ int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, f
     }
     DTF_CHECK_LAUNCH();
     if (a.nsplit > 1) {
-        if ((rc = ag_grid(((int64_t)B * Sq * Hq + 7) / 8, &grid))) return rc;
+        if ((rc = ag_grid((int64_t)B * Sq * Hq, &grid))) return rc;
         hipLaunchKernelGGL(ag_join_kernel, dim3(grid), dim3(256), 0, stream, a);
         DTF_CHECK_LAUNCH();
     }
@@ -655,7 +707,7 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)do_) | ((uintptr_t)dq) |
          ((uintptr_t)dk) | ((uintptr_t)dv) | ((uintptr_t)ws)) & 15) return -16;
     a.group = Hq / Hk;
-    const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk);
+    const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk, causal);
     if (splits > 1 && !ws) return -73;
     if ((int64_t)((Sq + 31) / 32) * a.group > 0x7fffffff) return -72;
     a.ntiles = (Sq - 1) / 128 + 1;

@@ -32,28 +32,49 @@ struct RnArgs {
 template <int DT, bool VEC, int TPR, int NE>
 struct RnRow {
     static constexpr int V = DT == DTF_BF16 ? 8 : 4;
+    struct Raw {                          // as it comes from memory
+        u32x4 q[VEC ? NE / V : 1];
+        float f[VEC ? 1 : NE];
+    };
     static __device__ __forceinline__ int col(int l, int e) { return VEC ? ((e / V) * TPR + l) * V + e % V : e * TPR + l; }
-    static __device__ __forceinline__ void load(const void* base, int64_t off, int H, int l, float (&v)[NE]) {
+    // off (elements): where the row begins, uniform in a wave -- so the address is a scalar base and a 32-bit lane offset
+    static __device__ __forceinline__ void fetch(const void* base, int64_t off, int H, int l, Raw& r) {
+        const char* p = reinterpret_cast<const char*>(base) + off * (16 / V);
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < NE / V; ++c) {
                 const int at = (c * TPR + l) * V;
-                u32x4 q = {0u, 0u, 0u, 0u};
-                if (at < H) q = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + (off + at) * (16 / V));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if constexpr (DT == DTF_BF16) {
-                        v[c * V + 2 * k] = __uint_as_float(q[k] << 16);
-                        v[c * V + 2 * k + 1] = __uint_as_float(q[k] & 0xffff0000u);
-                    } else v[c * V + k] = __uint_as_float(q[k]);
-                }
+                r.q[c] = (u32x4){0u, 0u, 0u, 0u};
+                if (at < H) r.q[c] = *reinterpret_cast<const u32x4*>(p + (unsigned)(at * (16 / V)));
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < NE; ++e) v[e] = e * TPR + l < H ? load1<DT>(base, off + e * TPR + l) : 0.f;
+            for (int e = 0; e < NE; ++e) r.f[e] = e * TPR + l < H ? load1<DT>(p + (unsigned)((e * TPR + l) * (16 / V)), 0) : 0.f;
         }
     }
+    static __device__ __forceinline__ void expand(const Raw& r, float (&v)[NE]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < NE / V; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == DTF_BF16) {
+                        v[c * V + 2 * k] = __uint_as_float(r.q[c][k] << 16);
+                        v[c * V + 2 * k + 1] = __uint_as_float(r.q[c][k] & 0xffff0000u);
+                    } else v[c * V + k] = __uint_as_float(r.q[c][k]);
+                }
+        } else {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) v[e] = r.f[e];
+        }
+    }
+    static __device__ __forceinline__ void load(const void* base, int64_t off, int H, int l, float (&v)[NE]) {
+        Raw r;
+        fetch(base, off, H, l, r);
+        expand(r, v);
+    }
     static __device__ __forceinline__ void store(void* base, int64_t off, int H, int l, const float (&v)[NE]) {
+        char* p = reinterpret_cast<char*>(base) + off * (16 / V);
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < NE / V; ++c) {
@@ -64,19 +85,16 @@ struct RnRow {
                     if constexpr (DT == DTF_BF16) q[k] = pack_bf16x2(v[c * V + 2 * k], v[c * V + 2 * k + 1]);
                     else q[k] = __float_as_uint(v[c * V + k]);
                 }
-                if (at < H) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(base) + (off + at) * (16 / V)) = q;
+                if (at < H) *reinterpret_cast<u32x4*>(p + (unsigned)(at * (16 / V))) = q;
             }
         } else {
 #pragma unroll
             for (int e = 0; e < NE; ++e)
-                if (e * TPR + l < H) store1<DT>(base, off + e * TPR + l, v[e]);
+                if (e * TPR + l < H) store1<DT>(p + (unsigned)((e * TPR + l) * (16 / V)), 0, v[e]);
         }
     }
-    // a parameter row of type wdt (the activations' type or fp32); absent: `missing`
-    static __device__ __forceinline__ void param(const void* p, int wdt, int H, int l, float missing, float (&v)[NE]) {
-#pragma unroll
-        for (int e = 0; e < NE; ++e) v[e] = missing;
-        if (!p) return;
+    // a parameter row of type wdt (the activations' type or fp32)
+    static __device__ __forceinline__ void param(const void* p, int wdt, int H, int l, float (&v)[NE]) {
         if (wdt == DT) load(p, 0, H, l, v);
         else {
 #pragma unroll
@@ -85,23 +103,38 @@ struct RnRow {
     }
 };
 
-// sums of a and b over the TPR threads of a row; `red` alternates between two halves, one barrier a call
-template <int TPR>
-__device__ __forceinline__ void rn_sum2(float& a, float& b, float (*red)[2][16], int& flip) {
-    a = wave_sum(a);
-    b = wave_sum(b);
+// sum over a wave, in every lane: inside rows of 16 by DPP (no trip through the LDS crossbar as a shuffle makes), then
+// across the four rows
+__device__ __forceinline__ float rn_wave_sum(float v) {
+#define RN_DPP(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
+    RN_DPP(0xB1);       // quad_perm 1 0 3 2
+    RN_DPP(0x4E);       // quad_perm 2 3 0 1
+    RN_DPP(0x141);      // row_half_mirror
+    RN_DPP(0x140);      // row_mirror
+#undef RN_DPP
+    const int i = __float_as_int(v);
+    return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
+           (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
+}
+
+// sum of a (and of b) over the TPR threads of a row; `red` alternates between two halves, one barrier a call
+template <int TPR, bool TWO>
+__device__ __forceinline__ void rn_sum(float& a, float& b, float (*red)[2][16], int& flip) {
+    a = rn_wave_sum(a);
+    if constexpr (TWO) b = rn_wave_sum(b);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6, w0 = wave & ~(TPR / 64 - 1);
         if ((threadIdx.x & 63) == 0) {
             red[flip][0][wave] = a;
-            red[flip][1][wave] = b;
+            if constexpr (TWO) red[flip][1][wave] = b;
         }
         __syncthreads();
-        a = b = 0.f;
+        a = 0.f;
+        if constexpr (TWO) b = 0.f;
 #pragma unroll
         for (int i = 0; i < TPR / 64; ++i) {
             a += red[flip][0][w0 + i];
-            b += red[flip][1][w0 + i];
+            if constexpr (TWO) b += red[flip][1][w0 + i];
         }
         flip ^= 1;
     }
@@ -117,7 +150,7 @@ __device__ __forceinline__ void rn_normalise(float (&v)[NE], int H, int l, float
     if (layer) {
 #pragma unroll
         for (int e = 0; e < NE; ++e) s += v[e];
-        rn_sum2<TPR>(s, z, red, flip);
+        rn_sum<TPR, false>(s, z, red, flip);
         mean = s * inv;
 #pragma unroll
         for (int e = 0; e < NE; ++e) v[e] = R::col(l, e) < H ? v[e] - mean : 0.f;
@@ -125,7 +158,7 @@ __device__ __forceinline__ void rn_normalise(float (&v)[NE], int H, int l, float
     s = z = 0.f;
 #pragma unroll
     for (int e = 0; e < NE; ++e) s = fmaf(v[e], v[e], s);
-    rn_sum2<TPR>(s, z, red, flip);
+    rn_sum<TPR, false>(s, z, red, flip);
     rstd = 1.f / sqrtf(s * inv + eps);
 #pragma unroll
     for (int e = 0; e < NE; ++e) v[e] *= rstd;
@@ -137,7 +170,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(RnArgs a)
     constexpr int RB = TPR < 256 ? 256 / TPR : 1;
     __shared__ float red[2][2][16];
     const int l = threadIdx.x % TPR, H = a.H;
-    const int64_t want = (int64_t)blockIdx.x * RB + threadIdx.x / TPR;
+    const int64_t want = (int64_t)blockIdx.x * RB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
     const int64_t row = want < a.M ? want : a.M - 1;           // spare rows of the last workgroup redo its last, unstored
     int flip = 0;
     float v[NE], p[NE], mean, rstd;
@@ -151,11 +184,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(RnArgs a)
                 a.stats[2 * a.M + row] = mean;
                 a.stats[3 * a.M + row] = rstd;
             }
-            R::param(a.pw, a.wdt, H, l, 1.f, p);
+            R::param(a.pw, a.wdt, H, l, p);
 #pragma unroll
             for (int e = 0; e < NE; ++e) n[e] *= p[e];
             if (a.pb) {
-                R::param(a.pb, a.wdt, H, l, 0.f, p);
+                R::param(a.pb, a.wdt, H, l, p);
 #pragma unroll
                 for (int e = 0; e < NE; ++e) n[e] += p[e];
             }
@@ -174,29 +207,33 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(RnArgs a)
         a.stats[row] = mean;
         a.stats[a.M + row] = rstd;
     }
-    R::param(a.w, a.wdt, H, l, 1.f, p);
+    R::param(a.w, a.wdt, H, l, p);
 #pragma unroll
     for (int e = 0; e < NE; ++e) v[e] *= p[e];
     if (a.b) {
-        R::param(a.b, a.wdt, H, l, 0.f, p);
+        R::param(a.b, a.wdt, H, l, p);
 #pragma unroll
         for (int e = 0; e < NE; ++e) v[e] += p[e];
     }
     if (want < a.M) R::store(a.y, row * H, H, l, v);
 }
 
-template <int DT, bool VEC, int TPR, int NE, bool LAYER>
+// A workgroup walks its rows with the next row's loads in flight and the parameters in registers (read again per row, they
+// cost a cache's latency between the two reductions).  SAME: parameters of the activations' type; else (fp32 parameters of
+// bf16 activations) they are read per row.
+template <int DT, bool VEC, int TPR, int NE, bool LAYER, bool SAME>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a) {
     typedef RnRow<DT, VEC, TPR, NE> R;
     constexpr int NT = TPR < 256 ? 256 : TPR, RB = NT / TPR;
     __shared__ float red[2][2][16];
     __shared__ float comb[RB > 1 ? NT * NE : 1];
-    const int l = threadIdx.x % TPR, slot = threadIdx.x / TPR, H = a.H;
+    const int l = threadIdx.x % TPR, slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), H = a.H;
     const int64_t group = blockIdx.x / a.nbx;
     const int bx = blockIdx.x - (int)group * a.nbx;
     const int64_t r0 = group * a.group_rows;
     const int64_t r1 = r0 + a.group_rows < a.M ? r0 + a.group_rows : a.M;
     const float inv = 1.f / (float)H;
+    const bool each = a.gate && a.rpg == 1;                    // a gate row per row, streamed like x
     int flip = 0;
     float sw[NE], sb[LAYER ? NE : 1], spw[NE], spb[LAYER ? NE : 1], sg[NE];
 #pragma unroll
@@ -205,52 +242,87 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
 #pragma unroll
         for (int e = 0; e < NE; ++e) sb[e] = spb[e] = 0.f;
     }
-    for (int64_t base = r0 + (int64_t)bx * RB; base < r1; base += (int64_t)a.nbx * RB) {     // (uniform in the workgroup)
+    typename R::Raw wr, pwr, pbr, gr, xr, hr, dyr, drr;
+    if constexpr (SAME) {
+        R::fetch(a.w, 0, H, l, wr);
+        if (a.pw) R::fetch(a.pw, 0, H, l, pwr);
+        if (LAYER && a.pb) R::fetch(a.pb, 0, H, l, pbr);
+    }
+    if (a.gate && !each) R::fetch(a.gate, r0 / a.rpg * H, H, l, gr);
+    auto row_at = [&](int64_t base) { return base + slot < r1 ? base + slot : r1 - 1; };      // spare rows redo the last, unstored
+    float mean = 0.f, rstd = 1.f, pmean = 0.f, prstd = 1.f;
+    auto fetch = [&](int64_t row) {
+        R::fetch(a.x, row * H, H, l, xr);
+        if (a.h) R::fetch(a.h, row * H, H, l, hr);
+        if (each) R::fetch(a.gate, row * H, H, l, gr);
+        if (a.dy) R::fetch(a.dy, row * H, H, l, dyr);
+        if (a.dr) R::fetch(a.dr, row * H, H, l, drr);
+        if (LAYER) mean = a.stats[row];
+        rstd = a.stats[a.M + row];
+        if (a.pw) {
+            if (LAYER) pmean = a.stats[2 * a.M + row];
+            prstd = a.stats[3 * a.M + row];
+        }
+    };
+    const int64_t first = r0 + (int64_t)bx * RB, stride = (int64_t)a.nbx * RB;
+    if (first < r1) fetch(row_at(first));
+    for (int64_t base = first; base < r1; base += stride) {    // (uniform in the workgroup)
         const bool valid = base + slot < r1;
-        const int64_t row = valid ? base + slot : r1 - 1;
+        const int64_t row = row_at(base);
         const float live = valid ? 1.f : 0.f;
-        float v[NE], n[NE], dr[NE], t[NE], p[NE];
-        R::load(a.x, row * H, H, l, v);
-        const float mean = LAYER ? a.stats[row] : 0.f, rstd = a.stats[a.M + row];
-        float pmean = 0.f, prstd = 1.f;
+        const float mu = mean, rs = rstd, pmu = pmean, prs = prstd;
+        float v[NE], n[NE], dr[NE], dy[NE], g[NE], p[NE];
+        R::expand(xr, v);
+        if (a.h) R::expand(hr, n);
+        if (a.gate) R::expand(gr, g);
+        if (a.dy) R::expand(dyr, dy);
+        if (a.dr) R::expand(drr, dr);
+        else {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) dr[e] = 0.f;
+        }
+        if (base + stride < r1) fetch(row_at(base + stride));
+        auto pre_w = [&]() {
+            if constexpr (SAME) R::expand(wr, p);
+            else R::param(a.w, a.wdt, H, l, p);
+        };
+        auto post_w = [&]() {
+            if constexpr (SAME) R::expand(pwr, p);
+            else R::param(a.pw, a.wdt, H, l, p);
+        };
+        auto normed = [&](float (&t)[NE]) {                    // n of the forward: h, or post's result from n = hhat
+#pragma unroll
+            for (int e = 0; e < NE; ++e) t[e] = n[e];
+            if (!a.pw) return;
+            post_w();
+#pragma unroll
+            for (int e = 0; e < NE; ++e) t[e] *= p[e];
+            if (LAYER && a.pb) {
+                if constexpr (SAME) R::expand(pbr, p);
+                else R::param(a.pb, a.wdt, H, l, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) t[e] += p[e];
+            }
+        };
         if (a.h) {
-            R::load(a.h, row * H, H, l, n);                    // n: hhat with a post norm, h without
             if (a.pw) {
-                if (LAYER) pmean = a.stats[2 * a.M + row];
-                prstd = a.stats[3 * a.M + row];
 #pragma unroll
-                for (int e = 0; e < NE; ++e) n[e] = R::col(l, e) < H ? (n[e] - pmean) * prstd : 0.f;
-                R::param(a.pw, a.wdt, H, l, 1.f, p);
-#pragma unroll
-                for (int e = 0; e < NE; ++e) t[e] = n[e] * p[e];
-                if (a.pb) {
-                    R::param(a.pb, a.wdt, H, l, 0.f, p);
-#pragma unroll
-                    for (int e = 0; e < NE; ++e) t[e] += p[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < NE; ++e) t[e] = n[e];
+                for (int e = 0; e < NE; ++e) n[e] = R::col(l, e) < H ? (n[e] - pmu) * prs : 0.f;
             }
+            float t[NE];
+            normed(t);
             if (a.gate) {
-                R::load(a.gate, row / a.rpg * H, H, l, p);
 #pragma unroll
-                for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, t[e] * p[e], v[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, t[e], v[e]);
+                for (int e = 0; e < NE; ++e) t[e] *= g[e];
             }
+#pragma unroll
+            for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, t[e], v[e]);
         }
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            v[e] = R::col(l, e) < H ? (v[e] - mean) * rstd : 0.f;        // rhat
-            dr[e] = 0.f;
-        }
-        if (a.dr) R::load(a.dr, row * H, H, l, dr);
+        for (int e = 0; e < NE; ++e) v[e] = R::col(l, e) < H ? (v[e] - mu) * rs : 0.f;        // rhat
         if (a.dy) {
-            float dy[NE], c1 = 0.f, c2 = 0.f;
-            R::load(a.dy, row * H, H, l, dy);
-            R::param(a.w, a.wdt, H, l, 1.f, p);
+            float c1 = 0.f, c2 = 0.f;
+            pre_w();
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
                 sw[e] = fmaf(live * dy[e], v[e], sw[e]);
@@ -259,33 +331,33 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
                 c1 = fmaf(dy[e], v[e], c1);
                 if constexpr (LAYER) c2 += dy[e];
             }
-            rn_sum2<TPR>(c1, c2, red, flip);
+            rn_sum<TPR, LAYER>(c1, c2, red, flip);
             c1 *= inv;
             c2 *= inv;
 #pragma unroll
-            for (int e = 0; e < NE; ++e) dr[e] = fmaf(rstd, dy[e] - v[e] * c1 - c2, dr[e]);
+            for (int e = 0; e < NE; ++e) dr[e] = fmaf(rs, dy[e] - v[e] * c1 - c2, dr[e]);
         }
         if (valid) R::store(a.dx, row * H, H, l, dr);
         if (!a.h) continue;
 #pragma unroll
         for (int e = 0; e < NE; ++e) dr[e] *= a.scale;
         if (a.gate) {
-            // t: n of the forward; p: gate (both again, after the registers served dy)
+            float t[NE];
+            normed(t);
 #pragma unroll
             for (int e = 0; e < NE; ++e) t[e] *= dr[e];
-            if (a.dgate) {
+            if (each) {
                 if (valid) R::store(a.dgate, row * H, H, l, t);
             } else {
 #pragma unroll
                 for (int e = 0; e < NE; ++e) sg[e] = fmaf(live, t[e], sg[e]);
             }
-            R::load(a.gate, row / a.rpg * H, H, l, p);
 #pragma unroll
-            for (int e = 0; e < NE; ++e) dr[e] *= p[e];                  // dn
+            for (int e = 0; e < NE; ++e) dr[e] *= g[e];                  // dn
         }
         if (a.pw) {
             float c1 = 0.f, c2 = 0.f;
-            R::param(a.pw, a.wdt, H, l, 1.f, p);
+            post_w();
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
                 if (R::col(l, e) >= H) dr[e] = 0.f;
@@ -295,11 +367,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
                 c1 = fmaf(dr[e], n[e], c1);
                 if constexpr (LAYER) c2 += dr[e];
             }
-            rn_sum2<TPR>(c1, c2, red, flip);
+            rn_sum<TPR, LAYER>(c1, c2, red, flip);
             c1 *= inv;
             c2 *= inv;
 #pragma unroll
-            for (int e = 0; e < NE; ++e) dr[e] = prstd * (dr[e] - n[e] * c1 - c2);
+            for (int e = 0; e < NE; ++e) dr[e] = prs * (dr[e] - n[e] * c1 - c2);
         }
         if (a.dh && valid) R::store(a.dh, row * H, H, l, dr);
     }
@@ -367,11 +439,17 @@ __global__ __launch_bounds__(1024) void rn_sum_kernel(RnSumArgs a) {
     }
 }
 
-static int rn_tpr(int H) { return H <= 1024 ? 64 : H <= 2048 ? 128 : H <= 4096 ? 256 : H <= 8192 ? 512 : 1024; }
+// Threads of a row.  Forward 16 elements a thread.  Backward 8 (its sums and the next row's loads take the registers), but
+// no more than 512 threads to H = 8192: 1024 threads leave 128 registers each, which spill.
+static int rn_tpr(int H, int ne) {
+    if (H <= 512) return 64;
+    if (H > 8192) return 1024;
+    return H <= 64 * ne ? 64 : H <= 128 * ne ? 128 : H <= 256 * ne ? 256 : 512;
+}
 
 static int rn_blocks(int64_t rows, int H, int64_t groups) {
-    const int tpr = rn_tpr(H), rb = tpr < 256 ? 256 / tpr : 1;
-    const int64_t target = tpr <= 256 ? 512 : 256;
+    const int tpr = rn_tpr(H, 8), rb = tpr < 256 ? 256 / tpr : 1;
+    const int64_t target = tpr <= 256 ? 1024 : H <= 4096 ? 512 : 256;      // what the card holds at once: 16 waves a CU, 8 above H = 4096
     int64_t n = target / groups, most = (rows + rb - 1) / rb;
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
@@ -384,15 +462,19 @@ int64_t dtf_residual_norm_ws(int64_t M, int H, int64_t groups, int narr) {
     return groups * rn_blocks((M + groups - 1) / groups, H, groups) * narr * H;
 }
 
-#define RN_BY_SHAPE(X, DTY, VECT)                                                                 \
+#define RN_SHAPES_FWD(X, DTY, VECT)                                                               \
     if (H <= 512) { X(DTY, VECT, 64, 8) } else if (H <= 1024) { X(DTY, VECT, 64, 16) }            \
     else if (H <= 2048) { X(DTY, VECT, 128, 16) } else if (H <= 4096) { X(DTY, VECT, 256, 16) }   \
     else if (H <= 8192) { X(DTY, VECT, 512, 16) } else { X(DTY, VECT, 1024, 16) }
-#define RN_DISPATCH(X)                                                        \
+#define RN_SHAPES_BWD(X, DTY, VECT)                                                               \
+    if (H <= 512) { X(DTY, VECT, 64, 8) } else if (H <= 1024) { X(DTY, VECT, 128, 8) }            \
+    else if (H <= 2048) { X(DTY, VECT, 256, 8) } else if (H <= 4096) { X(DTY, VECT, 512, 8) }     \
+    else if (H <= 8192) { X(DTY, VECT, 512, 16) } else { X(DTY, VECT, 1024, 16) }
+#define RN_DISPATCH(SHAPES, X)                                                \
     if (dt == DTF_BF16) {                                                     \
-        if (vec) { RN_BY_SHAPE(X, DTF_BF16, true) } else { RN_BY_SHAPE(X, DTF_BF16, false) } \
+        if (vec) { SHAPES(X, DTF_BF16, true) } else { SHAPES(X, DTF_BF16, false) } \
     } else {                                                                  \
-        if (vec) { RN_BY_SHAPE(X, DTF_F32, true) } else { RN_BY_SHAPE(X, DTF_F32, false) }   \
+        if (vec) { SHAPES(X, DTF_F32, true) } else { SHAPES(X, DTF_F32, false) }   \
     }
 
 static int rn_check(int dt, int wdt, int64_t M, int H, int64_t rpg) {
@@ -415,12 +497,12 @@ int dtf_residual_norm_fwd(const void* x, const void* h, const void* gate, const 
     const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)b | (uintptr_t)pw |
                          (uintptr_t)pb | (uintptr_t)y | (uintptr_t)r;
     const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
-    const int tpr = rn_tpr(H), nt = tpr < 256 ? 256 : tpr, rb = nt / tpr;
+    const int tpr = rn_tpr(H, 16), nt = tpr < 256 ? 256 : tpr, rb = nt / tpr;
     const int64_t grid = (M + rb - 1) / rb;
     if (grid > 0x7fffffff) return -92;
 #define RN_FWD(DTY, VECT, TPR, NE) \
     hipLaunchKernelGGL((rn_fwd_kernel<DTY, VECT, TPR, NE>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
-    RN_DISPATCH(RN_FWD)
+    RN_DISPATCH(RN_SHAPES_FWD, RN_FWD)
 #undef RN_FWD
     DTF_CHECK_LAUNCH();
     return 0;
@@ -460,14 +542,18 @@ int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const 
     const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)pw | (uintptr_t)pb |
                          (uintptr_t)dy | (uintptr_t)dr | (uintptr_t)dx | (uintptr_t)dh | (uintptr_t)a.dgate;
     const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
-    const int tpr = rn_tpr(H), nt = tpr < 256 ? 256 : tpr;
+    const int tpr = rn_tpr(H, 8), nt = tpr < 256 ? 256 : tpr;
     const int64_t grid = groups * a.nbx;
     if (grid > 0x7fffffff) return -92;
-#define RN_BWD(DTY, VECT, TPR, NE)                                                                                              \
-    if (layer) hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, true>), dim3((unsigned)grid), dim3(nt), 0, stream, a);     \
-    else hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, false>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
-    RN_DISPATCH(RN_BWD)
+#define RN_BWD_L(DTY, VECT, TPR, NE, SM)                                                                                         \
+    if (layer) hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, true, SM>), dim3((unsigned)grid), dim3(nt), 0, stream, a);  \
+    else hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, false, SM>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
+#define RN_BWD(DTY, VECT, TPR, NE)                                                        \
+    if (DTY == DTF_F32 || wdt == DTY) { RN_BWD_L(DTY, VECT, TPR, NE, true) }               \
+    else { RN_BWD_L(DTY, VECT, TPR, NE, false) }
+    RN_DISPATCH(RN_SHAPES_BWD, RN_BWD)
 #undef RN_BWD
+#undef RN_BWD_L
     DTF_CHECK_LAUNCH();
     if (s.n == 0) return 0;
     s.part = ws; s.H = H; s.narr = s.n;

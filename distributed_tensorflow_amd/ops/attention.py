@@ -115,7 +115,7 @@ def _general_kernels():
         P, I, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
         L = ctypes.c_int64
         _general = (hip.declare("dtf_attn_general_fwd", [P] * 7 + [I] * 7 + [Fl, P, P]),
-                    hip.declare("dtf_attn_general_bwd", [P] * 12 + [I] * 7 + [Fl, P, P]),
+                    hip.declare("dtf_attn_general_bwd", [P] * 11 + [I] * 7 + [Fl, P, P]),
                     hip.declare("dtf_attn_general_fwd_ws", [I] * 6, L), hip.declare("dtf_attn_general_bwd_ws", [I] * 7, L))
     return _general
 
@@ -128,41 +128,46 @@ def _operand(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _workspace(like, floats):
-    return like.new_empty(floats, dtype=torch.float32) if floats else None
-
-
 def _general_strides(*tensors):
     return (ctypes.c_int64 * (3 * len(tensors)))(*(0 if n == 1 else s for t in tensors for n, s in zip(t.shape[:3], t.stride())))
+
+
+def _general_forward(q, k, v, kv_len, causal, scale):
+    """-> (q, k, v as the kernels read them, out, log-sum-exp, the launch's remaining arguments)."""
+    q, k, v = _operand(q), _operand(k), _operand(v)
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    o = q.new_empty(q.shape)
+    lse = q.new_empty((B, Hq, Sq), dtype=torch.float32)
+    fwd, _, ws_floats, _ = _general_kernels()
+    n = ws_floats(B, Sq, Sk, Hq, Hk, D)
+    ws = lse.new_empty(n) if n else None
+    how = _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
+    rc = hip.launch(q, fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), hip.ptr(ws), *how)
+    hip.check(rc, "dtf_attn_general_fwd")
+    return q, k, v, o, lse, how
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_len, causal, scale):
-        q, k, v = _operand(q), _operand(k), _operand(v)
-        B, Sq, Hq, D = q.shape
-        Sk, Hk = k.shape[1], k.shape[2]
-        o = q.new_empty(q.shape)
-        lse = q.new_empty((B, Hq, Sq), dtype=torch.float32)
-        fwd, _, ws_floats, _ = _general_kernels()
-        ws = _workspace(q, ws_floats(B, Sq, Sk, Hq, Hk, D))
-        ctx.how = _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
-        rc = hip.launch(q, fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), hip.ptr(ws), *ctx.how)
-        hip.check(rc, "dtf_attn_general_fwd")
+        q, k, v, o, lse, ctx.how = _general_forward(q, k, v, kv_len, causal, scale)
         ctx.save_for_backward(q, k, v, o, lse, kv_len)
         return o
 
     @staticmethod
     @hip.first_order
     def backward(ctx, do):
-        q, k, v, o, lse, _ = ctx.saved_tensors
+        q, k, v, o, lse, kv_len = ctx.saved_tensors
+        st, B, Sq, Sk, Hq, Hk, D, causal, scale, _ = ctx.how
         if not do.is_contiguous() or do.data_ptr() % 16:
             do = do.clone(memory_format=torch.contiguous_format)
-        dq, dk, dv, dsum = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape), lse.new_empty(lse.shape)
+        dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
         _, bwd, _, ws_floats = _general_kernels()
-        ws = _workspace(q, ws_floats(*ctx.how[1:8]))
+        ws = lse.new_empty(ws_floats(B, Sq, Sk, Hq, Hk, D, causal))
         rc = hip.launch(q, bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                        dsum.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), hip.ptr(ws), *ctx.how)
+                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), st, B, Sq, Sk, Hq, Hk, D, causal, scale,
+                        hip.ptr(kv_len))
         hip.check(rc, "dtf_attn_general_bwd")
         return dq, dk, dv, None, None, None
 
@@ -205,6 +210,8 @@ def attention(q, k, v, causal=False, kv_len=None, scale=None):
         if kv_len.dtype != torch.int32:
             kv_len = kv_len.clamp(0, k.shape[1])
         kv_len = kv_len.to(device=q.device, dtype=torch.int32).contiguous()
+    if not hip.recorded(q, k, v):
+        return _general_forward(q, k, v, kv_len, int(bool(causal)), scale)[3]
     return _Attention.apply(q, k, v, kv_len, int(bool(causal)), scale)
 
 

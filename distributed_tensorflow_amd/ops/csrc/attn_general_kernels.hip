@@ -629,6 +629,8 @@ static bool ag_pack_rows(int Sq, int group) {
     return group > 1 && Sq <= 512 && ((int64_t)group * Sq + 127) / 128 < (int64_t)group * ((Sq + 127) / 128);
 }
 
+static int64_t ag_dsum_floats(int64_t B, int64_t Sq, int64_t Hq) { return (B * Sq * Hq + 3) / 4 * 4; }
+
 static int ag_fwd_splits(int B, int Sq, int Sk, int Hq, int Hk) {
     const bool pack = ag_pack_rows(Sq, Hq / Hk);
     const int64_t rows = pack ? (int64_t)(Hq / Hk) * Sq : Sq;
@@ -642,7 +644,7 @@ static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int causal) {
 
 extern "C" {
 
-// fp32 workspace of the forward / backward, in floats (0: none)
+// fp32 workspace of the forward (0: none) and of the backward (D per query and head, then the parts), in floats
 int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
     const int64_t n = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
     return n > 1 ? n * B * Sq * Hq * (D + 2) : 0;
@@ -650,7 +652,7 @@ int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
 
 int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
     const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, causal);
-    return n > 1 ? n * 2 * B * Sk * Hk * D : 0;
+    return ag_dsum_floats(B, Sq, Hq) + (n > 1 ? n * 2 * B * Sk * Hk * D : 0);
 }
 
 // st: the nine element strides (batch, token, head) of q, k, v; ws: dtf_attn_general_fwd_ws floats
@@ -689,15 +691,15 @@ int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, f
     return 0;
 }
 
-// o, do_: contiguous [B, Sq, Hq, D]; dsum: workspace [B, Hq, Sq]; dq like o, dk / dv contiguous [B, Sk, Hk, D];
-// ws: dtf_attn_general_bwd_ws floats
+// o, do_: contiguous [B, Sq, Hq, D]; dq like o, dk / dv contiguous [B, Sk, Hk, D]; ws: dtf_attn_general_bwd_ws floats
 int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                         float* dsum, void* dq, void* dk, void* dv, float* ws, const int64_t* st, int B, int Sq, int Sk, int Hq,
+                         void* dq, void* dk, void* dv, float* ws, const int64_t* st, int B, int Sq, int Sk, int Hq,
                          int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
     AgArgs a{};
     a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.o = (const u16*)o; a.dO = (const u16*)do_;
-    a.lse = const_cast<float*>(lse); a.dsum = dsum; a.dq = (u16*)dq; a.dk = (u16*)dk; a.dv = (u16*)dv; a.ws = ws;
+    a.lse = const_cast<float*>(lse); a.dsum = ws; a.dq = (u16*)dq; a.dk = (u16*)dk; a.dv = (u16*)dv;
+    a.ws = ws + ag_dsum_floats(B, Sq, Hq);
     a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
     a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
     a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
@@ -708,7 +710,7 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
          ((uintptr_t)dk) | ((uintptr_t)dv) | ((uintptr_t)ws)) & 15) return -16;
     a.group = Hq / Hk;
     const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk, causal);
-    if (splits > 1 && !ws) return -73;
+    if (!ws) return -73;
     if ((int64_t)((Sq + 31) / 32) * a.group > 0x7fffffff) return -72;
     a.ntiles = (Sq - 1) / 128 + 1;
     a.nsplit = 1;

@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -99,6 +100,17 @@ def launch(t, fn, *args):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     finally:
         torch.cuda.set_device(back)
+
+
+def recorded(*tensors):
+    """Whether a call on these tensors has to be recorded for gradients (an ``autograd.Function``'s own cost is 6 us a call)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def first_order(backward):

@@ -92,21 +92,26 @@ def _like(t):
     return None if t is None else t.new_empty(t.shape)
 
 
+def _forward(x, h, weight, bias, gate, post_weight, post_bias, rpg, scale, layer, eps):
+    """-> (y, r, the operands as the kernels read them and the statistics, the launch's sizes)."""
+    x, h, weight, bias, gate, post_weight, post_bias = map(_dense, (x, h, weight, bias, gate, post_weight, post_bias))
+    H = x.shape[-1]
+    M = x.numel() // H
+    y, r = x.new_empty(x.shape), _like(h)
+    stats = x.new_empty(4 * M, dtype=torch.float32)
+    how = hip.dt(x), hip.dt(weight), layer, M, H, rpg, scale
+    rc = hip.launch(x, _kernels()[0], x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(bias),
+                    hip.ptr(post_weight), hip.ptr(post_bias), y.data_ptr(), hip.ptr(r), stats.data_ptr(), *how, eps)
+    hip.check(rc, "dtf_residual_norm_fwd")
+    return y, r, (x, h, weight, bias, gate, post_weight, post_bias, stats), how
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, h, weight, bias, gate, post_weight, post_bias, rpg, scale, layer, eps):
-        x, h, weight, bias, gate, post_weight, post_bias = map(_dense, (x, h, weight, bias, gate, post_weight, post_bias))
-        H = x.shape[-1]
-        M = x.numel() // H
-        y, r = x.new_empty(x.shape), _like(h)
-        stats = x.new_empty(4 * M, dtype=torch.float32)
-        how = hip.dt(x), hip.dt(weight), layer, M, H, rpg, scale
-        rc = hip.launch(x, _kernels()[0], x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(bias),
-                        hip.ptr(post_weight), hip.ptr(post_bias), y.data_ptr(), hip.ptr(r), stats.data_ptr(), *how, eps)
-        hip.check(rc, "dtf_residual_norm_fwd")
+    def forward(ctx, *args):
+        y, r, operands, ctx.how = _forward(*args)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, h, weight, bias, gate, post_weight, post_bias, stats)
-        ctx.how = how
+        ctx.save_for_backward(*operands)
         return y, r
 
     @staticmethod
@@ -144,7 +149,8 @@ def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=
     if not x.is_cuda:
         return residual_norm_reference(x, h, weight, bias, gate=gate, scale=scale, post_weight=post_weight, post_bias=post_bias,
                                        kind=kind, eps=eps)
-    return _ResidualNorm.apply(x, h, weight, bias, gate, post_weight, post_bias, rpg or 1, scale, int(kind == "layer"), eps)
+    args = x, h, weight, bias, gate, post_weight, post_bias, rpg or 1, scale, int(kind == "layer"), eps
+    return _ResidualNorm.apply(*args) if hip.recorded(*args[:7]) else _forward(*args)[:2]
 
 
 def rms_norm(x, weight, eps=1e-6):
@@ -152,7 +158,8 @@ def rms_norm(x, weight, eps=1e-6):
     _checked(x, None, weight, None, None, None, None, "rms")
     if not x.is_cuda:
         return _normed(x.float(), weight, None, "rms", eps).to(x.dtype)
-    return _ResidualNorm.apply(x, None, weight, None, None, None, None, 1, 1.0, 0, float(eps))[0]
+    args = x, None, weight, None, None, None, None, 1, 1.0, 0, float(eps)
+    return (_ResidualNorm.apply(*args) if hip.recorded(x, weight) else _forward(*args))[0]
 
 
 class FusedRMSNorm(nn.Module):

@@ -146,4 +146,6 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved=False, amplitude=1.0, 
         return rotary_reference(q, k, inv_freq, positions, interleaved=interleaved, amplitude=amplitude, offset=offset)
     if q.numel() == 0 or (k is not None and k.numel() == 0):
         raise ValueError("rotary: q and k must hold at least one element")
+    if not hip.recorded(q, k):
+        return _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, 1.0)
     return _Rotary.apply(q, k, inv_freq, positions, interleaved, amplitude, offset)

@@ -33,12 +33,15 @@ struct AgArgs {
     float scale, scale_log2e;
 };
 
-// LDS image of a [rows][DP] bf16 tile, 16-B chunk c of row r.  Conflict-free (256 B of banks) both for ds_read_b128 of
-// 16 rows at one chunk and for ds_read_b64_tr_b16 of 8 rows x 32 columns.
+// LDS image of a [rows][DP] bf16 tile, 16-B chunk c of row r, without bank conflicts (256 B of banks) for ds_read_b128 of 16
+// rows at one chunk and for ds_read_b64_tr_b16 of 4 rows x 32 columns: the 32-B chunk is XORed so that rows 0..3 of a
+// 4-row block take different PAIRS of chunks (a plain XOR with the row puts rows 0 and 1 on the same pair: 2 extra cycles
+// a transposed read, a quarter of the LDS time), rows + 4 the odd places, rows + 8 the other 16-B half.
+template <int DP>
+__device__ __forceinline__ int ag_swz(int row) { return DP == 128 ? (row & 3) << 1 | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1); }
 template <int DP>
 __device__ __forceinline__ int ag_off(int row, int c) {
-    if constexpr (DP == 128) return row * 256 + ((((c >> 1) ^ (row & 7)) << 5) | (((c ^ (row >> 3)) & 1) << 4));
-    else return row * 128 + ((((c >> 1) ^ ((row >> 1) & 3)) << 5) | (((c ^ (row >> 3)) & 1) << 4));
+    return row * (2 * DP) + ((((c >> 1) ^ ag_swz<DP>(row)) << 5) | (((c ^ (row >> 3)) & 1) << 4));
 }
 
 __device__ __forceinline__ f32x16 ag_zero() {
@@ -106,8 +109,7 @@ struct AgTile {
     __device__ __forceinline__ void init(const u16* base_, int64_t rs_, int D, int wave, int lane) {
         row = wave * RPI + lane / (DP / 8);
         const int p = lane % (DP / 8);
-        const int x = DP == 128 ? row & 7 : (row >> 1) & 3;
-        const int c = (((p >> 1) ^ x) << 1) | ((p ^ (row >> 3)) & 1);      // STEP is a multiple of 16: the same for every row of a lane
+        const int c = (((p >> 1) ^ ag_swz<DP>(row)) << 1) | ((p ^ (row >> 3)) & 1);      // STEP is a multiple of 16: the same for every row of a lane
         col = c * 8 < D;
         base = reinterpret_cast<const char*>(base_);
         rs = rs_ * 2;
@@ -218,11 +220,12 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
         at.keep();
         f32x16 s[BN / 32];
 #pragma unroll
-        for (int u = 0; u < BN / 32; ++u) {
-            s[u] = ag_zero();
+        for (int u = 0; u < BN / 32; ++u) s[u] = ag_zero();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[u] = ag_mfma(at.rows(K, 32 * u, ks), qf[ks], s[u]);
-        }
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int u = 0; u < BN / 32; ++u) s[u] = ag_mfma(at.rows(K, 32 * u, ks), qf[ks], s[u]);
+        __builtin_amdgcn_s_setprio(1);                                     // a wave past its scores goes first: the other of the SIMD has its products to issue
         if (k0 + BN > lo) {
             const int left = vis - (k0 + 4 * g);
 #pragma unroll
@@ -261,6 +264,7 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
                 for (int dt = 0; dt < DT; ++dt) oacc[dt] = ag_mfma(at.cols(V, 32 * u + 16 * h2, dt), pf, oacc[dt]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     };
     if (kbeg < kend) fetch(K0, V0, kbeg);
     AG_LANDED();
@@ -412,6 +416,7 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
                 s = ag_mfma(at.rows(K, 32 * u, ks), qf[ks], s);
                 dp = ag_mfma(at.rows(V, 32 * u, ks), gf[ks], dp);
             }
+            __builtin_amdgcn_s_setprio(1);
             if (k0 + 32 * u + 32 > lo) {
                 const int left = vis - (k0 + 32 * u + 4 * g);
 #pragma unroll
@@ -425,6 +430,7 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[dt] = ag_mfma(at.cols(K, 32 * u + 16 * h2, dt), f, acc[dt]);
             }
+            __builtin_amdgcn_s_setprio(0);
         }
     };
     AG_LANDED();
@@ -526,6 +532,7 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
             s = ag_mfma(at.rows(Q, 0, ks), kf[ks], s);
             dp = ag_mfma(at.rows(G, 0, ks), DP == 128 ? at.rows(Vimg, wave * 32, ks) : vf[DP == 128 ? 0 : ks], dp);
         }
+        __builtin_amdgcn_s_setprio(1);
         if ((a.causal && q0 + off < jw + 31) || jw + 32 > klen) {          // some (query, key) of the tile is not seen
             const int from = !seen ? 0x7fffffff : a.causal ? j - off - q0 - 4 * g : -1;
 #pragma unroll
@@ -551,6 +558,7 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
                 dk[dt] = ag_mfma(at.cols(Q, 16 * h2, dt), df, dk[dt]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     };
     if (n0 < n1) fetch(Q0, G0, LD0);
     AG_LANDED();

@@ -304,18 +304,19 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
     }
 }
 
-// O = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup per row: 32 lanes of 4 columns x 8 threads that share the
-// parts (few rows have many parts, and a chain of dependent reads per part cost more than the attention before it).
+// O = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A row: 32 lanes of 4 columns x PY threads that share the parts (few rows
+// have many parts, and a chain of dependent reads per part cost more than the attention before it); 8 / PY rows a workgroup.
+template <int PY>
 __global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 os[8][32];
     __shared__ float ms[8], ls[8];
-    const int64_t n = (int64_t)a.B * a.Sq * a.Hq, row = blockIdx.x;
-    const int x = threadIdx.x % 32, y = threadIdx.x / 32, d = x * 4;
+    const int x = threadIdx.x % 32, z = threadIdx.x / 32, y = z % PY, d = x * 4;
+    const int64_t n = (int64_t)a.B * a.Sq * a.Hq, want = (int64_t)blockIdx.x * (8 / PY) + z / PY, row = want < n ? want : n - 1;
     const float* ml = a.ws + (int64_t)a.nsplit * n * a.D + row * 2;
     float m = AG_NEG, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = y; s < a.nsplit; s += 8) m = __builtin_elementwise_maximum(m, ml[s * n * 2]);
-    for (int s = y; s < a.nsplit; s += 8) {
+    for (int s = y; s < a.nsplit; s += PY) m = __builtin_elementwise_maximum(m, ml[s * n * 2]);
+    for (int s = y; s < a.nsplit; s += PY) {
         const float mp = ml[s * n * 2], w = mp == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(mp - m);
         l = fmaf(ml[s * n * 2 + 1], w, l);
         if (d < a.D) {
@@ -324,24 +325,23 @@ __global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
             for (int e = 0; e < 4; ++e) o[e] = fmaf(p[e], w, o[e]);
         }
     }
-    os[y][x] = o;
+    os[z][x] = o;
     if (x == 0) {
-        ms[y] = m;
-        ls[y] = l;
+        ms[z] = m;
+        ls[z] = l;
     }
     __syncthreads();
-    if (y > 0) return;
-    m = ms[0];
+    if (y > 0 || want >= n) return;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) m = __builtin_elementwise_maximum(m, ms[k]);
+    for (int k = 1; k < PY; ++k) m = __builtin_elementwise_maximum(m, ms[z + k]);
     l = 0.f;
     o = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float w = ms[k] == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
-        l = fmaf(ls[k], w, l);
+    for (int k = 0; k < PY; ++k) {
+        const float w = ms[z + k] == AG_NEG ? 0.f : __builtin_amdgcn_exp2f(ms[z + k] - m);
+        l = fmaf(ls[z + k], w, l);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(os[k][x][e], w, o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(os[z + k][x][e], w, o[e]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d < a.D) {
@@ -450,14 +450,14 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dK and dV: 4 waves x 32 keys, 32 queries a step, over all query heads of the key head's group (so shared
+// Backward, dK and dV: 4 waves x 32 keys, 32 queries a step (64 for DP = 64, whose steps were shorter than a fetch), over all query heads of the key head's group (so shared
 // heads' gradients are one fixed-order sum: no atomics).  S = Q . K^T, dP = dO . V^T (a lane owns one key),
 // dV^T += dO^T . P, dK^T += Q^T . dS.  nsplit > 1: that many workgroups share a tile's (head, query) steps, each writes
 // fp32 sums, and ag_add_kernel adds them in order.
 // ---------------------------------------------------------------------------
 template <int DP>
 __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
-    constexpr int KS = DP / 16, DT = DP / 32, BQ = 32, BM = 128;
+    constexpr int KS = DP / 16, DT = DP / 32, BQ = DP == 64 ? 64 : 32, BM = 128;
     __shared__ __attribute__((aligned(16))) unsigned char Q0[BQ * DP * 2], Q1[BQ * DP * 2], G0[BQ * DP * 2], G1[BQ * DP * 2];
     __shared__ __attribute__((aligned(16))) float LD0[128], LD1[128];                 // log-sum-exp (0..), D (64..) of a step's queries
     __shared__ __attribute__((aligned(16))) unsigned char Vimg[DP == 128 ? BM * DP * 2 : 16];
@@ -523,42 +523,46 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     at.init(lane);
     auto step = [&](const unsigned char* Q, const unsigned char* G, const float* LD) {
         at.keep();
-        const int q0 = begin + sq * BQ;
+        const int first = begin + sq * BQ;
         if (++sq == steps) sq = 0;
-        if (a.causal && q0 + BQ - 1 + off < jw) return;                    // no query of the step sees this wave's keys
-        f32x16 s = ag_zero(), dp = ag_zero();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            s = ag_mfma(at.rows(Q, 0, ks), kf[ks], s);
-            dp = ag_mfma(at.rows(G, 0, ks), DP == 128 ? at.rows(Vimg, wave * 32, ks) : vf[DP == 128 ? 0 : ks], dp);
-        }
-        __builtin_amdgcn_s_setprio(1);
-        if ((a.causal && q0 + off < jw + 31) || jw + 32 > klen) {          // some (query, key) of the tile is not seen
-            const int from = !seen ? 0x7fffffff : a.causal ? j - off - q0 - 4 * g : -1;
+        for (int r0 = 0; r0 < BQ; r0 += 32) {
+            const int q0 = first + r0;
+            if (a.causal && q0 + 31 + off < jw) continue;                  // none of these queries sees this wave's keys
+            f32x16 s = ag_zero(), dp = ag_zero();
 #pragma unroll
-            for (int x = 0; x < 16; ++x) s[x] = 8 * (x >> 2) + (x & 3) >= from ? s[x] : AG_NEG;
-        }
-#pragma unroll
-        for (int rq = 0; rq < 4; ++rq) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(LD + 8 * rq + 4 * g);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(LD + 64 + 8 * rq + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int x = 4 * rq + e;
-                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale_log2e, -l4[e]));
-                dp[x] = s[x] * (dp[x] - d4[e]);
+            for (int ks = 0; ks < KS; ++ks) {
+                s = ag_mfma(at.rows(Q, r0, ks), kf[ks], s);
+                dp = ag_mfma(at.rows(G, r0, ks), DP == 128 ? at.rows(Vimg, wave * 32, ks) : vf[DP == 128 ? 0 : ks], dp);
             }
-        }
+            __builtin_amdgcn_s_setprio(1);
+            if ((a.causal && q0 + off < jw + 31) || jw + 32 > klen) {      // some (query, key) of the tile is not seen
+                const int from = !seen ? 0x7fffffff : a.causal ? j - off - q0 - 4 * g : -1;
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-            const s16x8 pf = ag_pack(s, h2), df = ag_pack(dp, h2);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                dv[dt] = ag_mfma(at.cols(G, 16 * h2, dt), pf, dv[dt]);
-                dk[dt] = ag_mfma(at.cols(Q, 16 * h2, dt), df, dk[dt]);
+                for (int x = 0; x < 16; ++x) s[x] = 8 * (x >> 2) + (x & 3) >= from ? s[x] : AG_NEG;
             }
+#pragma unroll
+            for (int rq = 0; rq < 4; ++rq) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(LD + r0 + 8 * rq + 4 * g);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(LD + 64 + r0 + 8 * rq + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = 4 * rq + e;
+                    s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale_log2e, -l4[e]));
+                    dp[x] = s[x] * (dp[x] - d4[e]);
+                }
+            }
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+                const s16x8 pf = ag_pack(s, h2), df = ag_pack(dp, h2);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    dv[dt] = ag_mfma(at.cols(G, r0 + 16 * h2, dt), pf, dv[dt]);
+                    dk[dt] = ag_mfma(at.cols(Q, r0 + 16 * h2, dt), df, dk[dt]);
+                }
+            }
+            __builtin_amdgcn_s_setprio(0);
         }
-        __builtin_amdgcn_s_setprio(0);
     };
     if (n0 < n1) fetch(Q0, G0, LD0);
     AG_LANDED();
@@ -646,8 +650,9 @@ static int ag_fwd_splits(int B, int Sq, int Sk, int Hq, int Hk) {
 }
 
 // (512 workgroups are resident; causal tiles differ in length, so the longest should be no more than what a slot gets in all)
-static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int causal) {
-    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), (int64_t)((Sq + 31) / 32) * (Hq / Hk), 8, causal ? 1024 : 512);
+static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
+    const int bq = D > 64 ? 32 : 64;
+    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), (int64_t)((Sq + bq - 1) / bq) * (Hq / Hk), 256 / bq, causal ? 1024 : 512);
 }
 
 extern "C" {
@@ -659,7 +664,7 @@ int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
 }
 
 int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
-    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, causal);
+    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, D, causal);
     return ag_dsum_floats(B, Sq, Hq) + (n > 1 ? n * 2 * B * Sk * Hk * D : 0);
 }
 
@@ -692,8 +697,11 @@ int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, f
     }
     DTF_CHECK_LAUNCH();
     if (a.nsplit > 1) {
-        if ((rc = ag_grid((int64_t)B * Sq * Hq, &grid))) return rc;
-        hipLaunchKernelGGL(ag_join_kernel, dim3(grid), dim3(256), 0, stream, a);
+        const int py = a.nsplit <= 2 ? 2 : a.nsplit <= 4 ? 4 : 8;
+        if ((rc = ag_grid(((int64_t)B * Sq * Hq * py + 7) / 8, &grid))) return rc;
+        if (py == 2) hipLaunchKernelGGL((ag_join_kernel<2>), dim3(grid), dim3(256), 0, stream, a);
+        else if (py == 4) hipLaunchKernelGGL((ag_join_kernel<4>), dim3(grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((ag_join_kernel<8>), dim3(grid), dim3(256), 0, stream, a);
         DTF_CHECK_LAUNCH();
     }
     return 0;
@@ -717,7 +725,7 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)do_) | ((uintptr_t)dq) |
          ((uintptr_t)dk) | ((uintptr_t)dv) | ((uintptr_t)ws)) & 15) return -16;
     a.group = Hq / Hk;
-    const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk, causal);
+    const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk, D, causal);
     if (!ws) return -73;
     if ((int64_t)((Sq + 31) / 32) * a.group > 0x7fffffff) return -72;
     a.ntiles = (Sq - 1) / 128 + 1;

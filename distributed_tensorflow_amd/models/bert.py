@@ -10,6 +10,11 @@ Variables are named like google-research/bert checkpoints: ``bert/embeddings/wor
 ``bert/encoder/layer_0/attention/self/query/kernel``, ``cls/predictions/transform/dense/kernel``
 (TF stores kernels ``[in, out]``; the flat shard bytes here are torch's ``[out, in]``, recorded
 as such in the checkpoint index).
+
+Job options beside the published model: ``positions=rotary`` (K23 on queries and keys instead of the learned table, so the
+sequence length has no bound; ``rotary_scaling``, ``rotary_factor``, ``rotary_original`` stretch it), ``kv_heads=N`` (fewer key and value heads)
+and ``norm=pre_rms`` (RMS norms in front of attention and MLP, every block boundary one K24 pass).  The first two take their
+attention from K22, which has no limit on length.
 """
 import math
 
@@ -22,6 +27,8 @@ from ..ops.layernorm import FusedLayerNorm
 from ..ops.cross_entropy import cross_entropy
 from ..ops.embedding import dense_embedding
 from ..ops.linear import FusedLinear, linear_residual_layernorm
+from ..ops.residual_norm import FusedRMSNorm
+from ..ops.rotary import rotary, rotary_frequencies
 
 
 class _SplitQKV(torch.autograd.Function):
@@ -40,11 +47,59 @@ class _SplitQKV(torch.autograd.Function):
         return torch.stack([dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)], dim=2)
 
 
+class RotaryPositions:
+    """The frequencies of ``positions=rotary``, made once per device (in 64 bits, so they are no buffer of the model, whose
+    buffers follow its dtype)."""
+
+    def __init__(self, dim, base, scaling, factor, original_length):
+        self.spec = dict(dim=dim, base=base, scaling=scaling, factor=factor, original_length=original_length)
+        _, self.amplitude = rotary_frequencies(**self.spec)               # checks the options where the model is built
+        self._on = {}
+
+    def __call__(self, q, k):
+        if q.device not in self._on:
+            self._on[q.device] = rotary_frequencies(**self.spec, device=q.device)[0]
+        return rotary(q, k, self._on[q.device], amplitude=self.amplitude)
+
+
+def _general_attention(qkv, A, KV, kv_len, positions):
+    """Context ``[B, S, H]`` of a packed projection ``[B, S, (A + 2 KV) D]`` through K22 (and K23)."""
+    B, S, W = qkv.shape
+    q, k, v = qkv.view(B, S, A + 2 * KV, W // (A + 2 * KV)).split([A, KV, KV], dim=2)
+    if positions is not None:
+        q, k = positions(q, k)
+    return attention.attention(q, k, v, kv_len=kv_len).flatten(2)
+
+
+class PreNormLayer(nn.Module):
+    """``norm=pre_rms``: takes the residual stream and the output of the block before, returns the stream and its own output
+    -- the addition, and the norm behind it, are the next block's first pass."""
+
+    def __init__(self, H, A, I, act, KV, positions):
+        super().__init__()
+        self.A, self.KV, self.positions = A, KV, positions
+        self.attn_in_ln = FusedRMSNorm(H, eps=1e-6)
+        self.qkv = FusedLinear(H, (A + 2 * KV) * (H // A))
+        self.attn_out = FusedLinear(H, H)
+        self.mlp_in_ln = FusedRMSNorm(H, eps=1e-6)
+        self.inter = FusedLinear(H, I, act=act)
+        self.out = FusedLinear(I, H)
+
+    def forward(self, x, h, kv_len):
+        if h is None:
+            y = self.attn_in_ln(x)
+        else:
+            y, x = self.attn_in_ln(x, h)
+        y, x = self.mlp_in_ln(x, self.attn_out(_general_attention(self.qkv(y), self.A, self.KV, kv_len, self.positions)))
+        return x, self.out(self.inter(y))
+
+
 class Layer(nn.Module):
-    def __init__(self, H, A, I, p, act="gelu_tanh"):
+    def __init__(self, H, A, I, p, act="gelu_tanh", KV=None, positions=None):
         super().__init__()
         self.A = A
-        self.qkv = FusedLinear(H, 3 * H)
+        self.KV, self.positions = KV or A, positions
+        self.qkv = FusedLinear(H, (A + 2 * self.KV) * (H // A))
         self.attn_out = FusedLinear(H, H)
         self.attn_ln = FusedLayerNorm(H, eps=1e-12)
         self.inter = FusedLinear(H, I, act=act)
@@ -56,9 +111,14 @@ class Layer(nn.Module):
         B, S, H = x.shape
         # x feeds the projection and the residual: the fork sums both gradients inside the dX GEMM
         qkv, x = self.qkv.forward_fork(x, own_skip_grad=True)
-        qkv5 = qkv.view(B, S, 3, self.A, H // self.A)
         drop = self.p if self.training else 0.0
-        if drop == 0.0 and attention.kernel_eligible(qkv5):
+        general = self.positions is not None or self.KV != self.A
+        qkv5 = None if general else qkv.view(B, S, 3, self.A, H // self.A)
+        if general:
+            if drop:
+                raise ValueError("rotary positions and kv_heads are without attention dropout")
+            ctx = _general_attention(qkv, self.A, self.KV, kv_len, self.positions)
+        elif drop == 0.0 and attention.kernel_eligible(qkv5):
             # K11: consumes the packed projection in place, writes the context token-major, and its backward
             # writes dQ / dK / dV straight into the packed gradient -- no transposes or copies either way.
             # The padding mask is a prefix mask: handed over as one length per sequence.
@@ -74,15 +134,35 @@ class Layer(nn.Module):
 
 class Bert(nn.Module):
     def __init__(self, vocab=30522, hidden=768, layers=12, heads=12, intermediate=3072, max_pos=512,
-                 type_vocab=2, dropout=0.0, act="gelu_tanh"):
+                 type_vocab=2, dropout=0.0, act="gelu_tanh", kv_heads=0, positions="learned", norm="post_ln", rotary_base=10000.0,
+                 rotary_scaling="none", rotary_factor=1.0, rotary_original=512):
         super().__init__()
-        self.hidden, self.vocab = hidden, vocab
+        kv_heads = kv_heads or heads
+        if hidden % heads or heads % kv_heads:
+            raise ValueError("hidden %d must divide over %d heads, and these over %d kv_heads" % (hidden, heads, kv_heads))
+        if positions not in ("learned", "rotary") or norm not in ("post_ln", "pre_rms"):
+            raise ValueError("positions is learned or rotary, norm post_ln or pre_rms; got %r, %r" % (positions, norm))
+        if norm == "pre_rms" and dropout:
+            raise ValueError("norm=pre_rms is without dropout")
+        if (positions == "rotary" or norm == "pre_rms" or kv_heads != heads) and (hidden // heads % 8 or hidden // heads > 128):
+            raise ValueError("these options need head sizes that are multiples of 8 to 128, got %d" % (hidden // heads))
+        turn = None
+        if positions == "rotary":
+            turn = RotaryPositions(hidden // heads, rotary_base, rotary_scaling, rotary_factor, rotary_original)
+        self.hidden, self.vocab, self.kv_width = hidden, vocab, kv_heads * (hidden // heads)
         self.word_embeddings = nn.Embedding(vocab, hidden)
-        self.position_embeddings = nn.Embedding(max_pos, hidden)
+        if turn is None:
+            self.position_embeddings = nn.Embedding(max_pos, hidden)
         self.token_type_embeddings = nn.Embedding(type_vocab, hidden)
         self.emb_ln = FusedLayerNorm(hidden, eps=1e-12)
         # act: "gelu_tanh" is the google-research/bert definition (tanh form); "gelu" the erf form
-        self.layers = nn.ModuleList(Layer(hidden, heads, intermediate, dropout, act) for _ in range(layers))
+        self.pre_norm = norm == "pre_rms"
+        if self.pre_norm:
+            self.layers = nn.ModuleList(PreNormLayer(hidden, heads, intermediate, act, kv_heads, turn) for _ in range(layers))
+            self.final_ln = FusedRMSNorm(hidden, eps=1e-6)
+        else:
+            self.layers = nn.ModuleList(Layer(hidden, heads, intermediate, dropout, act, kv_heads, turn) for _ in range(layers))
+        self.learned_positions = turn is None
         self.pooler = FusedLinear(hidden, hidden)
         self.mlm_transform = FusedLinear(hidden, hidden, act=act)
         self.mlm_ln = FusedLayerNorm(hidden, eps=1e-12)
@@ -99,17 +179,24 @@ class Bert(nn.Module):
 
     def forward(self, input_ids, token_type_ids, attention_mask, masked_positions):
         B, S = input_ids.shape
-        pos = torch.arange(S, device=input_ids.device)
-        x = dense_embedding(input_ids, self.word_embeddings.weight) + self.position_embeddings(pos).unsqueeze(0) \
-            + dense_embedding(token_type_ids, self.token_type_embeddings.weight)
+        x = dense_embedding(input_ids, self.word_embeddings.weight)
+        if self.learned_positions:
+            x = x + self.position_embeddings(torch.arange(S, device=input_ids.device)).unsqueeze(0)
+        x = x + dense_embedding(token_type_ids, self.token_type_embeddings.weight)
         x = self.emb_ln(x)
         mask = kv_len = None
         if attention_mask is not None:
             # BERT's input mask marks real tokens with 1 and trailing padding with 0 (a prefix mask)
             mask = attention_mask[:, None, None, :].to(torch.bool)
             kv_len = attention_mask.sum(-1, dtype=torch.int32)
-        for layer in self.layers:
-            x = layer(x, mask, kv_len)
+        if self.pre_norm:
+            h = None
+            for layer in self.layers:
+                x, h = layer(x, h, kv_len)
+            x, _ = self.final_ln(x, h)
+        else:
+            for layer in self.layers:
+                x = layer(x, mask, kv_len)
         pooled = torch.tanh(self.pooler(x[:, 0]))
         # masked-LM head on the masked positions only (max_predictions_per_seq)
         idx = masked_positions.unsqueeze(-1).expand(-1, -1, self.hidden)
@@ -119,8 +206,12 @@ class Bert(nn.Module):
         return mlm_logits, self.nsp(pooled)
 
 
-def build(layers=12, hidden=768, heads=12, intermediate=3072, vocab=30522, seq_len=512, act="gelu_tanh", **_):
-    return Bert(int(vocab), int(hidden), int(layers), int(heads), int(intermediate), max(512, int(seq_len)), act=act)
+def build(layers=12, hidden=768, heads=12, intermediate=3072, vocab=30522, seq_len=512, act="gelu_tanh", kv_heads=0,
+          positions="learned", norm="post_ln", rotary_base=10000.0, rotary_scaling="none", rotary_factor=1.0,
+          rotary_original=512, **_):
+    return Bert(int(vocab), int(hidden), int(layers), int(heads), int(intermediate), max(512, int(seq_len)), act=act,
+                kv_heads=int(kv_heads), positions=positions, norm=norm, rotary_base=float(rotary_base), rotary_scaling=rotary_scaling,
+                rotary_factor=float(rotary_factor), rotary_original=int(rotary_original))
 
 
 def prepare(model, device):
@@ -137,15 +228,20 @@ def tf_variable_names(model):
     out = {}
     ln = {"weight": "gamma", "bias": "beta"}
     kb = {"weight": "kernel", "bias": "bias"}
-    H = model.hidden
+    H, KV = model.hidden, model.kv_width
+    rms = {"attn_in_ln": "attention/input/RMSNorm/gamma", "mlp_in_ln": "intermediate/input/RMSNorm/gamma"}
     for n, _ in model.named_parameters():
         p = n.split(".")
         if p[0] == "layers" and p[2] == "qkv":
             base = "bert/encoder/layer_%s/attention/self/" % p[1]
-            out[n] = [(base + "%s/%s" % (part, kb[p[3]]), i * H, (i + 1) * H)
-                      for i, part in enumerate(("query", "key", "value"))]
+            out[n] = [(base + "%s/%s" % (part, kb[p[3]]), a, b)
+                      for part, a, b in (("query", 0, H), ("key", H, H + KV), ("value", H + KV, H + 2 * KV))]
             continue
-        if p[0] in ("word_embeddings", "position_embeddings", "token_type_embeddings"):
+        if p[0] == "final_ln":
+            tf = "bert/encoder/output/RMSNorm/gamma"
+        elif p[0] == "layers" and p[2] in rms:
+            tf = "bert/encoder/layer_%s/" % p[1] + rms[p[2]]
+        elif p[0] in ("word_embeddings", "position_embeddings", "token_type_embeddings"):
             tf = "bert/embeddings/" + p[0]
         elif p[0] == "emb_ln":
             tf = "bert/embeddings/LayerNorm/" + ln[p[1]]

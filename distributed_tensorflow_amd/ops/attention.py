@@ -121,9 +121,10 @@ def _general_kernels():
 
 
 def _operand(t):
-    """As it is where the kernels can address it (dense head dimension, 16-B aligned rows), else a contiguous copy."""
+    """As it is where the kernels can address it (dense head dimension, 16-B aligned rows, tokens less than 2^25 elements
+    apart), else a contiguous copy."""
     st = t.stride()
-    if st[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
+    if st[3] == 1 and (st[1] < 1 << 25 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -187,6 +188,8 @@ def _check_general(q, k, v, kv_len, scale):
         raise ValueError("attention: %d query heads do not divide over %d key heads" % (Hq, k.shape[2]))
     if D % 8 or D > 128:
         raise ValueError("attention: the head dimension must be a multiple of 8 up to 128, got %d" % D)
+    if Hq * D >= 1 << 25:
+        raise ValueError("attention: %d heads of %d are too many" % (Hq, D))
     if max(Sq, k.shape[1]) > 1 << 30:
         raise ValueError("attention: sequences are at most 2**30 tokens long")
     if not (scale > 0 and math.isfinite(scale)):

@@ -187,3 +187,89 @@ def test_residual_norm_refusals():
     for err, kw in bad:
         with pytest.raises(err):
             residual_norm(**{**dict(x=x, h=x, weight=w), **kw})
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the model that calls them
+# ---------------------------------------------------------------------------------------------------------------------
+BERT = dict(layers=2, hidden=64, heads=4, intermediate=64, vocab=2000, seq_len=21)
+
+
+def _bert(**kw):
+    from distributed_tensorflow_amd.models import bert
+
+    torch.manual_seed(0)
+    m = bert.build(**BERT, **kw)
+    batch = list(bert.synthetic_batch(3, seed=1, seq_len=21, vocab=2000))
+    batch[2][1, 13:] = 0                                               # the second sequence is padded
+    return bert, m, tuple(batch)
+
+
+@pytest.mark.parametrize("kw", [dict(positions="rotary"), dict(kv_heads=2), dict(norm="pre_rms"),
+                                dict(positions="rotary", kv_heads=1, norm="pre_rms", rotary_scaling="by_parts", rotary_factor=4)])
+def test_bert_options_train(kw):
+    bert, m, batch = _bert(**kw)
+    loss = bert.loss_fn(m, batch)
+    loss.backward()
+    assert bool(torch.isfinite(loss))
+    for n, p in m.named_parameters():
+        assert p.grad is not None and bool(torch.isfinite(p.grad).all()), n
+    assert ("position_embeddings.weight" in dict(m.named_parameters())) == (kw.get("positions") != "rotary")
+    names = bert.tf_variable_names(m)
+    flat = [v if isinstance(v, str) else [x[0] for x in v] for v in names.values()]
+    flat = [x for v in flat for x in ([v] if isinstance(v, str) else v)]
+    assert len(set(flat)) == len(flat) and set(names) == {n for n, _ in m.named_parameters()}
+    rows = names["layers.0.qkv.weight"]
+    assert [b - a for _, a, b in rows] == [64, 16 * (kw.get("kv_heads") or 4), 16 * (kw.get("kv_heads") or 4)]
+    assert rows[-1][2] == m.layers[0].qkv.weight.shape[0]
+    # padding takes no part: other tokens there, the same loss
+    other = list(batch)
+    other[0] = batch[0].clone()
+    masked = {int(p) for p in batch[3][1]}
+    for at in range(13, 21):
+        if at not in masked:
+            other[0][1, at] = 1500
+    keep = torch.tensor([p < 13 for p in batch[3][1].tolist()])
+    a, _ = m(*batch[:4])
+    b, _ = m(*other[:4])
+    n = batch[3].shape[1]
+    torch.testing.assert_close(a[n:2 * n][keep], b[n:2 * n][keep], rtol=1e-5, atol=1e-6)
+
+
+def test_bert_fewer_key_heads_equal_repeated_ones():
+    """kv_heads=2 of 4 is the full-head model whose key and value heads come in equal pairs; the gradient of a shared head is
+    the sum of its copies'."""
+    import copy
+
+    bert, m, batch = _bert(kv_heads=2)
+    _, full, _ = _bert()
+    wide = copy.deepcopy(m)
+    for layer, src in zip(full.layers, m.layers):
+        for n in ("weight", "bias"):
+            q, k, v = getattr(src.qkv, n).detach().split([64, 32, 32])
+            k, v = (t.view(2, 16, -1).repeat_interleave(2, 0).reshape(64, -1) if n == "weight" else
+                    t.view(2, 16).repeat_interleave(2, 0).reshape(64) for t in (k, v))
+            getattr(layer.qkv, n).data.copy_(torch.cat([q, k, v]))
+    rest = {n: p for n, p in wide.named_parameters() if ".qkv." not in n}
+    with torch.no_grad():
+        for n, p in full.named_parameters():
+            if n in rest:
+                p.copy_(rest[n])
+    a, b = bert.loss_fn(m, batch), bert.loss_fn(full, batch)
+    torch.testing.assert_close(a, b, rtol=2e-6, atol=2e-6)
+    a.backward()
+    b.backward()
+    for s, f in zip(m.layers, full.layers):
+        gs, gf = s.qkv.weight.grad, f.qkv.weight.grad
+        torch.testing.assert_close(gs[:64], gf[:64], rtol=1e-4, atol=1e-6)
+        torch.testing.assert_close(gs[64:96].view(2, 16, 64), gf[64:128].view(2, 2, 16, 64).sum(1), rtol=1e-4, atol=1e-6)
+        torch.testing.assert_close(gs[96:].view(2, 16, 64), gf[128:].view(2, 2, 16, 64).sum(1), rtol=1e-4, atol=1e-6)
+
+
+def test_bert_option_refusals():
+    from distributed_tensorflow_amd.models import bert
+
+    for kw in (dict(kv_heads=3), dict(positions="sine"), dict(norm="none"), dict(positions="rotary", rotary_scaling="x"), dict(hidden=50),
+               dict(hidden=48, kv_heads=2), dict(hidden=1024, norm="pre_rms")):
+        with pytest.raises(ValueError):
+            bert.build(**{**BERT, **kw})

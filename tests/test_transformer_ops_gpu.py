@@ -274,3 +274,255 @@ def test_residual_norm_unaligned_rows_equal_aligned_ones(dev):
     for got in res:
         for n, g in zip(("y", "r", "dx", "dh", "dw", "dgate", "dpw"), got):
             oracle.close(g, want[n], tol[n], n)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# how they are called: offsets past 32 bits, the same tensor twice, streams, graphs, refusals
+# ---------------------------------------------------------------------------------------------------------------------
+def test_attention_offsets_past_32_bits(dev):
+    r = _randn(dev, 11)
+    B, S, H, D = 2, 130, 2, 64
+    q, k, v, do = (r(B, S, H, D).to(BF) for _ in range(4))
+    want = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*want, causal=True)
+    ref = (out.detach(),) + torch.autograd.grad(out, want, do)
+    far, rows = (1 << 31) + 64, (1 << 24) + 8
+    for bs, ss, n in ((far, H * D, S), (H * D, rows, S), (H * D, 1 << 25, 5)):      # sequences, tokens far apart; tokens too far: copied
+        buf = torch.empty(bs + n * ss + H * D, dtype=BF, device=dev)
+        kk = buf.as_strided((B, n, H, D), (bs, ss, D, 1))
+        kk.copy_(k[:, :n])
+        leaf = [t.detach().requires_grad_() for t in (q[:, :n], kk, v[:, :n])]
+        out = attention(*leaf, causal=True)
+        got = (out.detach(),) + torch.autograd.grad(out, leaf, do[:, :n])
+        for a, b in zip(ref[:4 if n == S else 2], got):                 # (the first tokens' outputs and dq do not depend on later ones)
+            assert torch.equal(a[:, :n], b)
+        del buf, kk, leaf, out
+
+
+def test_attention_results_past_32_bits(dev):
+    r = _randn(dev, 12)
+    B, S, H, D = (1 << 18) + 3, 16, 8, 64                               # 2^31 elements a tensor
+    q, k, v, do = (r(5, S, H, D).to(BF).repeat((B + 4) // 5, 1, 1, 1)[:B] for _ in range(4))
+    leaf = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*leaf, causal=True)
+    got = (out.detach(),) + torch.autograd.grad(out, leaf, do)
+    few = [t[-5:].clone().requires_grad_() for t in (q, k, v)]
+    out = attention(*few, causal=True)
+    for a, b in zip(got, (out.detach(),) + torch.autograd.grad(out, few, do[-5:])):
+        assert torch.equal(a[-5:], b)
+
+
+def test_rotary_and_norm_past_32_bits(dev):
+    r = _randn(dev, 13)
+    B, S, H, D = 1030, 512, 32, 128                                     # 2.16e9 elements a tensor
+    q = r(2, S, H, D).to(BF).repeat(B // 2, 1, 1, 1)
+    f, _ = rotary_frequencies(D, device=dev)
+    y, _ = rotary(q, None, f)
+    few, _ = rotary(q[-3:].clone(), None, f)
+    assert torch.equal(y[-3:], few)
+    x, h = q.view(-1, H * D), y.view(-1, H * D)
+    w, pw, gate = (1 + 0.1 * r(H * D).to(BF) for _ in range(3))
+    leaf = [t.detach().requires_grad_() for t in (x, h)]
+    out = residual_norm(*leaf, w, gate=gate, post_weight=pw, scale=0.5)
+    got = tuple(t.detach()[-40:].clone() for t in out) + tuple(t[-40:].clone() for t in torch.autograd.grad(out, leaf, (h, x)))
+    leaf = [t.detach()[-40:].clone().requires_grad_() for t in (x, h)]
+    out = residual_norm(*leaf, w, gate=gate, post_weight=pw, scale=0.5)
+    for a, b in zip(got, tuple(t.detach() for t in out) + torch.autograd.grad(out, leaf, (h[-40:], x[-40:]))):
+        assert torch.equal(a, b)
+
+
+def test_the_same_tensor_in_several_places(dev):
+    r = _randn(dev, 14)
+    x, do = r(2, 70, 4, 64).to(BF), r(2, 70, 4, 64).to(BF)
+    leaf = x.detach().requires_grad_()
+    g, = torch.autograd.grad(attention(leaf, leaf, leaf, causal=True), leaf, do)
+    three = [x.detach().clone().requires_grad_() for _ in range(3)]
+    dq, dk, dv = torch.autograd.grad(attention(*three, causal=True), three, do)
+    # autograd adds the three in bf16: two roundings of the sums
+    tol = 2 * oracle.U16 * (dq.double().abs() + dk.double().abs() + dv.double().abs())
+    oracle.close(g, dq.double() + dk.double() + dv.double(), tol, "sum of the three")
+    f, _ = rotary_frequencies(64, device=dev)
+    a, b = rotary(x, x, f)
+    assert torch.equal(a, b)
+    h = x.view(2, 70, 256)
+    w = torch.ones(256, device=dev, dtype=BF)
+    one, two = (h.detach().clone().requires_grad_() for _ in range(2))
+    y, s = residual_norm(one, two, w)
+    (y.sum() + (s * s.detach()).sum()).backward()
+    assert torch.equal(one.grad, two.grad) and one.grad.data_ptr() != two.grad.data_ptr()
+    both = h.detach().clone().requires_grad_()
+    y, s = residual_norm(both, both, w)
+    (y.sum() + (s * s.detach()).sum()).backward()
+    y2, s2 = residual_norm(h, h, w)
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+    assert torch.equal(both.grad, one.grad + two.grad)
+
+
+def _block(dev, seed):
+    """What one block of a decoder does with the operators: a step that returns its outputs and every gradient."""
+    r = _randn(dev, seed)
+    B, S, A, KV, D, H = 2, 150, 4, 2, 64, 256
+    p = dict(x=r(B, S, H), qkv=r(H, (A + 2 * KV) * D) / 16, out=r(A * D, H) / 16, n1=1 + 0.1 * r(H), n2=1 + 0.1 * r(H), post=1 + 0.1 * r(H),
+             gate=r(B, 1, H))
+    p = {n: t.to(BF).requires_grad_() for n, t in p.items()}
+    f, amp = rotary_frequencies(D, scaling="ntk", factor=2.0, device=dev)
+    lens = torch.tensor([S, 97], dtype=torch.int32, device=dev)
+    dy, dr = r(B, S, H).to(BF), r(B, S, H).to(BF)
+
+    def step():
+        y = rms_norm(p["x"], p["n1"])
+        q, k, v = (y.view(-1, H) @ p["qkv"]).view(B, S, A + 2 * KV, D).split([A, KV, KV], 2)
+        q, k = rotary(q, k, f, amplitude=amp)
+        o = attention(q, k, v, causal=True, kv_len=lens)
+        outs = residual_norm(p["x"], (o.view(-1, A * D) @ p["out"]).view(B, S, H), p["n2"], gate=p["gate"], post_weight=p["post"], scale=0.5)
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, list(p.values()), (dy, dr)))
+
+    return step, p, (f, amp, lens, dy, dr)
+
+
+def test_a_block_of_them_together(dev):
+    """One block's outputs and gradients against the same block in 64 bits on the CPU, where each operator is its definition.
+    Every tensor between two operators is rounded to bf16 (relative error of one rounding: 2^-9 in the mean square at most, and
+    with it the error its gradient carries): 16 of them on the longest way forward and back, and two roundings inside each
+    of five products; independent, so 2^-9 sqrt(26) = 1.0e-2 of a result's norm; twice that is allowed."""
+    step, p, (f, amp, lens, dy, dr) = _block(dev, 21)
+    got = step()
+    B, S, A, KV, D, H = 2, 150, 4, 2, 64, 256
+    w = {n: t.detach().cpu().double().requires_grad_() for n, t in p.items()}
+    f, dy, dr = f.cpu(), dy.cpu().double(), dr.cpu().double()
+
+    def normed(t, weight):
+        return t / torch.sqrt((t * t).mean(-1, keepdim=True) + 1e-6) * weight
+
+    y = normed(w["x"], w["n1"])
+    q, k, v = (y @ w["qkv"]).view(B, S, A + 2 * KV, D).split([A, KV, KV], 2)
+    angle = (torch.arange(S).double()[:, None] * f)[None, :, None, :]
+
+    def turn(t):
+        a, b = t.chunk(2, -1)
+        return amp * torch.cat([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], -1)
+
+    q, k = turn(q), turn(k).repeat_interleave(A // KV, 2)
+    v = v.repeat_interleave(A // KV, 2)
+    s = torch.einsum("bihd,bjhd->bhij", q, k) * D ** -0.5
+    j = torch.arange(S)
+    seen = (j[None, None, :] <= j[None, :, None]) & (j[None, None, :] < lens.cpu()[:, None, None])
+    o = torch.einsum("bhij,bjhd->bihd", s.masked_fill(~seen[:, None], -float("inf")).softmax(-1), v).reshape(B, S, A * D)
+    n = normed(o @ w["out"], w["post"]) * w["gate"]
+    r = w["x"] + 0.5 * n
+    outs = (normed(r, w["n2"]), r)
+    want = [t.detach() for t in outs] + list(torch.autograd.grad(outs, list(w.values()), (dy, dr)))
+    for name, a, b in zip(["y", "r"] + list(p), got, want):
+        off = ((a.cpu().double() - b).norm() / b.norm()).item()
+        assert off < 2 * 2 ** -9 * 26 ** 0.5, (name, off)
+
+
+def test_captured_and_replayed(dev):
+    """Two blocks captured into two graphs, replayed in turn with eager work between: every replay gives the eager bits."""
+    blocks = [_block(dev, s) for s in (31, 32)]
+    want = [b[0]() for b in blocks]
+    graphs, outs = [], []
+    for step, _, _ in blocks:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    for rep in range(4):
+        for i in (0, 1, 0) if rep % 2 else (1, 0):
+            for t in outs[i]:
+                t.fill_(7)
+            graphs[i].replay()
+            again = blocks[1 - i][0]()                                  # eager work right behind the replay
+            torch.cuda.synchronize()
+            for a, b in zip(outs[i], want[i]):
+                assert torch.equal(a, b)
+            for a, b in zip(again, want[1 - i]):
+                assert torch.equal(a, b)
+    x = blocks[0][1]["x"]
+    with torch.no_grad():
+        x.mul_(0.5)                                                     # new values in the captured inputs
+    new = blocks[0][0]()
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs[0], new):
+        assert torch.equal(a, b)
+    assert not torch.equal(new[0], want[0][0])
+
+
+def test_two_streams_at_once(dev):
+    blocks = [_block(dev, s) for s in (41, 42)]
+    want = [b[0]() for b in blocks]
+    streams = [torch.cuda.Stream() for _ in blocks]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for (step, _, _), st in zip(blocks, streams):
+            with torch.cuda.stream(st):
+                got.append(step())
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for a, b in zip(g, w):
+                assert torch.equal(a, b)
+
+
+def test_gpu_refusals(dev):
+    q = torch.zeros(1, 4, 2, 64, device=dev)
+    with pytest.raises(TypeError):
+        attention(q, q, q)
+    with pytest.raises(TypeError):
+        attention(q.half(), q.half(), q.half())
+    with pytest.raises(ValueError):
+        attention(q.to(BF), q.to(BF).cpu(), q.to(BF))
+    f, _ = rotary_frequencies(64)
+    with pytest.raises(ValueError):
+        rotary(q, q, f)                                                 # frequencies on another device
+    with pytest.raises(ValueError):
+        rotary(q, q, f.to(dev), torch.arange(4))
+    with pytest.raises(TypeError):
+        rotary(q.half(), None, f.to(dev))
+    with pytest.raises(ValueError):
+        rotary(q[:, :0], None, f.to(dev))
+    x = torch.zeros(2, 8, device=dev)
+    with pytest.raises(ValueError):
+        residual_norm(x, x, torch.ones(8))
+    with pytest.raises(TypeError):
+        rms_norm(x.half(), torch.ones(8, device=dev))
+    for make in (lambda t: attention(t, t, t), lambda t: rotary(t, None, f.to(dev))[0], lambda t: rms_norm(t, torch.ones(64, device=dev, dtype=BF))):
+        leaf = torch.randn(1, 4, 2, 64, device=dev).to(BF).requires_grad_()
+        g, = torch.autograd.grad(make(leaf).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), leaf)                          # not differentiable twice
+
+
+@pytest.mark.parametrize("kw", [dict(positions="rotary"), dict(kv_heads=2), dict(positions="rotary", kv_heads=1, norm="pre_rms")])
+def test_bert_options_match_the_plain_fp32_model(dev, kw):
+    """The model's options on the GPU in bf16 against the same module on the CPU in fp32, a padded batch at a length that is no
+    tile's multiple.  Bounds as for the published form of the model: 6e-2 of a gradient's norm at worst, 2.5e-2 in the mean."""
+    import copy
+
+    from distributed_tensorflow_amd.models import bert
+
+    torch.manual_seed(0)
+    ref = bert.build(layers=2, hidden=256, heads=4, intermediate=512, vocab=3000, seq_len=150, **kw).train()
+    batch = list(bert.synthetic_batch(8, device="cpu", seed=2, seq_len=150, vocab=3000))
+    batch[2][3, 100:] = 0
+    fused = bert.prepare(copy.deepcopy(ref), dev).train()
+    l_ref = bert.loss_fn(ref, tuple(batch))
+    l_ref.backward()
+    l_fused = bert.loss_fn(fused, tuple(t.to(dev) for t in batch))
+    l_fused.backward()
+    assert abs(l_fused.item() - l_ref.item()) / l_ref.item() < 1e-2
+    worst = []
+    for (n, p), (_, q) in zip(fused.named_parameters(), ref.named_parameters()):
+        if q.grad.norm() > 1e-6:
+            worst.append((((p.grad.float().cpu() - q.grad).norm() / q.grad.norm()).item(), n))
+    worst.sort(reverse=True)
+    assert worst[0][0] < 6e-2, worst[:5]
+    assert sum(w for w, _ in worst) / len(worst) < 2.5e-2, worst[:5]

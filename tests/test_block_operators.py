@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-import transformer_oracles as oracle
+import block_oracles as oracle
 from distributed_tensorflow_amd.ops import attention as A
 from distributed_tensorflow_amd.ops.residual_norm import FusedRMSNorm, residual_norm, rms_norm
 from distributed_tensorflow_amd.ops.rotary import rotary, rotary_frequencies

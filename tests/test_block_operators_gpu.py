@@ -1,9 +1,9 @@
 """The transformer-block kernels (K22 attention of any length, K23 rotary positions, K24 block boundary) against their
-definitions in 64 bits, with tolerances derived in ``transformer_oracles``."""
+definitions in 64 bits, with tolerances derived in ``block_oracles``."""
 import pytest
 import torch
 
-import transformer_oracles as oracle
+import block_oracles as oracle
 
 pytestmark = pytest.mark.gpu
 

@@ -162,6 +162,18 @@ __device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DP / 
         }
 }
 
+// the same as fp32 sums
+template <int DP>
+__device__ __forceinline__ void ag_store_part(float* row, const f32x16 (&acc)[DP / 32], int g, int D) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq)
+            if (32 * dt + 8 * rq < D)
+                *reinterpret_cast<f32x4*>(row + 32 * dt + 8 * rq + 4 * g) =
+                    (f32x4){acc[dt][4 * rq], acc[dt][4 * rq + 1], acc[dt][4 * rq + 2], acc[dt][4 * rq + 3]};
+}
+
 #define AG_LANDED() asm volatile("s_waitcnt vmcnt(0)" ::: "memory")      // this wave's LDS-DMA has arrived
 
 // ---------------------------------------------------------------------------
@@ -289,14 +301,7 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
         return;
     }
     const int64_t n = (int64_t)a.B * a.Sq * a.Hq;
-    float* po = a.ws + (sp * n + row) * a.D;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int rq = 0; rq < 4; ++rq) {
-            const int d = 32 * dt + 8 * rq + 4 * g;
-            if (32 * dt + 8 * rq < a.D) *reinterpret_cast<f32x4*>(po + d) = (f32x4){oacc[dt][4 * rq], oacc[dt][4 * rq + 1], oacc[dt][4 * rq + 2], oacc[dt][4 * rq + 3]};
-        }
+    ag_store_part<DP>(a.ws + (sp * n + row) * a.D, oacc, g, a.D);
     if (g == 0) {
         float* ml = a.ws + (int64_t)a.nsplit * n * a.D + (sp * n + row) * 2;
         ml[0] = m;
@@ -356,7 +361,8 @@ __global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
 
 // ---------------------------------------------------------------------------
 // Backward, dQ: 4 waves x 32 queries, 64 keys a step.  D comes from the matrix instruction too (the diagonal of O . dO^T,
-// summed over d in the order of dP = V . dO^T), so that a query with ONE key, whose O is that V row, has dS = 0 exactly.
+// summed over d in the order of dP = V . dO^T), so that a query with ONE key, whose O is that V row, has dS = 0 exactly.  nsplit > 1:
+// as in the forward, that many workgroups share a tile's keys; they write fp32 sums.
 // ---------------------------------------------------------------------------
 template <int DP>
 __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
@@ -364,9 +370,10 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kv = a.B * a.Hk, units = gridDim.x / a.ntiles;               // units: group x kv
+    const int kv = a.B * a.Hk, units = gridDim.x / a.ntiles;               // units: nsplit x group x kv
     const int t = a.ntiles - 1 - blockIdx.x / units, u = blockIdx.x % units;
-    const int b = u % kv / a.Hk, hk = u % kv % a.Hk, h = hk * a.group + u / kv;
+    const int b = u % kv / a.Hk, hk = u % kv % a.Hk, h = hk * a.group + u / kv % a.group;
+    const int sp = u / kv / a.group;
     const int klen = ag_klen(a, b);
     const int rw = t * BM + wave * 32, i = min(rw + (lane & 31), a.Sq - 1);
     const int vis = ag_vis(a, i, klen), end = ag_vis(a, min(t * BM + BM, a.Sq) - 1, klen);
@@ -384,7 +391,9 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
         kt.load(K, k0, klen, full, wave);
         vt.load(V, k0, klen, full, wave);
     };
-    if (end > 0) fetch(K0, V0, 0);
+    const int steps = (end + BN - 1) / BN;
+    const int kbeg = (int)((int64_t)steps * sp / a.nsplit) * BN, kend = min((int)((int64_t)steps * (sp + 1) / a.nsplit) * BN, end);
+    if (kbeg < kend) fetch(K0, V0, kbeg);
     float dsum = 0.f;
     {
         s16x8 of[KS];
@@ -399,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
     }
     const float lse = a.lse[li];
     const bool valid = rw + (lane & 31) < a.Sq;
-    if (valid && g == 0) a.dsum[li] = dsum;
+    if (valid && g == 0 && sp == 0) a.dsum[li] = dsum;
 
     f32x16 acc[DT];
 #pragma unroll
@@ -435,18 +444,20 @@ __global__ __launch_bounds__(256, 2) void ag_dq_kernel(AgArgs a) {
     };
     AG_LANDED();
     __syncthreads();
-    for (int k0 = 0; k0 < end; k0 += 2 * BN) {
-        if (k0 + BN < end) fetch(K1, V1, k0 + BN);
+    for (int k0 = kbeg; k0 < kend; k0 += 2 * BN) {
+        if (k0 + BN < kend) fetch(K1, V1, k0 + BN);
         if (k0 < hi) step(K0, V0, k0);
         AG_LANDED();
         __syncthreads();
-        if (k0 + BN >= end) break;
-        if (k0 + 2 * BN < end) fetch(K0, V0, k0 + 2 * BN);
+        if (k0 + BN >= kend) break;
+        if (k0 + 2 * BN < kend) fetch(K0, V0, k0 + 2 * BN);
         if (k0 + BN < hi) step(K1, V1, k0 + BN);
         AG_LANDED();
         __syncthreads();
     }
-    if (valid) ag_store_row<DP>(a.dq + row * a.D, acc, a.scale, g, a.D);
+    if (!valid) return;
+    if (a.nsplit == 1) ag_store_row<DP>(a.dq + row * a.D, acc, a.scale, g, a.D);
+    else ag_store_part<DP>(a.ws + ((int64_t)sp * a.B * a.Sq * a.Hq + row) * a.D, acc, g, a.D);
 }
 
 // ---------------------------------------------------------------------------
@@ -586,29 +597,21 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
         return;
     }
     const int64_t n = (int64_t)a.B * a.Sk * a.Hk * a.D;
-    float* pk = a.ws + sp * 2 * n + o;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int rq = 0; rq < 4; ++rq) {
-            const int d = 32 * dt + 8 * rq + 4 * g;
-            if (32 * dt + 8 * rq < a.D) {
-                *reinterpret_cast<f32x4*>(pk + d) = (f32x4){dk[dt][4 * rq], dk[dt][4 * rq + 1], dk[dt][4 * rq + 2], dk[dt][4 * rq + 3]};
-                *reinterpret_cast<f32x4*>(pk + n + d) = (f32x4){dv[dt][4 * rq], dv[dt][4 * rq + 1], dv[dt][4 * rq + 2], dv[dt][4 * rq + 3]};
-            }
-        }
+    ag_store_part<DP>(a.ws + sp * 2 * n + o, dk, g, a.D);
+    ag_store_part<DP>(a.ws + sp * 2 * n + n + o, dv, g, a.D);
 }
 
-// dK (blockIdx.y 0) and dV (1) from the partial sums, 4 elements a thread
-__global__ __launch_bounds__(256) void ag_add_kernel(AgArgs a) {
-    const int64_t n = (int64_t)a.B * a.Sk * a.Hk * a.D, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+// The parts of a tensor of n elements, `stride` floats apart, added in order, scaled and rounded: 4 elements a thread.
+// blockIdx.y 0: first tensor (scaled), 1: second, n floats behind it (dK and dV; dQ alone).
+__global__ __launch_bounds__(256) void ag_add_kernel(const float* parts, int nsplit, int64_t n, int64_t stride, float scale, u16* o0, u16* o1) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
-    const float* p = a.ws + blockIdx.y * n + i;
+    const float* p = parts + blockIdx.y * n + i;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
-    for (int k = 1; k < a.nsplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * 2 * n);
-    if (blockIdx.y == 0) s *= a.scale;
+    for (int k = 1; k < nsplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * stride);
+    if (blockIdx.y == 0) s *= scale;
     const u32x2 r = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
-    *reinterpret_cast<u32x2*>((blockIdx.y ? a.dv : a.dk) + i) = r;
+    *reinterpret_cast<u32x2*>((blockIdx.y ? o1 : o0) + i) = r;
 }
 
 // ---------------------------------------------------------------------------
@@ -657,6 +660,10 @@ static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int D, int causa
 
 extern "C" {
 
+static int ag_dq_splits(int B, int Sq, int Sk, int Hq) {
+    return ag_splits((int64_t)B * Hq * ((Sq - 1) / 128 + 1), (Sk + 63) / 64, 4, 512);
+}
+
 // fp32 workspace of the forward (0: none) and of the backward (D per query and head, then the parts), in floats
 int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
     const int64_t n = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
@@ -664,8 +671,9 @@ int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
 }
 
 int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
-    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, D, causal);
-    return ag_dsum_floats(B, Sq, Hq) + (n > 1 ? n * 2 * B * Sk * Hk * D : 0);
+    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, D, causal), nq = ag_dq_splits(B, Sq, Sk, Hq);
+    const int64_t kv = n > 1 ? n * 2 * B * Sk * Hk * D : 0, q = nq > 1 ? nq * B * Sq * Hq * D : 0;
+    return ag_dsum_floats(B, Sq, Hq) + (kv > q ? kv : q);              // (dQ's parts are added before dK's are written)
 }
 
 // st: the nine element strides (batch, token, head) of q, k, v; ws: dtf_attn_general_fwd_ws floats
@@ -729,11 +737,17 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     if (!ws) return -73;
     if ((int64_t)((Sq + 31) / 32) * a.group > 0x7fffffff) return -72;
     a.ntiles = (Sq - 1) / 128 + 1;
-    a.nsplit = 1;
-    if ((rc = ag_grid((int64_t)B * Hq * a.ntiles, &grid))) return rc;
+    a.nsplit = ag_dq_splits(B, Sq, Sk, Hq);
+    if ((rc = ag_grid((int64_t)B * Hq * a.ntiles * a.nsplit, &grid))) return rc;
     if (D > 64) hipLaunchKernelGGL((ag_dq_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((ag_dq_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
     DTF_CHECK_LAUNCH();
+    if (a.nsplit > 1) {
+        const int64_t n = (int64_t)B * Sq * Hq * D;
+        if ((rc = ag_grid((n + 1023) / 1024, &grid))) return rc;
+        hipLaunchKernelGGL(ag_add_kernel, dim3(grid), dim3(256), 0, stream, a.ws, a.nsplit, n, n, scale, a.dq, (u16*)nullptr);
+        DTF_CHECK_LAUNCH();
+    }
     a.ntiles = (Sk - 1) / 128 + 1;
     a.nsplit = splits;
     if ((rc = ag_grid((int64_t)B * Hk * a.ntiles * splits, &grid))) return rc;
@@ -741,8 +755,9 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     else hipLaunchKernelGGL((ag_dkv_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
     DTF_CHECK_LAUNCH();
     if (splits > 1) {
-        if ((rc = ag_grid(((int64_t)B * Sk * Hk * D + 1023) / 1024, &grid))) return rc;
-        hipLaunchKernelGGL(ag_add_kernel, dim3(grid, 2), dim3(256), 0, stream, a);
+        const int64_t n = (int64_t)B * Sk * Hk * D;
+        if ((rc = ag_grid((n + 1023) / 1024, &grid))) return rc;
+        hipLaunchKernelGGL(ag_add_kernel, dim3(grid, 2), dim3(256), 0, stream, a.ws, splits, n, 2 * n, scale, a.dk, a.dv);
         DTF_CHECK_LAUNCH();
     }
     return 0;

@@ -26,7 +26,10 @@ struct RoArgs {
 
 template <int V, int ESZ> struct RoVec;
 template <> struct RoVec<8, 2> { typedef u32x4 type; };
+template <> struct RoVec<4, 2> { typedef u32x2 type; };
+template <> struct RoVec<2, 2> { typedef unsigned int type; };
 template <> struct RoVec<4, 4> { typedef u32x4 type; };
+template <> struct RoVec<2, 4> { typedef u32x2 type; };
 template <> struct RoVec<1, 2> { typedef unsigned short type; };
 template <> struct RoVec<1, 4> { typedef unsigned int type; };
 
@@ -35,28 +38,33 @@ __device__ __forceinline__ void ro_unpack(const typename RoVec<V, DT == DTF_BF16
     if constexpr (V == 1) {
         if constexpr (DT == DTF_BF16) x[0] = bf16_to_f32(r);
         else x[0] = __uint_as_float(r);
-    } else if constexpr (DT == DTF_BF16) {
-#pragma unroll
-        for (int e = 0; e < V / 2; ++e) {
-            x[2 * e] = __uint_as_float(r[e] << 16);
-            x[2 * e + 1] = __uint_as_float(r[e] & 0xffff0000u);
-        }
     } else {
+        unsigned int w[DT == DTF_BF16 ? V / 2 : V];
+        __builtin_memcpy(w, &r, sizeof(w));
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = __uint_as_float(r[e]);
+        for (int e = 0; e < V; ++e) {
+            if constexpr (DT == DTF_BF16) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+            else x[e] = __uint_as_float(w[e]);
+        }
     }
 }
 
 template <int DT, int V>
 __device__ __forceinline__ typename RoVec<V, DT == DTF_BF16 ? 2 : 4>::type ro_pack(const float (&x)[V]) {
+    typename RoVec<V, DT == DTF_BF16 ? 2 : 4>::type r;
     if constexpr (V == 1) {
-        if constexpr (DT == DTF_BF16) return f32_to_bf16(x[0]);
-        else return __float_as_uint(x[0]);
-    } else if constexpr (DT == DTF_BF16) {
-        return (u32x4){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+        if constexpr (DT == DTF_BF16) r = f32_to_bf16(x[0]);
+        else r = __float_as_uint(x[0]);
     } else {
-        return (u32x4){__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+        unsigned int w[DT == DTF_BF16 ? V / 2 : V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if constexpr (DT == DTF_F32) w[e] = __float_as_uint(x[e]);
+            else if (e & 1) w[e / 2] = pack_bf16x2(x[e - 1], x[e]);
+        }
+        __builtin_memcpy(&r, w, sizeof(w));
     }
+    return r;
 }
 
 // A unit is V pairs (two vectors of V elements) or, past 2m, 2V elements that pass through.
@@ -160,16 +168,23 @@ int dtf_rotary(const void* q, const void* k, void* qo, void* ko, int dt, const i
     if (dt != DTF_F32 && dt != DTF_BF16) return -81;
     RoArgs a{q, k, qo, ko, st[0], st[1], st[2], st[3], st[4], st[5], pos, p_bs, p_ss, offset, (int64_t)B * S,
              inv_freq, S, Hq, Hk, D, m, 1, pos64, amp, sign};
-    const int V = dt == DTF_BF16 ? 8 : 4;
-    int64_t odd = ((uintptr_t)q | (uintptr_t)k | (uintptr_t)qo | (uintptr_t)ko) & 15;
-    for (int i = 0; i < (Hk ? 6 : 3); ++i) odd |= st[i] & (V - 1);
-    const bool vec = !odd && m % V == 0 && (D - 2 * m) % (2 * V) == 0;
-    // tokens of a workgroup: about RO_UNROLL units a thread, one sine and cosine a thread at most
-    const int units = (Hq + Hk) * (D / 2 / (vec ? V : 1));
-    int tb = 256 * RO_UNROLL / units;
-    if (tb > 256 / m) tb = 256 / m;
+    // elements a load: 16 B where the pairs, the rest of the head, the strides and the addresses allow, else the largest half
+    const int esz = dt == DTF_BF16 ? 2 : 4;
+    const uintptr_t al = (uintptr_t)q | (uintptr_t)k | (uintptr_t)qo | (uintptr_t)ko;
+    int V = 16 / esz;
+    auto fits = [&]() {
+        if ((al & (V * esz - 1)) || m % V || (D - 2 * m) % (2 * V)) return false;
+        for (int i = 0; i < (Hk ? 6 : 3); ++i)
+            if (st[i] % V) return false;
+        return true;
+    };
+    while (V > 1 && !fits()) V >>= 1;
+    // tokens of a workgroup: about RO_UNROLL units a thread
+    const int64_t units = (int64_t)(Hq + Hk) * (D / 2 / V);
+    if (units > 0x40000000) return -82;
+    int tb = (int)(256 * RO_UNROLL / units);
+    if (tb > RO_PAIRS / m) tb = RO_PAIRS / m;
     if (tb < 1) tb = 1;
-    if ((int64_t)units > 0x40000000) return -82;
     a.tb = tb;
     const int64_t grid = (a.tokens + tb - 1) / tb;
     if (grid > 0x7fffffff) return -82;
@@ -177,9 +192,10 @@ int dtf_rotary(const void* q, const void* k, void* qo, void* ko, int dt, const i
     if (interleaved) hipLaunchKernelGGL((rotary_kernel<DTY, VV, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);  \
     else hipLaunchKernelGGL((rotary_kernel<DTY, VV, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
     if (dt == DTF_BF16) {
-        if (vec) { RO_LAUNCH(DTF_BF16, 8) } else { RO_LAUNCH(DTF_BF16, 1) }
+        if (V == 8) { RO_LAUNCH(DTF_BF16, 8) } else if (V == 4) { RO_LAUNCH(DTF_BF16, 4) }
+        else if (V == 2) { RO_LAUNCH(DTF_BF16, 2) } else { RO_LAUNCH(DTF_BF16, 1) }
     } else {
-        if (vec) { RO_LAUNCH(DTF_F32, 4) } else { RO_LAUNCH(DTF_F32, 1) }
+        if (V == 4) { RO_LAUNCH(DTF_F32, 4) } else if (V == 2) { RO_LAUNCH(DTF_F32, 2) } else { RO_LAUNCH(DTF_F32, 1) }
     }
 #undef RO_LAUNCH
     DTF_CHECK_LAUNCH();

@@ -103,12 +103,16 @@ def _dense_heads(t):
     return t if t is None or t.stride(3) == 1 else t.contiguous()
 
 
+def _strides(t):
+    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
+
+
 def _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, sign):
     q, k = _dense_heads(q), _dense_heads(k)
     B, S, Hq, D = q.shape
     qo = q.new_empty(q.shape)
     ko = None if k is None else k.new_empty(k.shape)
-    st = (ctypes.c_int64 * 6)(*q.stride()[:3], *((0, 0, 0) if k is None else k.stride()[:3]))
+    st = (ctypes.c_int64 * 6)(*_strides(q), *((0, 0, 0) if k is None else _strides(k)))
     p_bs = p_ss = 0
     if positions is not None:
         p_ss = positions.stride(-1)

@@ -251,8 +251,9 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[u][e]);
         mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
-        if (__any(!(mx <= m + 8.f))) {
-            const float mn = __builtin_elementwise_maximum(m, mx);
+        const bool up = !(mx <= m + 8.f);                                  // (a query's own affair: its result does not depend on the wave's others)
+        if (__any(up)) {
+            const float mn = up ? __builtin_elementwise_maximum(m, mx) : m;
             const float alpha = mn == AG_NEG ? 1.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= alpha;

@@ -135,6 +135,20 @@ def test_attention_other_strides_and_orders(dev):
     assert torch.equal(g1, g2)
 
 
+@pytest.mark.parametrize("Hk", [4, 1])
+def test_attention_of_a_query_does_not_depend_on_the_others(dev, Hk):
+    q, k, v, do = _att_inputs(dev, 2, 300, 300, 4, Hk, 64, False)
+    out = attention(q, k, v)
+    g, = torch.autograd.grad(attention(leaf := q.detach().requires_grad_(), k, v), leaf, do)
+    other = q.clone()
+    other[:, 5], other[:, 200] = other[:, 5] * 50, 0
+    got = attention(other, k, v)
+    h, = torch.autograd.grad(attention(leaf := other.detach().requires_grad_(), k, v), leaf, do)
+    keep = [i for i in range(300) if i not in (5, 200)]
+    assert torch.equal(got[:, keep], out[:, keep]) and torch.equal(h[:, keep], g[:, keep])
+    assert torch.equal(attention(q[1:], k[1:], v[1:]), out[1:])
+
+
 def test_attention_nan_reaches_its_query(dev):
     q, k, v, _ = _att_inputs(dev, 1, 70, 70, 1, 1, 64, False)
     clean = attention(q, k, v, causal=True)

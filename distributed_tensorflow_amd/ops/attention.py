@@ -190,8 +190,8 @@ def _check_general(q, k, v, kv_len, scale):
         raise ValueError("attention: the head dimension must be a multiple of 8 up to 128, got %d" % D)
     if Hq * D >= 1 << 25:
         raise ValueError("attention: %d heads of %d are too many" % (Hq, D))
-    if max(Sq, k.shape[1]) > 1 << 30:
-        raise ValueError("attention: sequences are at most 2**30 tokens long")
+    if max(Sq, k.shape[1]) >= 1 << 30:
+        raise ValueError("attention: sequences are shorter than 2**30 tokens")
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError("attention: scale must be positive and finite, got %r" % (scale,))
     if kv_len is not None and (tuple(kv_len.shape) != (B,) or kv_len.is_floating_point() or kv_len.dtype == torch.bool):
@@ -203,7 +203,7 @@ def attention(q, k, v, causal=False, kv_len=None, scale=None):
     query head h reads key head ``h // (Hq / Hk)``, ``scale`` is ``1 / sqrt(D)`` by default.  ``causal``: query i sees the keys
     ``j <= i + Sk - Sq`` (the last query sees all).  ``kv_len`` (integers ``[B]``, values taken to ``[0, Sk]``): keys at or past
     it are padding and never read.  A query that sees no key gets zeros, and passes no gradient on."""
-    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(max(1, q.shape[-1])) if scale is None else hip.number(scale, "attention: scale")
     _check_general(q, k, v, kv_len, scale)
     if not q.is_cuda:
         return attention_general_reference(q, k, v, causal, kv_len, scale)
@@ -211,7 +211,7 @@ def attention(q, k, v, causal=False, kv_len=None, scale=None):
         raise TypeError("attention: the GPU kernels take bfloat16, got %s" % q.dtype)
     if kv_len is not None:
         if kv_len.dtype != torch.int32:
-            kv_len = kv_len.clamp(0, k.shape[1])
+            kv_len = kv_len.to(torch.int64).clamp(0, k.shape[1])
         kv_len = kv_len.to(device=q.device, dtype=torch.int32).contiguous()
     if not hip.recorded(q, k, v):
         return _general_forward(q, k, v, kv_len, int(bool(causal)), scale)[3]

@@ -22,9 +22,12 @@ struct RnArgs {
     void *dx, *dh, *dgate;                // dh null: not wanted (or equal to dx); dgate: per element only
     float* part;                          // [parts][narr][H]
     int64_t M, rpg;
-    int H, wdt, layer, nbx, narr;         // workgroup id = group * nbx + bx
+    int H, wdt, layer, narr;
+    // Rows come in groups of group_rows (the rows that share a gate row; one group without): workgroup id = (group - group0)
+    // * nbx + bx.  More groups than workgroups go over several launches: `add` to the sums of the launches before.
+    int nbx, add;
+    int64_t group0, group_rows;
     int s_w, s_b, s_pw, s_pb, s_g;        // slot of each sum in a partial row, -1: none
-    int64_t group_rows;                   // rows of one group of workgroups (a shared gate's rows, or M)
     float scale, eps;
 };
 
@@ -228,8 +231,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
     __shared__ float red[2][2][16];
     __shared__ float comb[RB > 1 ? NT * NE : 1];
     const int l = threadIdx.x % TPR, slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), H = a.H;
-    const int64_t group = blockIdx.x / a.nbx;
-    const int bx = blockIdx.x - (int)group * a.nbx;
+    const int64_t group = a.group0 + blockIdx.x / a.nbx;
+    const int bx = blockIdx.x % a.nbx;
     const int64_t r0 = group * a.group_rows;
     const int64_t r1 = r0 + a.group_rows < a.M ? r0 + a.group_rows : a.M;
     const float inv = 1.f / (float)H;
@@ -375,9 +378,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
         }
         if (a.dh && valid) R::store(a.dh, row * H, H, l, dr);
     }
-    float* out = a.part + (int64_t)blockIdx.x * a.narr * H;
-    auto flush = [&](const float* s, int at) {
-        if (at < 0) return;
+    // sum over the workgroup's row slots -> put(column, sum)
+    auto over_slots = [&](const float* s, auto put) {
         if constexpr (RB > 1) {
             __syncthreads();
 #pragma unroll
@@ -389,20 +391,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
                     float z = 0.f;
 #pragma unroll
                     for (int k = 0; k < RB; ++k) z += comb[(k * NE + e) * TPR + l];
-                    if (R::col(l, e) < H) out[(int64_t)at * H + R::col(l, e)] = z;
+                    if (R::col(l, e) < H) put(R::col(l, e), z);
                 }
             }
         } else {
 #pragma unroll
             for (int e = 0; e < NE; ++e)
-                if (R::col(l, e) < H) out[(int64_t)at * H + R::col(l, e)] = s[e];
+                if (R::col(l, e) < H) put(R::col(l, e), s[e]);
         }
+    };
+    float* out = a.part + (int64_t)blockIdx.x * a.narr * H;
+    auto flush = [&](const float* s, int at) {
+        if (at >= 0) over_slots(s, [&](int c, float z) { out[(int64_t)at * H + c] = a.add ? out[(int64_t)at * H + c] + z : z; });
     };
     flush(sw, a.s_w);
     if constexpr (LAYER) flush(sb, a.s_b);
     flush(spw, a.s_pw);
     if constexpr (LAYER) flush(spb, a.s_pb);
-    flush(sg, a.s_g);
+    if (a.gate && !each) {
+        if (a.s_g >= 0) flush(sg, a.s_g);
+        else over_slots(sg, [&](int c, float z) { store1<DT>(a.dgate, group * H + c, z); });      // the group's only workgroup
+    }
 }
 
 struct RnSumArgs {
@@ -447,19 +456,23 @@ static int rn_tpr(int H, int ne) {
     return H <= 64 * ne ? 64 : H <= 128 * ne ? 128 : H <= 256 * ne ? 256 : 512;
 }
 
-static int rn_blocks(int64_t rows, int H, int64_t groups) {
+// workgroups of the backward: nbx share a group's rows, gstep groups go into a launch
+static void rn_grid(int64_t M, int H, int64_t groups, int* nbx, int64_t* gstep) {
     const int tpr = rn_tpr(H, 8), rb = tpr < 256 ? 256 / tpr : 1;
     const int64_t target = tpr <= 256 ? 1024 : H <= 4096 ? 512 : 256;      // what the card holds at once: 16 waves a CU, 8 above H = 4096
-    int64_t n = target / groups, most = (rows + rb - 1) / rb;
-    if (n > most) n = most;
-    return n < 1 ? 1 : (int)n;
+    const int64_t n = target / groups, most = ((M + groups - 1) / groups + rb - 1) / rb;
+    *nbx = (int)(n < 1 ? 1 : n > most ? most : n);
+    *gstep = groups < target ? groups : target;
 }
 
 extern "C" {
 
-// fp32 workspace of the backward: groups = rows of a shared gate (1 without)
+// fp32 workspace of the backward, in floats: groups = rows of a shared gate (1 without), narr = number of sums
 int64_t dtf_residual_norm_ws(int64_t M, int H, int64_t groups, int narr) {
-    return groups * rn_blocks((M + groups - 1) / groups, H, groups) * narr * H;
+    int nbx;
+    int64_t gstep;
+    rn_grid(M, H, groups, &nbx, &gstep);
+    return gstep * nbx * narr * H;
 }
 
 #define RN_SHAPES_FWD(X, DTY, VECT)                                                               \
@@ -510,7 +523,7 @@ int dtf_residual_norm_fwd(const void* x, const void* h, const void* gate, const 
 
 // dgate [M, H] for a gate per element, else [M / rpg, H] through the partials; dw, db, dpw, dpb of type wdt; any of them
 // null where there is no such operand.  ws: dtf_residual_norm_ws(M, H, groups, narr) floats, groups = M / rpg for a shared
-// gate and 1 otherwise, narr = number of sums (dw, db, dpw, dpb, dgate of a shared gate).
+// gate and 1 otherwise, narr = number of sums (dw, db, dpw, dpb, dgate of a shared gate) or more.
 int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const void* w, const void* pw, const void* pb,
                           const float* stats, const void* dy, const void* dr, void* dx, void* dh, void* dgate, void* dw,
                           void* db, void* dpw, void* dpb, float* ws, int dt, int wdt, int layer, int64_t M, int H, int64_t rpg,
@@ -518,43 +531,47 @@ int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const 
     DTF_CLEAR_ERRORS();
     int rc = rn_check(dt, wdt, M, H, rpg);
     if (rc) return rc;
+    if (gate && (!dgate || !h)) return -93;
     RnArgs a{};
     a.x = x; a.h = h; a.gate = gate; a.w = w; a.pw = pw; a.pb = pb; a.stats = const_cast<float*>(stats); a.dy = dy; a.dr = dr;
     a.dx = dx; a.dh = dh; a.part = ws; a.M = M; a.rpg = rpg; a.H = H; a.wdt = wdt; a.layer = layer; a.scale = scale;
     const bool shared = gate && rpg > 1;
-    a.dgate = gate && !shared ? dgate : nullptr;
+    a.dgate = dgate;
     const int64_t groups = shared ? (M + rpg - 1) / rpg : 1;
     a.group_rows = shared ? rpg : M;
-    a.nbx = rn_blocks((M + groups - 1) / groups, H, groups);
+    int64_t gstep;
+    rn_grid(M, H, groups, &a.nbx, &gstep);
     RnSumArgs s{};
     auto sum = [&](void* out, int type, bool on, int64_t rows) {
         if (!on || !out) return -1;
         s.out[s.n] = out; s.dt[s.n] = type; s.first[s.n] = s.n; s.count[s.n] = rows;
-        s.parts[s.n] = rows > 1 ? a.nbx : groups * a.nbx;
+        s.parts[s.n] = rows > 1 ? a.nbx : gstep * a.nbx;
         return s.n++;
     };
     a.s_w = sum(dw, wdt, true, 1);
     a.s_b = sum(db, wdt, layer, 1);
     a.s_pw = sum(dpw, wdt, pw != nullptr, 1);
     a.s_pb = sum(dpb, wdt, layer && pw, 1);
-    a.s_g = sum(dgate, dt, shared, groups);
+    a.s_g = sum(dgate, dt, shared && a.nbx > 1, groups);
     a.narr = s.n;
     const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)pw | (uintptr_t)pb |
-                         (uintptr_t)dy | (uintptr_t)dr | (uintptr_t)dx | (uintptr_t)dh | (uintptr_t)a.dgate;
+                         (uintptr_t)dy | (uintptr_t)dr | (uintptr_t)dx | (uintptr_t)dh | (shared ? 0 : (uintptr_t)dgate);
     const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
     const int tpr = rn_tpr(H, 8), nt = tpr < 256 ? 256 : tpr;
-    const int64_t grid = groups * a.nbx;
-    if (grid > 0x7fffffff) return -92;
 #define RN_BWD_L(DTY, VECT, TPR, NE, SM)                                                                                         \
     if (layer) hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, true, SM>), dim3((unsigned)grid), dim3(nt), 0, stream, a);  \
     else hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, false, SM>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
 #define RN_BWD(DTY, VECT, TPR, NE)                                                        \
     if (DTY == DTF_F32 || wdt == DTY) { RN_BWD_L(DTY, VECT, TPR, NE, true) }               \
     else { RN_BWD_L(DTY, VECT, TPR, NE, false) }
-    RN_DISPATCH(RN_SHAPES_BWD, RN_BWD)
+    for (; a.group0 < groups; a.group0 += gstep) {
+        const int64_t grid = (groups - a.group0 < gstep ? groups - a.group0 : gstep) * a.nbx;
+        a.add = a.group0 > 0;
+        RN_DISPATCH(RN_SHAPES_BWD, RN_BWD)
+        DTF_CHECK_LAUNCH();
+    }
 #undef RN_BWD
 #undef RN_BWD_L
-    DTF_CHECK_LAUNCH();
     if (s.n == 0) return 0;
     s.part = ws; s.H = H; s.narr = s.n;
     int64_t rows = 0;

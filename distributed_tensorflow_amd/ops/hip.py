@@ -133,5 +133,12 @@ def check(rc, what):
         raise RuntimeError("%s failed with code %d" % (what, rc))
 
 
+def number(v, what):
+    """A plain number of an operator's arguments (a tensor's gradient would be lost without a word)."""
+    if isinstance(v, torch.Tensor):
+        raise TypeError("%s is a number, not a tensor" % what)
+    return float(v)
+
+
 def on_gpu(*tensors):
     return any(t is not None and t.is_cuda for t in tensors)

@@ -145,7 +145,7 @@ def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=
     rpg = _checked(x, h, weight, bias, gate, post_weight, post_bias, kind)
     if h is None:
         raise ValueError("residual_norm: h is missing (rms_norm has no residual)")
-    scale, eps = float(scale), float(eps)
+    scale, eps = hip.number(scale, "residual_norm: scale"), float(eps)
     if not x.is_cuda:
         return residual_norm_reference(x, h, weight, bias, gate=gate, scale=scale, post_weight=post_weight, post_bias=post_bias,
                                        kind=kind, eps=eps)

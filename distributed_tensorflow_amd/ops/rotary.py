@@ -145,7 +145,9 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved=False, amplitude=1.0, 
     ``None``; ``positions`` int32 / int64 ``[S]`` or ``[B, S]`` (default ``offset + arange(S)``); ``interleaved``: pairs are
     neighbours ``(x[2j], x[2j+1])`` instead of the two halves ``(x[j], x[j + m])``.  Gradients flow to q and k."""
     _checked(q, k, inv_freq, positions)
-    interleaved, amplitude, offset = int(bool(interleaved)), float(amplitude), int(offset)
+    interleaved, amplitude, offset = int(bool(interleaved)), hip.number(amplitude, "rotary: amplitude"), int(offset)
+    if offset and (positions is not None or abs(offset) > 1 << 52):
+        raise ValueError("rotary: offset goes with the default positions, and to 2**52 either way")
     if not q.is_cuda:
         return rotary_reference(q, k, inv_freq, positions, interleaved=interleaved, amplitude=amplitude, offset=offset)
     if q.numel() == 0 or (k is not None and k.numel() == 0):

@@ -56,6 +56,8 @@ def test_attention_on_the_cpu_rounds_once():
     q, k, v = r(2, 9, 4, 64).to(BF), r(2, 9, 2, 64).to(BF), r(2, 9, 2, 64).to(BF)
     want, tol = oracle.attention(q, k, v, causal=True)
     oracle.close(A.attention(q, k, v, causal=True), want["out"], tol["out"], "out")
+    few = torch.tensor([5, 200], dtype=torch.uint8)
+    assert torch.equal(A.attention(q, k, v, kv_len=few), A.attention(q, k, v, kv_len=torch.tensor([5, 9])))
     poisoned = v.clone()
     poisoned[:, 5:] = float("nan")
     n = torch.tensor([5, 0])
@@ -71,7 +73,7 @@ def test_attention_refusals():
         (ValueError, dict(q=torch.zeros(2, 4, 4, 136), k=torch.zeros(2, 6, 2, 136), v=torch.zeros(2, 6, 2, 136))),
         (ValueError, dict(q=q[:, :0])), (ValueError, dict(k=k[:, :0], v=k[:, :0])), (ValueError, dict(kv_len=torch.tensor([1]))),
         (ValueError, dict(kv_len=torch.tensor([1.0, 2.0]))), (ValueError, dict(kv_len=torch.tensor([True, False]))),
-        (ValueError, dict(scale=0.0)), (ValueError, dict(scale=-1.0)), (ValueError, dict(scale=math.inf)), (ValueError, dict(scale=math.nan)),
+        (TypeError, dict(scale=torch.tensor(1.0))), (ValueError, dict(scale=0.0)), (ValueError, dict(scale=-1.0)), (ValueError, dict(scale=math.inf)), (ValueError, dict(scale=math.nan)),
     ]
     for err, kw in bad:
         with pytest.raises(err):
@@ -124,7 +126,8 @@ def test_rotary_refusals():
         (TypeError, dict(q=q.double(), k=k.double())), (ValueError, dict(inv_freq=f.float())), (ValueError, dict(inv_freq=f[:0])),
         (ValueError, dict(inv_freq=torch.ones(9, dtype=F64))), (ValueError, dict(inv_freq=f.view(2, 4))), (ValueError, dict(inv_freq=f.repeat(2)[::2])),
         (ValueError, dict(positions=torch.zeros(5))), (ValueError, dict(positions=torch.zeros(4, dtype=torch.int64))),
-        (ValueError, dict(positions=torch.zeros(3, 5, dtype=torch.int64))),
+        (ValueError, dict(positions=torch.zeros(3, 5, dtype=torch.int64))), (TypeError, dict(amplitude=torch.ones(()))),
+        (ValueError, dict(positions=torch.zeros(5, dtype=torch.int64), offset=3)), (ValueError, dict(offset=1 << 60)),
     ]
     for err, kw in bad:
         with pytest.raises(err):
@@ -182,7 +185,7 @@ def test_residual_norm_refusals():
         (ValueError, dict(weight=w.to(BF))), (ValueError, dict(bias=w)), (ValueError, dict(kind="layer", bias=w.to(BF))),
         (ValueError, dict(kind="layer", post_bias=w)), (ValueError, dict(gate=w[:9])), (ValueError, dict(gate=w.to(BF))),
         (ValueError, dict(gate=torch.ones(1, 3, 10))), (ValueError, dict(gate=torch.ones(2, 3, 1))), (ValueError, dict(gate=torch.ones(1, 2, 3, 10))),
-        (ValueError, dict(x=torch.zeros(1, 16385), h=torch.zeros(1, 16385), weight=torch.ones(16385))),
+        (TypeError, dict(scale=torch.ones(()))), (ValueError, dict(x=torch.zeros(1, 16385), h=torch.zeros(1, 16385), weight=torch.ones(16385))),
     ]
     for err, kw in bad:
         with pytest.raises(err):

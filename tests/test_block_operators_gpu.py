@@ -109,6 +109,7 @@ def test_attention_key_lengths_outside_the_range(dev):
     b = attention(q, k, v, kv_len=torch.tensor([0, 70, 70], dtype=torch.int32))
     c = attention(q, k, v, kv_len=torch.tensor([-1, 1000, 70], dtype=torch.int32, device=dev))
     assert torch.equal(a, b) and torch.equal(a, c)
+    assert torch.equal(attention(q, k, v, kv_len=torch.tensor([0, 255, 70], dtype=torch.uint8, device=dev)), a)
 
 
 def test_attention_other_strides_and_orders(dev):
@@ -224,6 +225,7 @@ NORM = [
     ((5, 40, 16), "rms", False, "none", 1.0, BF, BF), ((3, 11, 520), "layer", True, "none", 1.0, F32, F32),
     ((700, 128), "rms", True, "channel", 0.5, BF, BF), ((6, 3, 5, 256), "rms", True, "sequence", 0.5, BF, BF),
     ((1500, 2, 64), "layer", False, "sequence", 1.0, BF, BF), ((2, 17, 5000), "rms", False, "channel", 1.0, BF, F32),
+    ((600, 3, 4096), "rms", True, "sequence", 0.5, BF, BF),              # more gate rows than workgroups (as 1500 x 64 above)
 ]
 
 

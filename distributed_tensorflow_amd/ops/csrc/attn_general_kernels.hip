@@ -237,6 +237,15 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int u = 0; u < BN / 32; ++u) s[u] = ag_mfma(at.rows(K, 32 * u, ks), qf[ks], s[u]);
+        // reads run PF ahead of their products (left alone, the compiler waits for two at a time)
+        constexpr int NR = KS * (BN / 32), PF = NR < 8 ? NR : 8;
+        __builtin_amdgcn_sched_group_barrier(0x100, PF, 0);
+#pragma unroll
+        for (int z = 0; z < NR - PF; ++z) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, PF, 0);
         __builtin_amdgcn_s_setprio(1);                                     // a wave past its scores goes first: the other of the SIMD has its products to issue
         if (k0 + BN > lo) {
             const int left = vis - (k0 + 4 * g);

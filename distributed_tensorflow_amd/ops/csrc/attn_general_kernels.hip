@@ -11,6 +11,12 @@
 //   O^T = V^T . P^T    the score accumulator, rounded to bf16, IS the B operand: registers 8s .. 8s+7 of a lane hold the
 //                      keys 16s + 8 (j >> 2) + 4 g + (j & 3), j = 0..7, g = lane >> 5; the A operand V^T comes in that
 //                      key order from two ds_read_b64_tr_b16
+// Bound by the matrix pipe and by power: 4 x 4096 tokens, 16 heads of 128, not causal: forward 555 us (990 TF/s), dQ 757 us
+// (1090 in its three products), dK/dV 1060 us (1040 in its four), where a large library product makes 1400..1600; the card
+// lowers its clock under them (1.8 of 2.4 GHz; on zeros instead of random values the same kernels take a fifth less).
+// Two waves a SIMD carry it: with 64 queries a wave (half the LDS reads, one wave a SIMD) the forward took 918 us, with
+// 32-key steps (three waves) 556, the next step's scores issued under this one's exponentials 640.  LDS reads are one operand
+// of every product, 33..46 % of its cycles.
 // P and dS are rounded to bf16 for the second products (their operands' type: half a step, 2^-9 of each term, random in
 // sign, so the sums keep the accuracy of the bf16 results); scores, maxima, sums, L, D and all accumulators are fp32.
 #include "dtf_common.h"
@@ -38,7 +44,9 @@ struct AgArgs {
 // 4-row block take different PAIRS of chunks (a plain XOR with the row puts rows 0 and 1 on the same pair: 2 extra cycles
 // a transposed read, a quarter of the LDS time), rows + 4 the odd places, rows + 8 the other 16-B half.
 template <int DP>
-__device__ __forceinline__ int ag_swz(int row) { return DP == 128 ? (row & 3) << 1 | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1); }
+__device__ __forceinline__ int ag_swz(int row) {
+    return DP == 128 ? (row & 3) << 1 | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+}
 template <int DP>
 __device__ __forceinline__ int ag_off(int row, int c) {
     return row * (2 * DP) + ((((c >> 1) ^ ag_swz<DP>(row)) << 5) | (((c ^ (row >> 3)) & 1) << 4));
@@ -109,7 +117,8 @@ struct AgTile {
     __device__ __forceinline__ void init(const u16* base_, int64_t rs_, int D, int wave, int lane) {
         row = wave * RPI + lane / (DP / 8);
         const int p = lane % (DP / 8);
-        const int c = (((p >> 1) ^ ag_swz<DP>(row)) << 1) | ((p ^ (row >> 3)) & 1);      // STEP is a multiple of 16: the same for every row of a lane
+        // (STEP is a multiple of 16: the same chunk for every row of a lane)
+        const int c = (((p >> 1) ^ ag_swz<DP>(row)) << 1) | ((p ^ (row >> 3)) & 1);
         col = c * 8 < D;
         base = reinterpret_cast<const char*>(base_);
         rs = rs_ * 2;
@@ -246,7 +255,8 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x8, PF, 0);
-        __builtin_amdgcn_s_setprio(1);                                     // a wave past its scores goes first: the other of the SIMD has its products to issue
+        // a wave past its scores goes first: the SIMD's other wave has products to issue meanwhile (decoder 363 -> 329 us)
+        __builtin_amdgcn_s_setprio(1);
         if (k0 + BN > lo) {
             const int left = vis - (k0 + 4 * g);
 #pragma unroll
@@ -260,7 +270,8 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, s[u][e]);
         mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2e;
-        const bool up = !(mx <= m + 8.f);                                  // (a query's own affair: its result does not depend on the wave's others)
+        // (a query's own affair: its bits do not depend on the wave's other queries)
+        const bool up = !(mx <= m + 8.f);
         if (__any(up)) {
             const float mn = up ? __builtin_elementwise_maximum(m, mx) : m;
             const float alpha = mn == AG_NEG ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -375,10 +386,11 @@ __global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
 // D = rowsum(dO o O) comes from the rounded O, whose half step weighs most where a query sees few keys (dS is then a
 // difference of like terms: 16 tokens, causal: error of dq against 64 bits 3.0e-3 of its norm, 256 tokens 2.6e-3, where one
 // rounding of the result makes 1.65e-3).  Tiles that see up to AG_FEW keys therefore sweep their keys twice and take
-// D = sum P dP in fp32 first: 2.4e-3 at every length, no time that shows.  A query with ONE key has O = that V row: its D is the diagonal of O . dO^T by the matrix instruction,
-// summed over d in the order of dP = V . dO^T, so its dS is 0 exactly.
+// D = sum P dP in fp32 first: 2.4e-3 at every length (8 x 512 tokens with AG_FEW 512: 31 us, with 256: 22 us, as exact).
+// A query with ONE key has O = that V row: its D is the diagonal of O . dO^T by the matrix instruction, summed over d in the
+// order of dP = V . dO^T, so its dS is 0 exactly.
 // ---------------------------------------------------------------------------
-#define AG_FEW 512
+#define AG_FEW 256
 
 template <int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void ag_dq_kernel(AgArgs a) {
@@ -502,16 +514,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void ag_dq_kernel(AgArgs a) 
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dK and dV: 4 waves x 32 keys, 32 queries a step (64 for DP = 64, whose steps were shorter than a fetch), over all query heads of the key head's group (so shared
-// heads' gradients are one fixed-order sum: no atomics).  S = Q . K^T, dP = dO . V^T (a lane owns one key),
-// dV^T += dO^T . P, dK^T += Q^T . dS.  nsplit > 1: that many workgroups share a tile's (head, query) steps, each writes
-// fp32 sums, and ag_add_kernel adds them in order.
+// Backward, dK and dV: 4 waves x 32 keys, 32 queries a step (64 for DP = 64, whose steps were shorter than a fetch: 8 x 1000
+// ragged tokens 78 -> 57 us), over all query heads of the key head's group (so shared heads' gradients are one fixed-order
+// sum: no atomics).  S = Q . K^T, dP = dO . V^T (a lane owns one key), dV^T += dO^T . P, dK^T += Q^T . dS.  nsplit > 1: that
+// many workgroups share a tile's (head, query) steps, each writes fp32 sums, and ag_add_kernel adds them in order.
 // ---------------------------------------------------------------------------
 template <int DP>
 __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, BQ = DP == 64 ? 64 : 32, BM = 128;
     __shared__ __attribute__((aligned(16))) unsigned char Q0[BQ * DP * 2], Q1[BQ * DP * 2], G0[BQ * DP * 2], G1[BQ * DP * 2];
-    __shared__ __attribute__((aligned(16))) float LD0[128], LD1[128];                 // log-sum-exp (0..), D (64..) of a step's queries
+    __shared__ __attribute__((aligned(16))) float LD0[128], LD1[128];      // log-sum-exp (0..), D (64..) of a step's queries
     __shared__ __attribute__((aligned(16))) unsigned char Vimg[DP == 128 ? BM * DP * 2 : 16];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -553,7 +565,8 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     qt.init(a.q + b * a.q_bs, a.q_ss, a.D, wave, lane);
     gt.init(a.dO + (int64_t)b * a.Sq * a.Hq * a.D, (int64_t)a.Hq * a.D, a.D, wave, lane);
     const char *qs = qt.base, *gs = gt.base;
-    int fh = steps ? n0 / steps : 0, fq = steps ? n0 % steps : 0, sq = fq;      // next step to fetch (head of the group, step), to compute
+    // next step to fetch (head of the group, step), to compute
+    int fh = steps ? n0 / steps : 0, fq = steps ? n0 % steps : 0, sq = fq;
     auto fetch = [&](unsigned char* Q, unsigned char* G, float* LD) {
         const int h = hk * a.group + fh, q0 = begin + fq * BQ;
         const bool full = a.D == DP && q0 + BQ <= a.Sq;
@@ -644,7 +657,8 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
 
 // The parts of a tensor of n elements, `stride` floats apart, added in order, scaled and rounded: 4 elements a thread.
 // blockIdx.y 0: first tensor (scaled), 1: second, n floats behind it (dK and dV; dQ alone).
-__global__ __launch_bounds__(256) void ag_add_kernel(const float* parts, int nsplit, int64_t n, int64_t stride, float scale, u16* o0, u16* o1) {
+__global__ __launch_bounds__(256) void ag_add_kernel(const float* parts, int nsplit, int64_t n, int64_t stride, float scale,
+                                                     u16* o0, u16* o1) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     const float* p = parts + blockIdx.y * n + i;
@@ -673,14 +687,17 @@ static int ag_grid(int64_t n, int* out) {
     return 0;
 }
 
-// Workgroups that share a tile: enough for `fill` workgroups, no fewer than `least` steps each.
+// Workgroups that share a tile: enough for `fill` workgroups, no fewer than `least` steps each.  512 are resident.  257 queries
+// on 7000 keys, 32 / 8 heads of 128, forward and join: fill 1 141 us, 512 84 + 12, 1024 85 + 19; one token on 8192 keys: fill 1
+// 147 us, 512 11 + 5.  dQ, 512 tokens, 12 heads of 64: fill 1 14 us, 512 11 + 2.
 static int ag_splits(int64_t grid, int64_t steps, int least, int fill) {
     int64_t n = fill / grid, most = steps / least;
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
 
-// PACK where a 128-row tile of one head's queries would be part empty and the group's rows fill fewer tiles
+// PACK where a 128-row tile of one head's queries would be part empty and the group's rows fill fewer tiles: 64 tokens on 2048
+// keys each, 32 / 8 heads: 94 us (5.7 TB/s of K and V), head by head 366; 257 queries on 7000 keys 84 + 12, 104 + 8.
 static bool ag_pack_rows(int Sq, int group) {
     return group > 1 && Sq <= 512 && ((int64_t)group * Sq + 127) / 128 < (int64_t)group * ((Sq + 127) / 128);
 }
@@ -693,10 +710,12 @@ static int ag_fwd_splits(int B, int Sq, int Sk, int Hq, int Hk) {
     return ag_splits((int64_t)B * (pack ? Hk : Hq) * ((rows + 127) / 128), (Sk + 63) / 64, 4, 512);
 }
 
-// (512 workgroups are resident; causal tiles differ in length, so the longest should be no more than what a slot gets in all)
+// Causal tiles differ in length, so the longest should be no more than what a slot gets in all: 8192 tokens, 16 / 4 heads of
+// 128, dK/dV and the sum of the parts: fill 512 882 + 13 us, 1024 640 + 22, 2048 658 + 48; unshared 1423.
 static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
     const int bq = D > 64 ? 32 : 64;
-    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), (int64_t)((Sq + bq - 1) / bq) * (Hq / Hk), 256 / bq, causal ? 1024 : 512);
+    const int64_t steps = (int64_t)((Sq + bq - 1) / bq) * (Hq / Hk);
+    return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), steps, 256 / bq, causal ? 1024 : 512);
 }
 
 extern "C" {

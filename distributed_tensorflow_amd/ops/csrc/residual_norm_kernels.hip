@@ -11,7 +11,10 @@
 //   dr = dr_in + rstd (a - rhat mean(a rhat) [- mean(a)]),  a = dy w;   dx = dr;   dn = scale gate dr;   dgate = scale n dr
 //   dh = rstd_h (c - hhat mean(c hhat) [- mean(c)]),  c = dn w_post
 // The sums over rows (dw, db, dgate of a shared gate) run in registers over a workgroup's rows, one fp32 partial row per
-// workgroup, and a second kernel adds the partials in a fixed order: no atomics.  Both directions are HBM-bound.
+// workgroup, and a second kernel adds the partials in a fixed order: no atomics.
+// Both directions are HBM-bound.  16384 rows of 4096, bf16, both norms, a gate per sequence: forward 4 streams of 134 MB in
+// 96 us (5.6 TB/s), backward 6 streams in 157 + 6 us (4.9 TB/s; a copy makes 4.95).  Rows whose width is no multiple of 16 B
+// go by elements (1001, bf16, 16384 rows: 68 and 190 us, 1.9 and 1.0 TB/s: their reads are 2 B wide).
 #include "dtf_common.h"
 
 struct RnArgs {
@@ -448,18 +451,21 @@ __global__ __launch_bounds__(1024) void rn_sum_kernel(RnSumArgs a) {
     }
 }
 
-// Threads of a row.  Forward 16 elements a thread.  Backward 8 (its sums and the next row's loads take the registers), but
-// no more than 512 threads to H = 8192: 1024 threads leave 128 registers each, which spill.
+// Threads of a row.  Forward 16 elements a thread.  Backward 8 (its sums and the next row's loads take the registers: 16 at
+// width 4096 left two waves a SIMD, 250 us where 8 take 157), but no more than 512 threads to H = 8192: 1024 leave 128
+// registers each, which spill (8192 rows of 8192, one norm: 145 against 139 us).
 static int rn_tpr(int H, int ne) {
     if (H <= 512) return 64;
     if (H > 8192) return 1024;
     return H <= 64 * ne ? 64 : H <= 128 * ne ? 128 : H <= 256 * ne ? 256 : 512;
 }
 
-// workgroups of the backward: nbx share a group's rows, gstep groups go into a launch
+// Workgroups of the backward: nbx share a group's rows, gstep groups go into a launch.  8 waves a CU.  Backward and the sum
+// of the parts behind it at 16384 rows, 8 against 16 waves a CU: width 4096 (rms, both norms) 157 + 6 against 164 + 9 us,
+// 2048 105 + 5 / 119 + 8; layer norms at 768 (65536 rows) 162 + 5 / 156 + 8.
 static void rn_grid(int64_t M, int H, int64_t groups, int* nbx, int64_t* gstep) {
     const int tpr = rn_tpr(H, 8), rb = tpr < 256 ? 256 / tpr : 1;
-    const int64_t target = tpr <= 256 ? 1024 : H <= 4096 ? 512 : 256;      // what the card holds at once: 16 waves a CU, 8 above H = 4096
+    const int64_t target = tpr <= 256 ? 512 : 256;
     const int64_t n = target / groups, most = ((M + groups - 1) / groups + rb - 1) / rb;
     *nbx = (int)(n < 1 ? 1 : n > most ? most : n);
     *gstep = groups < target ? groups : target;

@@ -39,6 +39,8 @@ struct AgArgs {
     float scale, scale_log2e;
 };
 
+// Tiles are DP = 64 or 128 columns wide in LDS, of which loads and products take DC = 32, 64, 96 or 128 (D, rounded up to 32).
+// Against DC = DP, 4 x 4096 tokens, 8 heads of 32: forward 162 -> 139 us, backward 558 -> 380; of 96: 270 -> 240, 865 -> 757.
 // LDS image of a [rows][DP] bf16 tile, 16-B chunk c of row r, without bank conflicts (256 B of banks) for ds_read_b128 of 16
 // rows at one chunk and for ds_read_b64_tr_b16 of 4 rows x 32 columns: the 32-B chunk is XORed so that rows 0..3 of a
 // 4-row block take different PAIRS of chunks (a plain XOR with the row puts rows 0 and 1 on the same pair: 2 extra cycles
@@ -106,31 +108,31 @@ __device__ const u32x4 ag_zeros = {0u, 0u, 0u, 0u};
 __device__ const float ag_inf = __builtin_inff();
 typedef __attribute__((address_space(1))) const void ag_glb_void;
 
-template <int DP, int ROWS, int NT>
+template <int DP, int DC, int ROWS, int NT>
 struct AgTile {
     static constexpr int RPI = 1024 / (2 * DP), N = ROWS / RPI / (NT / 64), STEP = RPI * (NT / 64);
     const char* base;        // of the matrix (uniform)
     int64_t rs;              // bytes from row to row
     unsigned off;            // this lane's byte offset from the tile's first row (a token stride is below 2^25 elements)
-    int row;
-    bool col;
-    __device__ __forceinline__ void init(const u16* base_, int64_t rs_, int D, int wave, int lane) {
+    int row, c;              // this lane's tile row and chunk
+    __device__ __forceinline__ void init(const u16* base_, int64_t rs_, int wave, int lane) {
         row = wave * RPI + lane / (DP / 8);
         const int p = lane % (DP / 8);
         // (STEP is a multiple of 16: the same chunk for every row of a lane)
-        const int c = (((p >> 1) ^ ag_swz<DP>(row)) << 1) | ((p ^ (row >> 3)) & 1);
-        col = c * 8 < D;
+        c = (((p >> 1) ^ ag_swz<DP>(row)) << 1) | ((p ^ (row >> 3)) & 1);
         base = reinterpret_cast<const char*>(base_);
         rs = rs_ * 2;
         off = (unsigned)row * (unsigned)rs + c * 16;
     }
-    // rows row0 .. row0 + ROWS - 1 of the matrix; `full`: all of them are below limit and D == DP (uniform)
-    __device__ __forceinline__ void load(unsigned char* img, int row0, int limit, bool full, int wave) const {
+    // rows row0 .. row0 + ROWS - 1 of the matrix; columns past DC stay as they are (nothing reads them)
+    __device__ __forceinline__ void load(unsigned char* img, int row0, int limit, int D, int wave) const {
+        const bool full = D == DC && row0 + ROWS <= limit;                 // (uniform)
+        if (DC < DP && c * 8 >= DC) return;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const char* p = base + (row0 + i * STEP) * rs;
             const void* from = p + off;
-            if (!full && !(col && row0 + row + i * STEP < limit)) from = &ag_zeros;
+            if (!full && !(c * 8 < D && row0 + row + i * STEP < limit)) from = &ag_zeros;
             __builtin_amdgcn_global_load_lds((ag_glb_void*)from, (ag_lds_void*)(img + (i * (NT / 64) + wave) * 1024), 16, 0, 0);
         }
     }
@@ -146,20 +148,20 @@ __device__ __forceinline__ int ag_vis(const AgArgs& a, int i, int klen) {
 
 __device__ __forceinline__ int ag_klen(const AgArgs& a, int b) { return a.kv_len ? max(0, min(a.kv_len[b], a.Sk)) : a.Sk; }
 
-template <int DP>
-__device__ __forceinline__ void ag_frags(s16x8 (&f)[DP / 16], const u16* row, int g, int D) {
+template <int DC>
+__device__ __forceinline__ void ag_frags(s16x8 (&f)[DC / 16], const u16* row, int g, int D) {
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
+    for (int ks = 0; ks < DC / 16; ++ks) {
         f[ks] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
         if (16 * ks + 8 * g < D) f[ks] = *reinterpret_cast<const s16x8*>(row + 16 * ks + 8 * g);
     }
 }
 
 // accumulator tiles [32 d][this lane's row] -> 4 bf16 at a time
-template <int DP>
-__device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DP / 32], float f, int g, int D) {
+template <int DC>
+__device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DC / 32], float f, int g, int D) {
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DC / 32; ++dt)
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
             const int d = 32 * dt + 8 * rq + 4 * g;
@@ -172,10 +174,10 @@ __device__ __forceinline__ void ag_store_row(u16* row, const f32x16 (&acc)[DP / 
 }
 
 // the same as fp32 sums
-template <int DP>
-__device__ __forceinline__ void ag_store_part(float* row, const f32x16 (&acc)[DP / 32], int g, int D) {
+template <int DC>
+__device__ __forceinline__ void ag_store_part(float* row, const f32x16 (&acc)[DC / 32], int g, int D) {
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DC / 32; ++dt)
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq)
             if (32 * dt + 8 * rq < D)
@@ -192,9 +194,9 @@ __device__ __forceinline__ void ag_store_part(float* row, const f32x16 (&acc)[DP
 // many heads still fill the matrix tile and read K, V once.  nsplit > 1: that many workgroups share a tile's keys, each
 // writes its (O, m, l), and ag_join_kernel adds them.
 // ---------------------------------------------------------------------------
-template <int DP, bool PACK>
+template <int DP, int DC, bool PACK>
 __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
-    constexpr int KS = DP / 16, DT = DP / 32, BN = 64, BM = 128;
+    constexpr int KS = DC / 16, DT = DC / 32, BN = 64, BM = 128;
     __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -221,14 +223,13 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
     const int kbeg = (int)((int64_t)steps * sp / a.nsplit) * BN, kend = min((int)((int64_t)steps * (sp + 1) / a.nsplit) * BN, end);
 
     s16x8 qf[KS];
-    ag_frags<DP>(qf, a.q + b * a.q_bs + i * a.q_ss + head * a.q_hs, g, a.D);
-    AgTile<DP, BN, 256> kt, vt;
-    kt.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ss, a.D, wave, lane);
-    vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, a.D, wave, lane);
+    ag_frags<DC>(qf, a.q + b * a.q_bs + i * a.q_ss + head * a.q_hs, g, a.D);
+    AgTile<DP, DC, BN, 256> kt, vt;
+    kt.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ss, wave, lane);
+    vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, wave, lane);
     auto fetch = [&](unsigned char* K, unsigned char* V, int k0) {
-        const bool full = a.D == DP && k0 + BN <= klen;
-        kt.load(K, k0, klen, full, wave);
-        vt.load(V, k0, klen, full, wave);
+        kt.load(K, k0, klen, a.D, wave);
+        vt.load(V, k0, klen, a.D, wave);
     };
 
     f32x16 oacc[DT];
@@ -317,12 +318,12 @@ __global__ __launch_bounds__(256, 2) void ag_fwd_kernel(AgArgs a) {
     if (rw + (lane & 31) >= rows) return;
     const int64_t row = ((int64_t)b * a.Sq + i) * a.Hq + head;
     if (a.nsplit == 1) {
-        ag_store_row<DP>(a.out + row * a.D, oacc, l == 0.f ? 0.f : 1.f / l, g, a.D);
+        ag_store_row<DC>(a.out + row * a.D, oacc, l == 0.f ? 0.f : 1.f / l, g, a.D);
         if (g == 0) a.lse[((int64_t)b * a.Hq + head) * a.Sq + i] = l == 0.f ? __builtin_inff() : m + log2f(l);
         return;
     }
     const int64_t n = (int64_t)a.B * a.Sq * a.Hq;
-    ag_store_part<DP>(a.ws + (sp * n + row) * a.D, oacc, g, a.D);
+    ag_store_part<DC>(a.ws + (sp * n + row) * a.D, oacc, g, a.D);
     if (g == 0) {
         float* ml = a.ws + (int64_t)a.nsplit * n * a.D + (sp * n + row) * 2;
         ml[0] = m;
@@ -392,9 +393,9 @@ __global__ __launch_bounds__(256) void ag_join_kernel(AgArgs a) {
 // ---------------------------------------------------------------------------
 #define AG_FEW 256
 
-template <int DP>
+template <int DP, int DC>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void ag_dq_kernel(AgArgs a) {
-    constexpr int KS = DP / 16, DT = DP / 32, BN = 64, BM = 128;
+    constexpr int KS = DC / 16, DT = DC / 32, BN = 64, BM = 128;
     __shared__ __attribute__((aligned(16))) unsigned char K0[BN * DP * 2], K1[BN * DP * 2], V0[BN * DP * 2], V1[BN * DP * 2];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -409,22 +410,21 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void ag_dq_kernel(AgArgs a) 
 
     const int64_t row = ((int64_t)b * a.Sq + i) * a.Hq + h, li = ((int64_t)b * a.Hq + h) * a.Sq + i;
     s16x8 qf[KS], gf[KS];
-    ag_frags<DP>(qf, a.q + b * a.q_bs + i * a.q_ss + h * a.q_hs, g, a.D);
-    ag_frags<DP>(gf, a.dO + row * a.D, g, a.D);
-    AgTile<DP, BN, 256> kt, vt;
-    kt.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ss, a.D, wave, lane);
-    vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, a.D, wave, lane);
+    ag_frags<DC>(qf, a.q + b * a.q_bs + i * a.q_ss + h * a.q_hs, g, a.D);
+    ag_frags<DC>(gf, a.dO + row * a.D, g, a.D);
+    AgTile<DP, DC, BN, 256> kt, vt;
+    kt.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ss, wave, lane);
+    vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, wave, lane);
     auto fetch = [&](unsigned char* K, unsigned char* V, int k0) {
-        const bool full = a.D == DP && k0 + BN <= klen;
-        kt.load(K, k0, klen, full, wave);
-        vt.load(V, k0, klen, full, wave);
+        kt.load(K, k0, klen, a.D, wave);
+        vt.load(V, k0, klen, a.D, wave);
     };
     const int steps = (end + BN - 1) / BN;
     const int kbeg = (int)((int64_t)steps * sp / a.nsplit) * BN, kend = min((int)((int64_t)steps * (sp + 1) / a.nsplit) * BN, end);
     float dsum = 0.f;
     {
         s16x8 of[KS];
-        ag_frags<DP>(of, a.o + row * a.D, g, a.D);
+        ag_frags<DC>(of, a.o + row * a.D, g, a.D);
         f32x16 x = ag_zero();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) x = ag_mfma(of[ks], gf[ks], x);
@@ -509,8 +509,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void ag_dq_kernel(AgArgs a) 
     };
     sweep(kbeg, kend, step);
     if (!valid) return;
-    if (a.nsplit == 1) ag_store_row<DP>(a.dq + row * a.D, acc, a.scale, g, a.D);
-    else ag_store_part<DP>(a.ws + ((int64_t)sp * a.B * a.Sq * a.Hq + row) * a.D, acc, g, a.D);
+    if (a.nsplit == 1) ag_store_row<DC>(a.dq + row * a.D, acc, a.scale, g, a.D);
+    else ag_store_part<DC>(a.ws + ((int64_t)sp * a.B * a.Sq * a.Hq + row) * a.D, acc, g, a.D);
 }
 
 // ---------------------------------------------------------------------------
@@ -519,9 +519,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void ag_dq_kernel(AgArgs a) 
 // sum: no atomics).  S = Q . K^T, dP = dO . V^T (a lane owns one key), dV^T += dO^T . P, dK^T += Q^T . dS.  nsplit > 1: that
 // many workgroups share a tile's (head, query) steps, each writes fp32 sums, and ag_add_kernel adds them in order.
 // ---------------------------------------------------------------------------
-template <int DP>
+template <int DP, int DC>
 __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
-    constexpr int KS = DP / 16, DT = DP / 32, BQ = DP == 64 ? 64 : 32, BM = 128;
+    constexpr int KS = DC / 16, DT = DC / 32, BQ = DP == 64 ? 64 : 32, BM = 128;
     __shared__ __attribute__((aligned(16))) unsigned char Q0[BQ * DP * 2], Q1[BQ * DP * 2], G0[BQ * DP * 2], G1[BQ * DP * 2];
     __shared__ __attribute__((aligned(16))) float LD0[128], LD1[128];      // log-sum-exp (0..), D (64..) of a step's queries
     __shared__ __attribute__((aligned(16))) unsigned char Vimg[DP == 128 ? BM * DP * 2 : 16];
@@ -539,12 +539,12 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     // K rows in registers; V rows too for DP = 64, in LDS for DP = 128 (32 registers more would leave one wave a SIMD)
     const bool seen = j < klen;
     s16x8 kf[KS], vf[DP == 128 ? 1 : KS];
-    ag_frags<DP>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
+    ag_frags<DC>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
     if constexpr (DP == 128) {
-        AgTile<DP, BM, 256> vt;
-        vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, a.D, wave, lane);
-        vt.load(Vimg, t * BM, klen, a.D == DP && t * BM + BM <= klen, wave);
-    } else ag_frags<DP>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, a.D);
+        AgTile<DP, DC, BM, 256> vt;
+        vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, wave, lane);
+        vt.load(Vimg, t * BM, klen, a.D, wave);
+    } else ag_frags<DC>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, a.D);
     if (!seen) {                                       // padded keys: whatever they hold takes no part
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -561,19 +561,18 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     const int steps = t * BM < klen && begin < a.Sq ? (a.Sq - begin + BQ - 1) / BQ : 0;
     const int64_t total = (int64_t)steps * a.group;
     const int n0 = (int)(total * sp / a.nsplit), n1 = (int)(total * (sp + 1) / a.nsplit);
-    AgTile<DP, BQ, 256> qt, gt;
-    qt.init(a.q + b * a.q_bs, a.q_ss, a.D, wave, lane);
-    gt.init(a.dO + (int64_t)b * a.Sq * a.Hq * a.D, (int64_t)a.Hq * a.D, a.D, wave, lane);
+    AgTile<DP, DC, BQ, 256> qt, gt;
+    qt.init(a.q + b * a.q_bs, a.q_ss, wave, lane);
+    gt.init(a.dO + (int64_t)b * a.Sq * a.Hq * a.D, (int64_t)a.Hq * a.D, wave, lane);
     const char *qs = qt.base, *gs = gt.base;
     // next step to fetch (head of the group, step), to compute
     int fh = steps ? n0 / steps : 0, fq = steps ? n0 % steps : 0, sq = fq;
     auto fetch = [&](unsigned char* Q, unsigned char* G, float* LD) {
         const int h = hk * a.group + fh, q0 = begin + fq * BQ;
-        const bool full = a.D == DP && q0 + BQ <= a.Sq;
         qt.base = qs + h * a.q_hs * 2;
         gt.base = gs + (int64_t)h * a.D * 2;
-        qt.load(Q, q0, a.Sq, full, wave);
-        gt.load(G, q0, a.Sq, full, wave);
+        qt.load(Q, q0, a.Sq, a.D, wave);
+        gt.load(G, q0, a.Sq, a.D, wave);
         if (wave < 2) {                                // no query: log-sum-exp +inf (P = 0) and D 0
             const float* from = (wave ? a.dsum : a.lse) + ((int64_t)b * a.Hq + h) * a.Sq + q0 + lane;
             if (q0 + lane >= a.Sq) from = wave ? reinterpret_cast<const float*>(&ag_zeros) : &ag_inf;
@@ -646,13 +645,13 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     if (j >= a.Sk) return;
     const int64_t o = (((int64_t)b * a.Sk + j) * a.Hk + hk) * a.D;
     if (a.nsplit == 1) {
-        ag_store_row<DP>(a.dk + o, dk, a.scale, g, a.D);
-        ag_store_row<DP>(a.dv + o, dv, 1.f, g, a.D);
+        ag_store_row<DC>(a.dk + o, dk, a.scale, g, a.D);
+        ag_store_row<DC>(a.dv + o, dv, 1.f, g, a.D);
         return;
     }
     const int64_t n = (int64_t)a.B * a.Sk * a.Hk * a.D;
-    ag_store_part<DP>(a.ws + sp * 2 * n + o, dk, g, a.D);
-    ag_store_part<DP>(a.ws + sp * 2 * n + n + o, dv, g, a.D);
+    ag_store_part<DC>(a.ws + sp * 2 * n + o, dk, g, a.D);
+    ag_store_part<DC>(a.ws + sp * 2 * n + n + o, dv, g, a.D);
 }
 
 // The parts of a tensor of n elements, `stride` floats apart, added in order, scaled and rounded: 4 elements a thread.
@@ -718,6 +717,10 @@ static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int D, int causa
     return ag_splits((int64_t)B * Hk * ((Sk - 1) / 128 + 1), steps, 256 / bq, causal ? 1024 : 512);
 }
 
+#define AG_BY_WIDTH(X)                                              \
+    if (D > 96) { X(128, 128) } else if (D > 64) { X(128, 96) }     \
+    else if (D > 32) { X(64, 64) } else { X(64, 32) }
+
 extern "C" {
 
 static int ag_dq_splits(int B, int Sq, int Sk, int Hq) {
@@ -756,13 +759,11 @@ int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, f
     a.nsplit = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
     if (a.nsplit > 1 && !ws) return -73;
     if ((rc = ag_grid((int64_t)B * (pack ? Hk : Hq) * a.ntiles * a.nsplit, &grid))) return rc;
-    if (D > 64) {
-        if (pack) hipLaunchKernelGGL((ag_fwd_kernel<128, true>), dim3(grid), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((ag_fwd_kernel<128, false>), dim3(grid), dim3(256), 0, stream, a);
-    } else {
-        if (pack) hipLaunchKernelGGL((ag_fwd_kernel<64, true>), dim3(grid), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((ag_fwd_kernel<64, false>), dim3(grid), dim3(256), 0, stream, a);
-    }
+#define AG_FWD(DP, DC)                                                                                     \
+    if (pack) hipLaunchKernelGGL((ag_fwd_kernel<DP, DC, true>), dim3(grid), dim3(256), 0, stream, a);      \
+    else hipLaunchKernelGGL((ag_fwd_kernel<DP, DC, false>), dim3(grid), dim3(256), 0, stream, a);
+    AG_BY_WIDTH(AG_FWD)
+#undef AG_FWD
     DTF_CHECK_LAUNCH();
     if (a.nsplit > 1) {
         const int py = a.nsplit <= 2 ? 2 : a.nsplit <= 4 ? 4 : 8;
@@ -799,8 +800,9 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     a.ntiles = (Sq - 1) / 128 + 1;
     a.nsplit = ag_dq_splits(B, Sq, Sk, Hq);
     if ((rc = ag_grid((int64_t)B * Hq * a.ntiles * a.nsplit, &grid))) return rc;
-    if (D > 64) hipLaunchKernelGGL((ag_dq_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((ag_dq_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
+#define AG_DQ(DP, DC) hipLaunchKernelGGL((ag_dq_kernel<DP, DC>), dim3(grid), dim3(256), 0, stream, a);
+    AG_BY_WIDTH(AG_DQ)
+#undef AG_DQ
     DTF_CHECK_LAUNCH();
     if (a.nsplit > 1) {
         const int64_t n = (int64_t)B * Sq * Hq * D;
@@ -811,8 +813,9 @@ int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void
     a.ntiles = (Sk - 1) / 128 + 1;
     a.nsplit = splits;
     if ((rc = ag_grid((int64_t)B * Hk * a.ntiles * splits, &grid))) return rc;
-    if (D > 64) hipLaunchKernelGGL((ag_dkv_kernel<128>), dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((ag_dkv_kernel<64>), dim3(grid), dim3(256), 0, stream, a);
+#define AG_DKV(DP, DC) hipLaunchKernelGGL((ag_dkv_kernel<DP, DC>), dim3(grid), dim3(256), 0, stream, a);
+    AG_BY_WIDTH(AG_DKV)
+#undef AG_DKV
     DTF_CHECK_LAUNCH();
     if (splits > 1) {
         const int64_t n = (int64_t)B * Sk * Hk * D;

@@ -41,6 +41,9 @@ ATT = [
     (2, 1, 300, 8, 2, 128, False, (300, 5)), (2, 7, 515, 8, 1, 128, True, None), (1, 100, 40, 2, 2, 64, True, None),
     (2, 140, 1, 3, 1, 64, True, None), (1, 257, 1100, 4, 4, 64, True, (900,)), (4, 1, 129, 4, 4, 64, False, (0, 1, 64, 129)),
     (1, 31, 2000, 40, 8, 128, True, None), (1, 513, 65, 2, 1, 128, False, None),
+    # every width of the products, with and without columns behind the head's
+    (2, 150, 150, 4, 2, 24, True, (150, 31)), (2, 1, 400, 4, 1, 32, False, (400, 9)), (1, 90, 333, 8, 1, 40, False, None),
+    (1, 200, 200, 3, 3, 72, True, None), (2, 3, 700, 8, 2, 96, True, None), (1, 130, 190, 2, 1, 104, False, (150,)),
 ]
 
 

@@ -124,8 +124,9 @@ def _operand(t):
     """As it is where the kernels can address it (dense head dimension, 16-B aligned rows, tokens less than 2^25 elements
     apart), else a contiguous copy."""
     st = t.stride()
-    if st[3] == 1 and (st[1] < 1 << 25 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
-        return t
+    if st[3] == 1 and (st[1] < 1 << 25 or t.shape[1] == 1) and t.data_ptr() % 16 == 0:
+        if all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -202,7 +203,11 @@ def attention(q, k, v, causal=False, kv_len=None, scale=None):
     """``softmax(scale q k^T) v`` per head: ``q`` ``[B, Sq, Hq, D]``, ``k`` and ``v`` ``[B, Sk, Hk, D]`` -> ``[B, Sq, Hq, D]``;
     query head h reads key head ``h // (Hq / Hk)``, ``scale`` is ``1 / sqrt(D)`` by default.  ``causal``: query i sees the keys
     ``j <= i + Sk - Sq`` (the last query sees all).  ``kv_len`` (integers ``[B]``, values taken to ``[0, Sk]``): keys at or past
-    it are padding and never read.  A query that sees no key gets zeros, and passes no gradient on."""
+    it are padding and never read.  A query that sees no key gets zeros, and passes no gradient on.  (An infinity or NaN at a
+    key that only causality hides may reach queries before it, as in any product with a probability of 0.)
+
+    Scores, softmax statistics and sums are fp32; probabilities and their gradients are rounded to bf16 for the second products.
+    Gradients are sums in a fixed order (no atomics) and do not depend on what else is in the batch."""
     scale = 1.0 / math.sqrt(max(1, q.shape[-1])) if scale is None else hip.number(scale, "attention: scale")
     _check_general(q, k, v, kv_len, scale)
     if not q.is_cuda:

@@ -180,6 +180,8 @@ def _check_general(q, k, v, kv_len, scale):
             raise ValueError("attention: %s is [B, S, heads, D], got %s" % (n, tuple(t.shape)))
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError("attention: q, k and v must share dtype and device")
+        if not t.is_floating_point():
+            raise TypeError("attention: q, k and v are floating-point tensors, got %s" % t.dtype)
     B, Sq, Hq, D = q.shape
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
         raise ValueError("attention: q %s, k %s and v %s do not fit together" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))

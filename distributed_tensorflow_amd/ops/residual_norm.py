@@ -10,6 +10,7 @@ bf16 or fp32, any width to 16384; parameters in the activations' type or fp32.  
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 import torch.nn as nn
@@ -58,6 +59,13 @@ def _rows_per_gate(x, gate):
                 return rows
     raise ValueError("residual_norm: a gate for x %s is x's own shape, or that with 1 for its last leading dimensions (one row a "
                      "sequence), or [%d]; got %s" % (tuple(x.shape), x.shape[-1], tuple(gate.shape)))
+
+
+def _checked_eps(eps):
+    eps = hip.number(eps, "residual_norm: eps")
+    if not 0 <= eps < math.inf:
+        raise ValueError("residual_norm: eps must be finite and not negative, got %r" % eps)
+    return eps
 
 
 def _checked(x, h, weight, bias, gate, post_weight, post_bias, kind):
@@ -145,7 +153,7 @@ def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=
     rpg = _checked(x, h, weight, bias, gate, post_weight, post_bias, kind)
     if h is None:
         raise ValueError("residual_norm: h is missing (rms_norm has no residual)")
-    scale, eps = hip.number(scale, "residual_norm: scale"), float(eps)
+    scale, eps = hip.number(scale, "residual_norm: scale"), _checked_eps(eps)
     if not x.is_cuda:
         return residual_norm_reference(x, h, weight, bias, gate=gate, scale=scale, post_weight=post_weight, post_bias=post_bias,
                                        kind=kind, eps=eps)
@@ -156,9 +164,10 @@ def residual_norm(x, h, weight, bias=None, *, gate=None, scale=1.0, post_weight=
 def rms_norm(x, weight, eps=1e-6):
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension: the norm in front of a first block."""
     _checked(x, None, weight, None, None, None, None, "rms")
+    eps = _checked_eps(eps)
     if not x.is_cuda:
         return _normed(x.float(), weight, None, "rms", eps).to(x.dtype)
-    args = x, None, weight, None, None, None, None, 1, 1.0, 0, float(eps)
+    args = x, None, weight, None, None, None, None, 1, 1.0, 0, eps
     return (_ResidualNorm.apply(*args) if hip.recorded(x, weight) else _forward(*args))[0]
 
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -73,6 +74,8 @@ def _checked(q, k, inv_freq, positions):
         raise ValueError("rotary: the head dimension must be even, got %d" % D)
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous() or inv_freq.device != q.device:
         raise ValueError("rotary: inv_freq is a contiguous float64 vector on the operands' device (rotary_frequencies)")
+    if inv_freq.requires_grad:
+        raise ValueError("rotary: inv_freq gets no gradient (pass inv_freq.detach())")
     if not 0 < 2 * inv_freq.numel() <= D or inv_freq.numel() > 1024:
         raise ValueError("rotary: %d pairs do not fit a head of %d" % (inv_freq.numel(), D))
     if positions is not None:
@@ -145,7 +148,7 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved=False, amplitude=1.0, 
     ``None``; ``positions`` int32 / int64 ``[S]`` or ``[B, S]`` (default ``offset + arange(S)``); ``interleaved``: pairs are
     neighbours ``(x[2j], x[2j+1])`` instead of the two halves ``(x[j], x[j + m])``.  Gradients flow to q and k."""
     _checked(q, k, inv_freq, positions)
-    interleaved, amplitude, offset = int(bool(interleaved)), hip.number(amplitude, "rotary: amplitude"), int(offset)
+    interleaved, amplitude, offset = int(bool(interleaved)), hip.number(amplitude, "rotary: amplitude"), operator.index(offset)
     if offset and (positions is not None or abs(offset) > 1 << 52):
         raise ValueError("rotary: offset goes with the default positions, and to 2**52 either way")
     if not q.is_cuda:

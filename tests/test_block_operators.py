@@ -74,6 +74,7 @@ def test_attention_refusals():
         (ValueError, dict(q=q[:, :0])), (ValueError, dict(k=k[:, :0], v=k[:, :0])), (ValueError, dict(kv_len=torch.tensor([1]))),
         (ValueError, dict(kv_len=torch.tensor([1.0, 2.0]))), (ValueError, dict(kv_len=torch.tensor([True, False]))),
         (TypeError, dict(scale=torch.tensor(1.0))), (ValueError, dict(scale=0.0)), (ValueError, dict(scale=-1.0)), (ValueError, dict(scale=math.inf)), (ValueError, dict(scale=math.nan)),
+        (TypeError, dict(q=q.int(), k=k.int(), v=k.int())),
     ]
     for err, kw in bad:
         with pytest.raises(err):
@@ -128,6 +129,7 @@ def test_rotary_refusals():
         (ValueError, dict(positions=torch.zeros(5))), (ValueError, dict(positions=torch.zeros(4, dtype=torch.int64))),
         (ValueError, dict(positions=torch.zeros(3, 5, dtype=torch.int64))), (TypeError, dict(amplitude=torch.ones(()))),
         (ValueError, dict(positions=torch.zeros(5, dtype=torch.int64), offset=3)), (ValueError, dict(offset=1 << 60)),
+        (TypeError, dict(offset=0.5)), (ValueError, dict(inv_freq=f.clone().requires_grad_())),
     ]
     for err, kw in bad:
         with pytest.raises(err):
@@ -186,6 +188,7 @@ def test_residual_norm_refusals():
         (ValueError, dict(kind="layer", post_bias=w)), (ValueError, dict(gate=w[:9])), (ValueError, dict(gate=w.to(BF))),
         (ValueError, dict(gate=torch.ones(1, 3, 10))), (ValueError, dict(gate=torch.ones(2, 3, 1))), (ValueError, dict(gate=torch.ones(1, 2, 3, 10))),
         (TypeError, dict(scale=torch.ones(()))), (ValueError, dict(x=torch.zeros(1, 16385), h=torch.zeros(1, 16385), weight=torch.ones(16385))),
+        (TypeError, dict(eps=torch.ones(()))), (ValueError, dict(eps=-1e-6)), (ValueError, dict(eps=math.nan)), (ValueError, dict(eps=math.inf)),
     ]
     for err, kw in bad:
         with pytest.raises(err):

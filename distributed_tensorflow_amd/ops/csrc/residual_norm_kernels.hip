@@ -13,9 +13,10 @@
 // The sums over rows (dw, db, dgate of a shared gate) run in registers over a workgroup's rows, one fp32 partial row per
 // workgroup, and a second kernel adds the partials in a fixed order: no atomics.
 // Both directions are HBM-bound.  16384 rows of 4096, bf16, both norms, a gate per sequence: forward 4 streams of 134 MB in
-// 96 us (5.6 TB/s), backward 6 streams in 157 + 6 us (4.9 TB/s; a copy makes 4.95).  Rows whose width is no multiple of 16 B
-// go by elements (1001, bf16, 16384 rows: 68 and 190 us, 1.9 and 1.0 TB/s: their reads are 2 B wide).
+// 96 us (5.6 TB/s), backward 6 streams in 157 + 6 us (4.9 TB/s; a copy makes 4.95).  Without the gate, widths that are no
+// multiple of 16 B: 4094 100 and 157 us, 4095 (every other row begins inside a dword) 120 and 206.
 #include "dtf_common.h"
+#include <type_traits>
 
 struct RnArgs {
     const void *x, *h, *gate, *w, *b, *pw, *pb;
@@ -34,69 +35,104 @@ struct RnArgs {
     float scale, eps;
 };
 
-// element e of thread l's share of a row: vectors of V when rows allow 16-B access, else every TPR-th element
-template <int DT, bool VEC, int TPR, int NE>
+// Element e of thread l's share of a row: vectors of 16 B.  RN_ALIGNED: rows begin and end with one.  RN_ANY: they begin
+// anywhere (the hardware takes unaligned vectors), and the thread whose vector would pass the row's end takes the row's last
+// 16 B, of which the elements that its neighbour has too are zero in it (a shorter load there breaks the loads in flight:
+// 16384 rows of 4094, bf16, backward 398 us against 157; all by elements 950).  RN_TINY: rows shorter than a vector.
+enum { RN_ALIGNED, RN_ANY, RN_TINY };
+typedef u32x4 rn_any4 __attribute__((aligned(2)));
+typedef unsigned int rn_any1 __attribute__((aligned(2)));
+
+template <int DT, int MODE, int TPR, int NE>
 struct RnRow {
-    static constexpr int V = DT == DTF_BF16 ? 8 : 4;
+    static constexpr int V = DT == DTF_BF16 ? 8 : 4, ESZ = 16 / V;
+    typedef typename std::conditional<MODE == RN_ALIGNED, u32x4, rn_any4>::type vec;
     struct Raw {                          // as it comes from memory
-        u32x4 q[VEC ? NE / V : 1];
-        float f[VEC ? 1 : NE];
+        u32x4 q[NE / V];
     };
-    static __device__ __forceinline__ int col(int l, int e) { return VEC ? ((e / V) * TPR + l) * V + e % V : e * TPR + l; }
+    static __device__ __forceinline__ int first(int l, int c, int H) {     // column of vector c's first element
+        const int at = (c * TPR + l) * V;
+        return MODE == RN_ANY ? min(at, H - V) : at;
+    }
+    static __device__ __forceinline__ int over(int l, int c, int H) { return (c * TPR + l) * V - (H - V); }
+    static __device__ __forceinline__ int col(int l, int e, int H) { return first(l, e / V, H) + e % V; }
+    static __device__ __forceinline__ bool has(int l, int e, int H) {
+        return MODE == RN_ANY ? e % V >= over(l, e / V, H) : col(l, e, H) < H;
+    }
     // off (elements): where the row begins, uniform in a wave -- so the address is a scalar base and a 32-bit lane offset
     static __device__ __forceinline__ void fetch(const void* base, int64_t off, int H, int l, Raw& r) {
-        const char* p = reinterpret_cast<const char*>(base) + off * (16 / V);
-        if constexpr (VEC) {
+        const char* p = reinterpret_cast<const char*>(base) + off * ESZ;
+#pragma unroll
+        for (int c = 0; c < NE / V; ++c) {
+            r.q[c] = (u32x4){0u, 0u, 0u, 0u};
+            if ((c * TPR + l) * V >= H) continue;
+            if constexpr (MODE == RN_TINY) {                               // (c, l = 0, H < V)
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (k < H) {
+                        if constexpr (DT == DTF_F32) r.q[c][k] = reinterpret_cast<const unsigned int*>(p)[k];
+                        else r.q[c][k / 2] |= (unsigned int)reinterpret_cast<const unsigned short*>(p)[k] << (k & 1) * 16;
+                    }
+            } else r.q[c] = *reinterpret_cast<const vec*>(p + (unsigned)(first(l, c, H) * ESZ));
+        }
+    }
+    // what a thread does not own -> 0
+    static __device__ __forceinline__ void trim(Raw& r, int H, int l) {
+        if constexpr (MODE == RN_ANY) {
 #pragma unroll
             for (int c = 0; c < NE / V; ++c) {
-                const int at = (c * TPR + l) * V;
-                r.q[c] = (u32x4){0u, 0u, 0u, 0u};
-                if (at < H) r.q[c] = *reinterpret_cast<const u32x4*>(p + (unsigned)(at * (16 / V)));
-            }
-        } else {
+                const int n = over(l, c, H);
 #pragma unroll
-            for (int e = 0; e < NE; ++e) r.f[e] = e * TPR + l < H ? load1<DT>(p + (unsigned)((e * TPR + l) * (16 / V)), 0) : 0.f;
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == DTF_F32) r.q[c][k] = k >= n ? r.q[c][k] : 0u;
+                    else r.q[c][k] &= 2 * k >= n ? 0xffffffffu : 2 * k + 1 >= n ? 0xffff0000u : 0u;
+                }
+            }
         }
     }
     static __device__ __forceinline__ void expand(const Raw& r, float (&v)[NE]) {
-        if constexpr (VEC) {
 #pragma unroll
-            for (int c = 0; c < NE / V; ++c)
+        for (int c = 0; c < NE / V; ++c)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if constexpr (DT == DTF_BF16) {
-                        v[c * V + 2 * k] = __uint_as_float(r.q[c][k] << 16);
-                        v[c * V + 2 * k + 1] = __uint_as_float(r.q[c][k] & 0xffff0000u);
-                    } else v[c * V + k] = __uint_as_float(r.q[c][k]);
-                }
-        } else {
-#pragma unroll
-            for (int e = 0; e < NE; ++e) v[e] = r.f[e];
-        }
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (DT == DTF_BF16) {
+                    v[c * V + 2 * k] = __uint_as_float(r.q[c][k] << 16);
+                    v[c * V + 2 * k + 1] = __uint_as_float(r.q[c][k] & 0xffff0000u);
+                } else v[c * V + k] = __uint_as_float(r.q[c][k]);
+            }
+    }
+    static __device__ __forceinline__ void row(Raw r, int H, int l, float (&v)[NE]) {
+        trim(r, H, l);
+        expand(r, v);
     }
     static __device__ __forceinline__ void load(const void* base, int64_t off, int H, int l, float (&v)[NE]) {
         Raw r;
         fetch(base, off, H, l, r);
-        expand(r, v);
+        row(r, H, l, v);
     }
     static __device__ __forceinline__ void store(void* base, int64_t off, int H, int l, const float (&v)[NE]) {
-        char* p = reinterpret_cast<char*>(base) + off * (16 / V);
-        if constexpr (VEC) {
+        char* p = reinterpret_cast<char*>(base) + off * ESZ;
 #pragma unroll
-            for (int c = 0; c < NE / V; ++c) {
-                const int at = (c * TPR + l) * V;
-                u32x4 q;
+        for (int c = 0; c < NE / V; ++c) {
+            u32x4 q;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (DT == DTF_BF16) q[k] = pack_bf16x2(v[c * V + 2 * k], v[c * V + 2 * k + 1]);
+                else q[k] = __float_as_uint(v[c * V + k]);
+            }
+            const int at = (c * TPR + l) * V;
+            char* t = p + (unsigned)(first(l, c, H) * ESZ);
+            if (at >= H) continue;
+            if (MODE == RN_ALIGNED || (MODE == RN_ANY && over(l, c, H) <= 0)) *reinterpret_cast<vec*>(t) = q;
+            else {                                                         // bytes from `lo` on, to `hi` (uniform)
+                const int lo = MODE == RN_ANY ? (V - H % V) * ESZ : 0, hi = MODE == RN_ANY ? 16 : H * ESZ;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    if constexpr (DT == DTF_BF16) q[k] = pack_bf16x2(v[c * V + 2 * k], v[c * V + 2 * k + 1]);
-                    else q[k] = __float_as_uint(v[c * V + k]);
+                    if (4 * k >= lo && 4 * k + 4 <= hi) *reinterpret_cast<rn_any1*>(t + 4 * k) = q[k];
+                    else if (4 * k >= lo && 4 * k < hi) *reinterpret_cast<unsigned short*>(t + 4 * k) = (unsigned short)q[k];
+                    else if (4 * k + 2 == lo) *reinterpret_cast<unsigned short*>(t + 4 * k + 2) = (unsigned short)(q[k] >> 16);
                 }
-                if (at < H) *reinterpret_cast<u32x4*>(p + (unsigned)(at * (16 / V))) = q;
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < NE; ++e)
-                if (e * TPR + l < H) store1<DT>(p + (unsigned)((e * TPR + l) * (16 / V)), 0, v[e]);
         }
     }
     // a parameter row of type wdt (the activations' type or fp32)
@@ -104,7 +140,7 @@ struct RnRow {
         if (wdt == DT) load(p, 0, H, l, v);
         else {
 #pragma unroll
-            for (int e = 0; e < NE; ++e) v[e] = col(l, e) < H ? reinterpret_cast<const float*>(p)[col(l, e)] : 0.f;
+            for (int e = 0; e < NE; ++e) v[e] = has(l, e, H) ? reinterpret_cast<const float*>(p)[col(l, e, H)] : 0.f;
         }
     }
 };
@@ -159,7 +195,7 @@ __device__ __forceinline__ void rn_normalise(float (&v)[NE], int H, int l, float
         rn_sum<TPR, false>(s, z, red, flip);
         mean = s * inv;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) v[e] = R::col(l, e) < H ? v[e] - mean : 0.f;
+        for (int e = 0; e < NE; ++e) v[e] = R::has(l, e, H) ? v[e] - mean : 0.f;
     }
     s = z = 0.f;
 #pragma unroll
@@ -170,9 +206,9 @@ __device__ __forceinline__ void rn_normalise(float (&v)[NE], int H, int l, float
     for (int e = 0; e < NE; ++e) v[e] *= rstd;
 }
 
-template <int DT, bool VEC, int TPR, int NE>
+template <int DT, int MODE, int TPR, int NE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(RnArgs a) {
-    typedef RnRow<DT, VEC, TPR, NE> R;
+    typedef RnRow<DT, MODE, TPR, NE> R;
     constexpr int RB = TPR < 256 ? 256 / TPR : 1;
     __shared__ float red[2][2][16];
     const int l = threadIdx.x % TPR, H = a.H;
@@ -227,9 +263,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(RnArgs a)
 // A workgroup walks its rows with the next row's loads in flight and the parameters in registers (read again per row, they
 // cost a cache's latency between the two reductions).  SAME: parameters of the activations' type; else (fp32 parameters of
 // bf16 activations) they are read per row.
-template <int DT, bool VEC, int TPR, int NE, bool LAYER, bool SAME>
+template <int DT, int MODE, int TPR, int NE, bool LAYER, bool SAME>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a) {
-    typedef RnRow<DT, VEC, TPR, NE> R;
+    typedef RnRow<DT, MODE, TPR, NE> R;
     constexpr int NT = TPR < 256 ? 256 : TPR, RB = NT / TPR;
     __shared__ float red[2][2][16];
     __shared__ float comb[RB > 1 ? NT * NE : 1];
@@ -272,17 +308,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
     };
     const int64_t first = r0 + (int64_t)bx * RB, stride = (int64_t)a.nbx * RB;
     if (first < r1) fetch(row_at(first));
+    if constexpr (SAME) {
+        R::trim(wr, H, l);
+        if (a.pw) R::trim(pwr, H, l);
+        if (LAYER && a.pb) R::trim(pbr, H, l);
+    }
     for (int64_t base = first; base < r1; base += stride) {    // (uniform in the workgroup)
         const bool valid = base + slot < r1;
         const int64_t row = row_at(base);
         const float live = valid ? 1.f : 0.f;
         const float mu = mean, rs = rstd, pmu = pmean, prs = prstd;
         float v[NE], n[NE], dr[NE], dy[NE], g[NE], p[NE];
-        R::expand(xr, v);
-        if (a.h) R::expand(hr, n);
-        if (a.gate) R::expand(gr, g);
-        if (a.dy) R::expand(dyr, dy);
-        if (a.dr) R::expand(drr, dr);
+        R::row(xr, H, l, v);
+        if (a.h) R::row(hr, H, l, n);
+        if (a.gate) R::row(gr, H, l, g);
+        if (a.dy) R::row(dyr, H, l, dy);
+        if (a.dr) R::row(drr, H, l, dr);
         else {
 #pragma unroll
             for (int e = 0; e < NE; ++e) dr[e] = 0.f;
@@ -313,7 +354,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
         if (a.h) {
             if (a.pw) {
 #pragma unroll
-                for (int e = 0; e < NE; ++e) n[e] = R::col(l, e) < H ? (n[e] - pmu) * prs : 0.f;
+                for (int e = 0; e < NE; ++e) n[e] = R::has(l, e, H) ? (n[e] - pmu) * prs : 0.f;
             }
             float t[NE];
             normed(t);
@@ -325,7 +366,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
             for (int e = 0; e < NE; ++e) v[e] = fmaf(a.scale, t[e], v[e]);
         }
 #pragma unroll
-        for (int e = 0; e < NE; ++e) v[e] = R::col(l, e) < H ? (v[e] - mu) * rs : 0.f;        // rhat
+        for (int e = 0; e < NE; ++e) v[e] = R::has(l, e, H) ? (v[e] - mu) * rs : 0.f;        // rhat
         if (a.dy) {
             float c1 = 0.f, c2 = 0.f;
             pre_w();
@@ -366,7 +407,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
             post_w();
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
-                if (R::col(l, e) >= H) dr[e] = 0.f;
+                if (!R::has(l, e, H)) dr[e] = 0.f;
                 spw[e] = fmaf(live * dr[e], n[e], spw[e]);
                 if constexpr (LAYER) spb[e] = fmaf(live, dr[e], spb[e]);
                 dr[e] *= p[e];
@@ -394,13 +435,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(RnArgs a)
                     float z = 0.f;
 #pragma unroll
                     for (int k = 0; k < RB; ++k) z += comb[(k * NE + e) * TPR + l];
-                    if (R::col(l, e) < H) put(R::col(l, e), z);
+                    if (R::has(l, e, H)) put(R::col(l, e, H), z);
                 }
             }
         } else {
 #pragma unroll
             for (int e = 0; e < NE; ++e)
-                if (R::col(l, e) < H) put(R::col(l, e), s[e]);
+                if (R::has(l, e, H)) put(R::col(l, e, H), s[e]);
         }
     };
     float* out = a.part + (int64_t)blockIdx.x * a.narr * H;
@@ -489,11 +530,11 @@ int64_t dtf_residual_norm_ws(int64_t M, int H, int64_t groups, int narr) {
     if (H <= 512) { X(DTY, VECT, 64, 8) } else if (H <= 1024) { X(DTY, VECT, 128, 8) }            \
     else if (H <= 2048) { X(DTY, VECT, 256, 8) } else if (H <= 4096) { X(DTY, VECT, 512, 8) }     \
     else if (H <= 8192) { X(DTY, VECT, 512, 16) } else { X(DTY, VECT, 1024, 16) }
-#define RN_DISPATCH(SHAPES, X)                                                \
-    if (dt == DTF_BF16) {                                                     \
-        if (vec) { SHAPES(X, DTF_BF16, true) } else { SHAPES(X, DTF_BF16, false) } \
-    } else {                                                                  \
-        if (vec) { SHAPES(X, DTF_F32, true) } else { SHAPES(X, DTF_F32, false) }   \
+#define RN_BY_TYPE(SHAPES, X, MODE)                                                              \
+    if (dt == DTF_BF16) {                                                                        \
+        if (H < 8) { X(DTF_BF16, RN_TINY, 64, 8) } else { SHAPES(X, DTF_BF16, MODE) }            \
+    } else {                                                                                     \
+        if (H < 4) { X(DTF_F32, RN_TINY, 64, 8) } else { SHAPES(X, DTF_F32, MODE) }              \
     }
 
 static int rn_check(int dt, int wdt, int64_t M, int H, int64_t rpg) {
@@ -521,7 +562,8 @@ int dtf_residual_norm_fwd(const void* x, const void* h, const void* gate, const 
     if (grid > 0x7fffffff) return -92;
 #define RN_FWD(DTY, VECT, TPR, NE) \
     hipLaunchKernelGGL((rn_fwd_kernel<DTY, VECT, TPR, NE>), dim3((unsigned)grid), dim3(nt), 0, stream, a);
-    RN_DISPATCH(RN_SHAPES_FWD, RN_FWD)
+    // (16384 rows of 2048: 45 us, 50 as rows that begin anywhere; the backward takes the same time either way)
+    if (vec) { RN_BY_TYPE(RN_SHAPES_FWD, RN_FWD, RN_ALIGNED) } else { RN_BY_TYPE(RN_SHAPES_FWD, RN_FWD, RN_ANY) }
 #undef RN_FWD
     DTF_CHECK_LAUNCH();
     return 0;
@@ -560,9 +602,6 @@ int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const 
     a.s_pb = sum(dpb, wdt, layer && pw, 1);
     a.s_g = sum(dgate, dt, shared && a.nbx > 1, groups);
     a.narr = s.n;
-    const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)pw | (uintptr_t)pb |
-                         (uintptr_t)dy | (uintptr_t)dr | (uintptr_t)dx | (uintptr_t)dh | (shared ? 0 : (uintptr_t)dgate);
-    const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
     const int tpr = rn_tpr(H, 8), nt = tpr < 256 ? 256 : tpr;
 #define RN_BWD_L(DTY, VECT, TPR, NE, SM)                                                                                         \
     if (layer) hipLaunchKernelGGL((rn_bwd_kernel<DTY, VECT, TPR, NE, true, SM>), dim3((unsigned)grid), dim3(nt), 0, stream, a);  \
@@ -573,7 +612,7 @@ int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const 
     for (; a.group0 < groups; a.group0 += gstep) {
         const int64_t grid = (groups - a.group0 < gstep ? groups - a.group0 : gstep) * a.nbx;
         a.add = a.group0 > 0;
-        RN_DISPATCH(RN_SHAPES_BWD, RN_BWD)
+        RN_BY_TYPE(RN_SHAPES_BWD, RN_BWD, RN_ANY)
         DTF_CHECK_LAUNCH();
     }
 #undef RN_BWD

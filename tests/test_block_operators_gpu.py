@@ -229,6 +229,12 @@ NORM = [
     ((700, 128), "rms", True, "channel", 0.5, BF, BF), ((6, 3, 5, 256), "rms", True, "sequence", 0.5, BF, BF),
     ((1500, 2, 64), "layer", False, "sequence", 1.0, BF, BF), ((2, 17, 5000), "rms", False, "channel", 1.0, BF, F32),
     ((600, 3, 4096), "rms", True, "sequence", 0.5, BF, BF),              # more gate rows than workgroups (as 1500 x 64 above)
+    # rows that end inside a vector, and rows shorter than one
+    ((3, 41, 2047), "rms", True, "sequence", 0.5, BF, BF), ((2, 30, 4094), "layer", True, "full", 1.0, BF, BF),
+    ((1, 9, 513), "layer", False, "channel", 1.0, BF, F32), ((2, 8, 1022), "rms", True, "full", 0.5, BF, F32),
+    ((2, 20, 2051), "layer", True, "sequence", 1.0, F32, F32), ((2, 33, 9), "layer", True, "none", 1.0, BF, BF),
+    ((4, 7, 7), "layer", True, "channel", 1.0, BF, BF), ((2, 70, 5), "rms", True, "sequence", 1.0, BF, F32),
+    ((3, 5, 3), "layer", True, "full", 1.0, F32, F32), ((2, 40, 2), "rms", False, "full", 1.0, BF, BF), ((2, 9, 6001), "rms", True, "full", 1.0, BF, BF),
 ]
 
 

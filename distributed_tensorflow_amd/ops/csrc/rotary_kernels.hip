@@ -7,7 +7,8 @@
 // fraction left in 32 bits), its sine and cosine in fp32.  A workgroup owns TB tokens: each of its threads computes one
 // (token, pair)'s sine and cosine into LDS, then all heads of q and k of those tokens stream through it -- q and k are
 // read and written once, no table of angles exists in memory.
-// HBM-bound: 16384 tokens, 40 heads of 128, bf16: 335 MB in 62 us (5.4 TB/s), fp32 at half the tokens 60 us (5.6).
+// HBM-bound: 16384 tokens, 40 heads of 128, bf16: 335 MB in 63 us (5.3 TB/s), fp32 at half the tokens 57 us (5.9); 74 of the
+// 128 turned 72 us (vectors that begin inside a dword).
 #include "dtf_common.h"
 #include <type_traits>
 
@@ -68,12 +69,15 @@ __device__ __forceinline__ typename RoVec<V, DT == DTF_BF16 ? 2 : 4>::type ro_pa
     return r;
 }
 
-// A unit is V pairs (two vectors of V elements) or, past 2m, 2V elements that pass through.
+// A unit is V pairs (two vectors of V elements) or, past 2m, two vectors that pass through.  A last unit that would pass the
+// end of its range lies over the one before it (both write the same values); less than a vector past 2m is stored by words.
+// Vectors begin anywhere: the hardware takes them unaligned.
 template <int DT, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(RoArgs a) {
     constexpr int ESZ = DT == DTF_BF16 ? 2 : 4;
-    typedef typename RoVec<V, ESZ>::type vec;
+    typedef typename RoVec<V, ESZ>::type vec __attribute__((aligned(ESZ)));
     typedef typename std::conditional<DT == DTF_BF16, unsigned short, unsigned int>::type elem;
+    typedef unsigned int word __attribute__((aligned(2)));
     __shared__ __attribute__((aligned(16))) float cs[RO_PAIRS], sn[RO_PAIRS];
     const int tid = threadIdx.x, m = a.m;
     const int64_t t0 = (int64_t)blockIdx.x * a.tb;
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RoArgs a) {
         sn[p] = sv * a.amp * a.sign;
     }
     __syncthreads();
-    const int rot = m / V, U = rot + (a.D - 2 * m) / (2 * V), H = a.Hq + a.Hk, total = nt * H * U;
+    const int rest = a.D - 2 * m, rot = (m + V - 1) / V, U = rot + (rest + 2 * V - 1) / (2 * V), H = a.Hq + a.Hk, total = nt * H * U;
     for (int i0 = tid; i0 < total; i0 += 256 * RO_UNROLL) {
         vec x[RO_UNROLL], y[RO_UNROLL];
         elem* dst[RO_UNROLL];
@@ -108,9 +112,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RoArgs a) {
                                    : (const elem*)a.k + b * a.k_bs + s * a.k_ss + (h - a.Hq) * a.k_hs;
             dst[n] = is_q ? (elem*)a.qo + (t * a.Hq + h) * a.D : (elem*)a.ko + (t * a.Hk + (h - a.Hq)) * a.D;
             const bool turn = u < rot;
-            const int first = turn ? (INTER ? 2 * u * V : u * V) : 2 * m + (u - rot) * 2 * V;
-            dist[n] = turn && !INTER ? m : V;
-            pr[n] = turn ? tt * m + u * V : -1;
+            const int j = min(u * V, m - V);                              // a turning unit's first pair
+            const int first = turn ? (INTER ? 2 * j : j) : 2 * m + min((u - rot) * 2 * V, rest < V ? rest - V : max(0, rest - 2 * V));
+            dist[n] = turn ? (INTER ? V : m) : max(0, min(V, rest - V));
+            pr[n] = turn ? tt * m + j : -1;
             dst[n] += first;
             x[n] = *reinterpret_cast<const vec*>(src + first);
             y[n] = *reinterpret_cast<const vec*>(src + first + dist[n]);
@@ -150,6 +155,13 @@ __global__ __launch_bounds__(256) void rotary_kernel(RoArgs a) {
                 }
                 x[n] = ro_pack<DT, V>(p);
                 y[n] = ro_pack<DT, V>(q);
+            } else if (rest < V) {
+                if constexpr (V * ESZ > 4) {                              // (V > 2: rest is even)
+#pragma unroll
+                    for (int k = 0; k < V * ESZ / 4; ++k)
+                        if (k * 4 >= (V - rest) * ESZ) reinterpret_cast<word*>(dst[n])[k] = x[n][k];
+                }
+                continue;
             }
             *reinterpret_cast<vec*>(dst[n]) = x[n];
             *reinterpret_cast<vec*>(dst[n] + dist[n]) = y[n];
@@ -169,20 +181,12 @@ int dtf_rotary(const void* q, const void* k, void* qo, void* ko, int dt, const i
     if (dt != DTF_F32 && dt != DTF_BF16) return -81;
     RoArgs a{q, k, qo, ko, st[0], st[1], st[2], st[3], st[4], st[5], pos, p_bs, p_ss, offset, (int64_t)B * S,
              inv_freq, S, Hq, Hk, D, m, 1, pos64, amp, sign};
-    // elements a load: 16 B where the pairs, the rest of the head, the strides and the addresses allow, else the largest half
-    // (8192 tokens, 40 heads, 76 of 128 turned: 4-B loads 57 us, single elements 86)
-    const int esz = dt == DTF_BF16 ? 2 : 4;
-    const uintptr_t al = (uintptr_t)q | (uintptr_t)k | (uintptr_t)qo | (uintptr_t)ko;
-    int V = 16 / esz;
-    auto fits = [&]() {
-        if ((al & (V * esz - 1)) || m % V || (D - 2 * m) % (2 * V)) return false;
-        for (int i = 0; i < (Hk ? 6 : 3); ++i)
-            if (st[i] % V) return false;
-        return true;
-    };
-    while (V > 1 && !fits()) V >>= 1;
+    // elements a load: 16 B, or the largest half that fits the pairs (16384 tokens, 40 heads, 76 of 128 turned, bf16: 66 us; by
+    // 8 B 85, by 4 B 130)
+    int V = dt == DTF_BF16 ? 8 : 4;
+    while (m < V) V >>= 1;
     // tokens of a workgroup: about RO_UNROLL units a thread (34440 tokens with 2 heads of 96, fp32: 32 us, 42 with one unit each)
-    const int64_t units = (int64_t)(Hq + Hk) * (D / 2 / V);
+    const int64_t units = (int64_t)(Hq + Hk) * ((m + V - 1) / V + (D - 2 * m + 2 * V - 1) / (2 * V));
     if (units > 0x40000000) return -82;
     int tb = (int)(256 * RO_UNROLL / units);
     if (tb > RO_PAIRS / m) tb = RO_PAIRS / m;

@@ -171,6 +171,9 @@ ROT = [
     (1, 1, 1, 1, 2, 1, F32), (8, 1, 32, 8, 128, 64, BF), (2, 37, 12, 12, 64, 32, BF), (3, 50, 4, 2, 96, 32, F32),
     (2, 33, 3, 1, 128, 7, BF), (1, 129, 2, 2, 80, 40, BF), (1, 65, 2, 1, 64, 8, BF), (2, 17, 5, 5, 10, 3, F32), (1, 300, 40, 8, 128, 64, BF),
     (1, 70, 2, 1, 256, 128, F32), (2, 19, 2, 2, 2048, 1024, BF), (1, 21, 4, 4, 128, 38, BF),
+    # pairs and rests that are no whole vectors: the last one over the one before, a rest of less than a vector
+    (2, 23, 4, 2, 128, 37, BF), (1, 40, 3, 1, 128, 63, BF), (2, 9, 2, 2, 96, 45, BF), (1, 31, 2, 1, 64, 29, F32), (2, 13, 2, 1, 26, 9, BF),
+    (1, 17, 3, 2, 20, 9, F32), (1, 25, 2, 1, 6, 2, BF), (1, 26, 2, 1, 4, 1, BF), (1, 27, 1, 1, 8, 3, F32), (3, 7, 2, 1, 22, 8, BF),
 ]
 
 

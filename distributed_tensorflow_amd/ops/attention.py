@@ -121,30 +121,35 @@ def _general_kernels():
 
 
 def _operand(t):
-    """As it is where the kernels can address it (dense head dimension, 16-B aligned rows, tokens less than 2^25 elements
-    apart), else a contiguous copy."""
-    st = t.stride()
-    if st[3] == 1 and (st[1] < 1 << 25 or t.shape[1] == 1) and t.data_ptr() % 16 == 0:
-        if all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], st)):
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """-> (t, its batch, token and head stride, 0 where there is one): as it is where the kernels can address it (dense head
+    dimension, 16-B aligned rows, tokens less than 2^25 elements apart), else a contiguous copy."""
+    B, S, H, D = t.shape
+    b, s, h, d = t.stride()
+    if B == 1:
+        b = 0
+    if S == 1:
+        s = 0
+    if H == 1:
+        h = 0
+    if d == 1 and s < 1 << 25 and not (b | s | h) & 7 and not t.data_ptr() & 15:
+        return t, b, s, h
+    return t.clone(memory_format=torch.contiguous_format), S * H * D, H * D, D
 
 
-def _general_strides(*tensors):
-    return (ctypes.c_int64 * (3 * len(tensors)))(*(0 if n == 1 else s for t in tensors for n, s in zip(t.shape[:3], t.stride())))
+_Strides = ctypes.c_int64 * 9
 
 
 def _general_forward(q, k, v, kv_len, causal, scale):
     """-> (q, k, v as the kernels read them, out, log-sum-exp, the launch's remaining arguments)."""
-    q, k, v = _operand(q), _operand(k), _operand(v)
+    (q, *sq), (k, *sk), (v, *sv) = _operand(q), _operand(k), _operand(v)
     B, Sq, Hq, D = q.shape
-    Sk, Hk = k.shape[1], k.shape[2]
-    o = q.new_empty(q.shape)
+    _, Sk, Hk, _ = k.shape
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, Hq, Sq), dtype=torch.float32)
     fwd, _, ws_floats, _ = _general_kernels()
     n = ws_floats(B, Sq, Sk, Hq, Hk, D)
     ws = lse.new_empty(n) if n else None
-    how = _general_strides(q, k, v), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
+    how = _Strides(*sq, *sk, *sv), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
     rc = hip.launch(q, fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), hip.ptr(ws), *how)
     hip.check(rc, "dtf_attn_general_fwd")
     return q, k, v, o, lse, how
@@ -164,7 +169,8 @@ class _Attention(torch.autograd.Function):
         st, B, Sq, Sk, Hq, Hk, D, causal, scale, _ = ctx.how
         if not do.is_contiguous() or do.data_ptr() % 16:
             do = do.clone(memory_format=torch.contiguous_format)
-        dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
+        dq, dk = torch.empty_like(o), torch.empty_like(k, memory_format=torch.contiguous_format)
+        dv = torch.empty_like(dk)
         _, bwd, _, ws_floats = _general_kernels()
         ws = lse.new_empty(ws_floats(B, Sq, Sk, Hq, Hk, D, causal))
         rc = hip.launch(q, bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
@@ -175,29 +181,30 @@ class _Attention(torch.autograd.Function):
 
 
 def _check_general(q, k, v, kv_len, scale):
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError("attention: %s is [B, S, heads, D], got %s" % (n, tuple(t.shape)))
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("attention: q, k and v must share dtype and device")
-        if not t.is_floating_point():
-            raise TypeError("attention: q, k and v are floating-point tensors, got %s" % t.dtype)
-    B, Sq, Hq, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise ValueError("attention: q %s, k %s and v %s do not fit together" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if min(q.shape) < 1 or min(k.shape) < 1:
-        raise ValueError("attention: no dimension may be empty, got q %s and k %s" % (tuple(q.shape), tuple(k.shape)))
-    if Hq % k.shape[2]:
-        raise ValueError("attention: %d query heads do not divide over %d key heads" % (Hq, k.shape[2]))
+    shape, keys, dtype, device = q.shape, k.shape, q.dtype, q.device
+    if not len(shape) == len(keys) == v.dim() == 4:
+        raise ValueError("attention: q, k and v are [B, S, heads, D], got %s, %s and %s" % (tuple(shape), tuple(keys), tuple(v.shape)))
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
+        raise ValueError("attention: q, k and v must share dtype and device")
+    if not dtype.is_floating_point:
+        raise TypeError("attention: q, k and v are floating-point tensors, got %s" % dtype)
+    B, Sq, Hq, D = shape
+    Bk, Sk, Hk, Dk = keys
+    if keys != v.shape or Bk != B or Dk != D:
+        raise ValueError("attention: q %s, k %s and v %s do not fit together" % (tuple(shape), tuple(keys), tuple(v.shape)))
+    if 0 in shape or 0 in keys:
+        raise ValueError("attention: no dimension may be empty, got q %s and k %s" % (tuple(shape), tuple(keys)))
+    if Hq % Hk:
+        raise ValueError("attention: %d query heads do not divide over %d key heads" % (Hq, Hk))
     if D % 8 or D > 128:
         raise ValueError("attention: the head dimension must be a multiple of 8 up to 128, got %d" % D)
     if Hq * D >= 1 << 25:
         raise ValueError("attention: %d heads of %d are too many" % (Hq, D))
-    if max(Sq, k.shape[1]) >= 1 << 30:
+    if Sq >= 1 << 30 or Sk >= 1 << 30:
         raise ValueError("attention: sequences are shorter than 2**30 tokens")
-    if not (scale > 0 and math.isfinite(scale)):
+    if not 0 < scale < math.inf:
         raise ValueError("attention: scale must be positive and finite, got %r" % (scale,))
-    if kv_len is not None and (tuple(kv_len.shape) != (B,) or kv_len.is_floating_point() or kv_len.dtype == torch.bool):
+    if kv_len is not None and (kv_len.shape != (B,) or kv_len.is_floating_point() or kv_len.dtype == torch.bool):
         raise ValueError("attention: kv_len holds one integer for each of the %d sequences" % B)
 
 

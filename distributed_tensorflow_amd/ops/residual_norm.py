@@ -48,6 +48,8 @@ def residual_norm_reference(x, h, weight, bias=None, *, gate=None, scale=1.0, po
 
 def _rows_per_gate(x, gate):
     """Rows of x that share a row of the gate: the gate's leading dimensions are x's up to some axis and 1 from there on."""
+    if gate.shape == x.shape:
+        return 1
     shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
     if len(shape) == x.dim() and shape[-1] == x.shape[-1]:
         lead = tuple(x.shape[:-1])
@@ -71,23 +73,25 @@ def _checked_eps(eps):
 def _checked(x, h, weight, bias, gate, post_weight, post_bias, kind):
     if kind not in ("rms", "layer"):
         raise ValueError("residual_norm: kind is 'rms' or 'layer', got %r" % (kind,))
+    shape, dtype, device = x.shape, x.dtype, x.device
     hip.dt(x)
-    if x.dim() < 1 or x.numel() == 0 or x.shape[-1] > MAX_WIDTH:
-        raise ValueError("residual_norm: x is [..., H] with 1 <= H <= %d and at least one row, got %s" % (MAX_WIDTH, tuple(x.shape)))
-    if h is not None and (h.shape != x.shape or h.dtype != x.dtype or h.device != x.device):
+    if not shape or 0 in shape or shape[-1] > MAX_WIDTH:
+        raise ValueError("residual_norm: x is [..., H] with 1 <= H <= %d and at least one row, got %s" % (MAX_WIDTH, tuple(shape)))
+    if h is not None and (h.shape != shape or h.dtype != dtype or h.device != device):
         raise ValueError("residual_norm: h must match x in shape, dtype and device")
-    if gate is not None and (gate.dtype != x.dtype or gate.device != x.device):
+    if gate is not None and (gate.dtype != dtype or gate.device != device):
         raise ValueError("residual_norm: the gate must match x in dtype and device")
     if post_bias is not None and post_weight is None:
         raise ValueError("residual_norm: post_bias without post_weight")
     if kind == "rms" and (bias is not None or post_bias is not None):
         raise ValueError("residual_norm: an RMS norm has no bias")
+    width, wdt = shape[-1:], weight.dtype
     for p in (weight, bias, post_weight, post_bias):
         if p is None:
             continue
-        if tuple(p.shape) != (x.shape[-1],) or p.device != x.device:
-            raise ValueError("residual_norm: parameters are [%d] on x's device, got %s" % (x.shape[-1], tuple(p.shape)))
-        if p.dtype not in (x.dtype, torch.float32) or p.dtype != weight.dtype:
+        if p.shape != width or p.device != device:
+            raise ValueError("residual_norm: parameters are [%d] on x's device, got %s" % (shape[-1], tuple(p.shape)))
+        if p.dtype != wdt or (wdt != dtype and wdt != torch.float32):
             raise ValueError("residual_norm: parameters share one dtype, x's or float32")
     return None if gate is None else _rows_per_gate(x, gate)
 
@@ -97,15 +101,16 @@ def _dense(t):
 
 
 def _like(t):
-    return None if t is None else t.new_empty(t.shape)
+    return None if t is None else torch.empty_like(t)
 
 
 def _forward(x, h, weight, bias, gate, post_weight, post_bias, rpg, scale, layer, eps):
     """-> (y, r, the operands as the kernels read them and the statistics, the launch's sizes)."""
-    x, h, weight, bias, gate, post_weight, post_bias = map(_dense, (x, h, weight, bias, gate, post_weight, post_bias))
+    x, h, weight, bias, gate, post_weight, post_bias = [
+        t if t is None or t.is_contiguous() else t.contiguous() for t in (x, h, weight, bias, gate, post_weight, post_bias)]
     H = x.shape[-1]
     M = x.numel() // H
-    y, r = x.new_empty(x.shape), _like(h)
+    y, r = torch.empty_like(x), _like(h)
     stats = x.new_empty(4 * M, dtype=torch.float32)
     how = hip.dt(x), hip.dt(weight), layer, M, H, rpg, scale
     rc = hip.launch(x, _kernels()[0], x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(bias),
@@ -130,7 +135,7 @@ class _ResidualNorm(torch.autograd.Function):
         x, h, weight, bias, gate, post_weight, post_bias, stats = ctx.saved_tensors
         _, _, _, M, H, rpg, scale = how = ctx.how
         dy, dr = _dense(dy), _dense(dr)
-        dx = x.new_empty(x.shape)
+        dx = torch.empty_like(x)
         same = post_weight is None and gate is None and scale == 1.0      # then dh = dx, written once
         dh = None if same else _like(h)
         dw, db, dgate, dpw, dpb = _like(weight), _like(bias), _like(gate), _like(post_weight), _like(post_bias)

@@ -60,28 +60,30 @@ def rotary_frequencies(dim, base=10000.0, scaling="none", factor=1.0, original_l
 
 
 def _checked(q, k, inv_freq, positions):
-    both = (q,) if k is None else (q, k)
-    for t in both:
-        if t.dim() != 4:
-            raise ValueError("rotary: q and k are [B, S, heads, D], got %s" % (tuple(t.shape),))
-        if t.dtype != q.dtype or t.device != q.device:
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if len(shape) != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("rotary: q and k are [B, S, heads, D], got %s" % ", ".join(str(tuple(t.shape)) for t in (q, k) if t is not None))
+    hip.dt(q)
+    B, S, _, D = shape
+    if k is not None:
+        if k.dtype != dtype or k.device != device:
             raise ValueError("rotary: q and k must share dtype and device")
-        hip.dt(t)
-    B, S, _, D = q.shape
-    if k is not None and (k.shape[0], k.shape[1], k.shape[3]) != (B, S, D):
-        raise ValueError("rotary: q %s and k %s differ in more than their heads" % (tuple(q.shape), tuple(k.shape)))
+        Bk, Sk, _, Dk = k.shape
+        if Bk != B or Sk != S or Dk != D:
+            raise ValueError("rotary: q %s and k %s differ in more than their heads" % (tuple(shape), tuple(k.shape)))
     if D % 2:
         raise ValueError("rotary: the head dimension must be even, got %d" % D)
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous() or inv_freq.device != q.device:
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous() or inv_freq.device != device:
         raise ValueError("rotary: inv_freq is a contiguous float64 vector on the operands' device (rotary_frequencies)")
     if inv_freq.requires_grad:
         raise ValueError("rotary: inv_freq gets no gradient (pass inv_freq.detach())")
-    if not 0 < 2 * inv_freq.numel() <= D or inv_freq.numel() > 1024:
-        raise ValueError("rotary: %d pairs do not fit a head of %d" % (inv_freq.numel(), D))
+    m = inv_freq.numel()
+    if not 0 < 2 * m <= D or m > 1024:
+        raise ValueError("rotary: %d pairs do not fit a head of %d" % (m, D))
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+        if positions.dtype not in (torch.int64, torch.int32) or positions.device != device:
             raise ValueError("rotary: positions are int32 / int64 on the operands' device")
-        if tuple(positions.shape) not in ((S,), (B, S), (1, S)):
+        if positions.shape not in ((B, S), (S,), (1, S)):
             raise ValueError("rotary: positions are [S] or [B, S], got %s for B=%d S=%d" % (tuple(positions.shape), B, S))
 
 
@@ -102,27 +104,33 @@ def rotary_reference(q, k, inv_freq, positions=None, *, interleaved=False, ampli
     return tuple(None if t is None else _turn(t.float(), cos, sin, interleaved).to(t.dtype) for t in (q, k))
 
 
-def _dense_heads(t):
-    return t if t is None or t.stride(3) == 1 else t.contiguous()
+_Strides = ctypes.c_int64 * 6
 
 
-def _strides(t):
-    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
+def _operand(t):
+    """-> (t with a dense head dimension, its batch, token and head stride)."""
+    if t.stride(3) != 1:
+        t = t.contiguous()
+    return t, t.stride()[:3]
 
 
 def _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, sign):
-    q, k = _dense_heads(q), _dense_heads(k)
+    q, sq = _operand(q)
     B, S, Hq, D = q.shape
-    qo = q.new_empty(q.shape)
-    ko = None if k is None else k.new_empty(k.shape)
-    st = (ctypes.c_int64 * 6)(*_strides(q), *((0, 0, 0) if k is None else _strides(k)))
-    p_bs = p_ss = 0
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is None:
+        k_at, ko, ko_at, Hk, sk = None, None, None, 0, (0, 0, 0)
+    else:
+        k, sk = _operand(k)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_at, ko_at, Hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
+    p_at, p_64, p_bs, p_ss = None, 0, 0, 0
     if positions is not None:
-        p_ss = positions.stride(-1)
-        p_bs = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    rc = hip.launch(q, _kernel(), q.data_ptr(), hip.ptr(k), qo.data_ptr(), hip.ptr(ko), hip.dt(q), st, hip.ptr(positions),
-                    int(positions is not None and positions.dtype == torch.int64), p_bs, p_ss, offset, inv_freq.data_ptr(), B, S,
-                    Hq, 0 if k is None else k.shape[2], D, inv_freq.numel(), interleaved, amplitude, sign)
+        p_at, p_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+        *p_bs, p_ss = positions.stride()
+        p_bs = p_bs[0] if p_bs and positions.shape[0] > 1 else 0
+    rc = hip.launch(q, _kernel(), q.data_ptr(), k_at, qo.data_ptr(), ko_at, hip.dt(q), _Strides(*sq, *sk), p_at, p_64, p_bs, p_ss,
+                    offset, inv_freq.data_ptr(), B, S, Hq, Hk, D, inv_freq.numel(), interleaved, amplitude, sign)
     hip.check(rc, "dtf_rotary")
     return qo, ko
 

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 import os
 
 import torch
@@ -112,12 +113,14 @@ _general = None
 def _general_kernels():
     global _general
     if _general is None:
-        P, I, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
-        L = ctypes.c_int64
-        _general = (hip.declare("dtf_attn_general_fwd", [P] * 7 + [I] * 7 + [Fl, P, P]),
-                    hip.declare("dtf_attn_general_bwd", [P] * 11 + [I] * 7 + [Fl, P, P]),
-                    hip.declare("dtf_attn_general_fwd_ws", [I] * 6, L), hip.declare("dtf_attn_general_bwd_ws", [I] * 7, L))
+        C, P, L = ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int64
+        _general = (hip.declare("dtf_attn_general_fwd", [C, C, P]), hip.declare("dtf_attn_general_bwd", [C, C, P]),
+                    hip.declare("dtf_attn_general_fwd_ws", [C], L), hip.declare("dtf_attn_general_bwd_ws", [C], L))
     return _general
+
+
+_call = struct.Struct("<9qQ7if").pack              # AgCall of csrc/attn_general_kernels.hip
+_fwd_tensors, _bwd_tensors = struct.Struct("<6Q").pack, struct.Struct("<10Q").pack
 
 
 def _operand(t):
@@ -136,46 +139,53 @@ def _operand(t):
     return t.clone(memory_format=torch.contiguous_format), S * H * D, H * D, D
 
 
-_Strides = ctypes.c_int64 * 9
+def _dense(t):
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _general_forward(q, k, v, kv_len, causal, scale):
-    """-> (q, k, v as the kernels read them, out, log-sum-exp, the launch's remaining arguments)."""
+def _general_operands(q, k, v, kv_len, causal, scale):
+    """-> (q, k, v as the kernels read them, what the call is about)."""
     (q, *sq), (k, *sk), (v, *sv) = _operand(q), _operand(k), _operand(v)
     B, Sq, Hq, D = q.shape
     _, Sk, Hk, _ = k.shape
+    return q, k, v, _call(*sq, *sk, *sv, hip.ptr(kv_len), B, Sq, Sk, Hq, Hk, D, causal, scale)
+
+
+def _general_forward(q, k, v, kv_len, causal, scale):
+    """-> (q, k, v as the kernels read them, out, log-sum-exp)."""
+    q, k, v, how = _general_operands(q, k, v, kv_len, causal, scale)
+    B, Sq, Hq, _ = q.shape
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, Hq, Sq), dtype=torch.float32)
     fwd, _, ws_floats, _ = _general_kernels()
-    n = ws_floats(B, Sq, Sk, Hq, Hk, D)
+    n = ws_floats(how)
     ws = lse.new_empty(n) if n else None
-    how = _Strides(*sq, *sk, *sv), B, Sq, Sk, Hq, Hk, D, causal, scale, hip.ptr(kv_len)
-    rc = hip.launch(q, fwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), hip.ptr(ws), *how)
+    rc = hip.launch(q, fwd, _fwd_tensors(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), hip.ptr(ws)), how)
     hip.check(rc, "dtf_attn_general_fwd")
-    return q, k, v, o, lse, how
+    return q, k, v, o, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_len, causal, scale):
-        q, k, v, o, lse, ctx.how = _general_forward(q, k, v, kv_len, causal, scale)
+        q, k, v, o, lse = _general_forward(q, k, v, kv_len, causal, scale)
         ctx.save_for_backward(q, k, v, o, lse, kv_len)
+        ctx.how = causal, scale
         return o
 
     @staticmethod
     @hip.first_order
     def backward(ctx, do):
-        q, k, v, o, lse, kv_len = ctx.saved_tensors
-        st, B, Sq, Sk, Hq, Hk, D, causal, scale, _ = ctx.how
-        if not do.is_contiguous() or do.data_ptr() % 16:
-            do = do.clone(memory_format=torch.contiguous_format)
+        q, k, v, o, lse, kv_len = ctx.saved_tensors       # (hooks on saved tensors may bring them back in another layout)
+        kv_len = None if kv_len is None else kv_len.contiguous()
+        q, k, v, how = _general_operands(q, k, v, kv_len, *ctx.how)
+        o, lse, do = _dense(o), _dense(lse), _dense(do)
         dq, dk = torch.empty_like(o), torch.empty_like(k, memory_format=torch.contiguous_format)
         dv = torch.empty_like(dk)
         _, bwd, _, ws_floats = _general_kernels()
-        ws = lse.new_empty(ws_floats(B, Sq, Sk, Hq, Hk, D, causal))
-        rc = hip.launch(q, bwd, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), st, B, Sq, Sk, Hq, Hk, D, causal, scale,
-                        hip.ptr(kv_len))
+        ws = lse.new_empty(ws_floats(how))
+        rc = hip.launch(q, bwd, _bwd_tensors(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr()), how)
         hip.check(rc, "dtf_attn_general_bwd")
         return dq, dk, dv, None, None, None
 

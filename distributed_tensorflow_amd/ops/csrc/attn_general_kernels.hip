@@ -727,37 +727,58 @@ static int ag_dq_splits(int B, int Sq, int Sk, int Hq) {
     return ag_splits((int64_t)B * Hq * ((Sq - 1) / 128 + 1), (Sk + 63) / 64, 4, 512);
 }
 
-// fp32 workspace of the forward (0: none) and of the backward (D per query and head, then the parts), in floats
-int64_t dtf_attn_general_fwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D) {
-    const int64_t n = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
-    return n > 1 ? n * B * Sq * Hq * (D + 2) : 0;
-}
+// What a call is about, packed by its caller (one pointer is cheaper to hand over than twenty arguments): the element strides
+// (batch, token, head) of q, k, v; keys of each sequence or null; sizes.
+struct AgCall {
+    int64_t st[9];
+    const int* kv_len;
+    int B, Sq, Sk, Hq, Hk, D, causal;
+    float scale;
+};
+static_assert(sizeof(AgCall) == 112, "packed by the caller");
 
-int64_t dtf_attn_general_bwd_ws(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
-    const int64_t n = ag_dkv_splits(B, Sq, Sk, Hq, Hk, D, causal), nq = ag_dq_splits(B, Sq, Sk, Hq);
-    const int64_t kv = n > 1 ? n * 2 * B * Sk * Hk * D : 0, q = nq > 1 ? nq * B * Sq * Hq * D : 0;
-    return ag_dsum_floats(B, Sq, Hq) + (kv > q ? kv : q);              // (dQ's parts are added before dK's are written)
-}
-
-// st: the nine element strides (batch, token, head) of q, k, v; ws: dtf_attn_general_fwd_ws floats
-int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, float* lse, float* ws, const int64_t* st, int B,
-                         int Sq, int Sk, int Hq, int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
-    DTF_CLEAR_ERRORS();
+static AgArgs ag_args(const AgCall& c) {
     AgArgs a{};
-    a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.out = (u16*)o; a.lse = lse; a.ws = ws;
-    a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
-    a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
-    a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
-    a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
-    int rc = ag_check(a, st, 9), grid = 0;
+    a.q_bs = c.st[0]; a.q_ss = c.st[1]; a.q_hs = c.st[2]; a.k_bs = c.st[3]; a.k_ss = c.st[4]; a.k_hs = c.st[5];
+    a.v_bs = c.st[6]; a.v_ss = c.st[7]; a.v_hs = c.st[8];
+    a.kv_len = c.kv_len; a.B = c.B; a.Sq = c.Sq; a.Sk = c.Sk; a.Hq = c.Hq; a.Hk = c.Hk; a.D = c.D; a.causal = c.causal;
+    a.group = c.Hk > 0 ? c.Hq / c.Hk : 0;
+    a.scale = c.scale; a.scale_log2e = c.scale * 1.4426950408889634f;
+    return a;
+}
+
+static bool ag_aligned(void* const* p, int n, int skip) {
+    uintptr_t all = 0;
+    for (int i = 0; i < n; ++i) all |= i == skip ? 0 : (uintptr_t)p[i];
+    return !(all & 15);
+}
+
+// fp32 workspace of the forward (0: none) and of the backward (D per query and head, then the parts), in floats
+int64_t dtf_attn_general_fwd_ws(const AgCall* c) {
+    const int64_t n = ag_fwd_splits(c->B, c->Sq, c->Sk, c->Hq, c->Hk);
+    return n > 1 ? n * c->B * c->Sq * c->Hq * (c->D + 2) : 0;
+}
+
+int64_t dtf_attn_general_bwd_ws(const AgCall* c) {
+    const int64_t n = ag_dkv_splits(c->B, c->Sq, c->Sk, c->Hq, c->Hk, c->D, c->causal), nq = ag_dq_splits(c->B, c->Sq, c->Sk, c->Hq);
+    const int64_t kv = n > 1 ? n * 2 * c->B * c->Sk * c->Hk * c->D : 0, q = nq > 1 ? nq * c->B * c->Sq * c->Hq * c->D : 0;
+    return ag_dsum_floats(c->B, c->Sq, c->Hq) + (kv > q ? kv : q);     // (dQ's parts are added before dK's are written)
+}
+
+// p: q, k, v, o, lse (fp32), ws (dtf_attn_general_fwd_ws floats, or null)
+int dtf_attn_general_fwd(void* const* p, const AgCall* c, hipStream_t stream) {
+    DTF_CLEAR_ERRORS();
+    AgArgs a = ag_args(*c);
+    a.q = (const u16*)p[0]; a.k = (const u16*)p[1]; a.v = (const u16*)p[2]; a.out = (u16*)p[3]; a.lse = (float*)p[4]; a.ws = (float*)p[5];
+    const int B = c->B, Sq = c->Sq, Sk = c->Sk, Hq = c->Hq, Hk = c->Hk, D = c->D;
+    int rc = ag_check(a, c->st, 9), grid = 0;
     if (rc) return rc;
-    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)ws)) & 15) return -16;
-    a.group = Hq / Hk;
+    if (!ag_aligned(p, 6, 4)) return -16;
     const bool pack = ag_pack_rows(Sq, a.group);
     const int64_t rows = pack ? (int64_t)a.group * Sq : Sq;
     a.ntiles = (int)((rows + 127) / 128);
     a.nsplit = ag_fwd_splits(B, Sq, Sk, Hq, Hk);
-    if (a.nsplit > 1 && !ws) return -73;
+    if (a.nsplit > 1 && !a.ws) return -73;
     if ((rc = ag_grid((int64_t)B * (pack ? Hk : Hq) * a.ntiles * a.nsplit, &grid))) return rc;
 #define AG_FWD(DP, DC)                                                                                     \
     if (pack) hipLaunchKernelGGL((ag_fwd_kernel<DP, DC, true>), dim3(grid), dim3(256), 0, stream, a);      \
@@ -776,24 +797,20 @@ int dtf_attn_general_fwd(const void* q, const void* k, const void* v, void* o, f
     return 0;
 }
 
-// o, do_: contiguous [B, Sq, Hq, D]; dq like o, dk / dv contiguous [B, Sk, Hk, D]; ws: dtf_attn_general_bwd_ws floats
-int dtf_attn_general_bwd(const void* q, const void* k, const void* v, const void* o, const void* do_, const float* lse,
-                         void* dq, void* dk, void* dv, float* ws, const int64_t* st, int B, int Sq, int Sk, int Hq,
-                         int Hk, int D, int causal, float scale, const int* kv_len, hipStream_t stream) {
+// p: q, k, v, o, dO, lse, dq, dk, dv, ws (dtf_attn_general_bwd_ws floats); o, dO, dq contiguous [B, Sq, Hq, D], dk, dv
+// contiguous [B, Sk, Hk, D]
+int dtf_attn_general_bwd(void* const* p, const AgCall* c, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
-    AgArgs a{};
-    a.q = (const u16*)q; a.k = (const u16*)k; a.v = (const u16*)v; a.o = (const u16*)o; a.dO = (const u16*)do_;
-    a.lse = const_cast<float*>(lse); a.dsum = ws; a.dq = (u16*)dq; a.dk = (u16*)dk; a.dv = (u16*)dv;
-    a.ws = ws + ag_dsum_floats(B, Sq, Hq);
-    a.q_bs = st[0]; a.q_ss = st[1]; a.q_hs = st[2]; a.k_bs = st[3]; a.k_ss = st[4]; a.k_hs = st[5];
-    a.v_bs = st[6]; a.v_ss = st[7]; a.v_hs = st[8];
-    a.kv_len = kv_len; a.B = B; a.Sq = Sq; a.Sk = Sk; a.Hq = Hq; a.Hk = Hk; a.D = D; a.causal = causal;
-    a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f;
-    int rc = ag_check(a, st, 9), grid = 0;
+    AgArgs a = ag_args(*c);
+    const int B = c->B, Sq = c->Sq, Sk = c->Sk, Hq = c->Hq, Hk = c->Hk, D = c->D, causal = c->causal;
+    const float scale = c->scale;
+    float* ws = (float*)p[9];
+    a.q = (const u16*)p[0]; a.k = (const u16*)p[1]; a.v = (const u16*)p[2]; a.o = (const u16*)p[3]; a.dO = (const u16*)p[4];
+    a.lse = (float*)p[5]; a.dq = (u16*)p[6]; a.dk = (u16*)p[7]; a.dv = (u16*)p[8]; a.dsum = ws;
+    int rc = ag_check(a, c->st, 9), grid = 0;
     if (rc) return rc;
-    if ((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)o) | ((uintptr_t)do_) | ((uintptr_t)dq) |
-         ((uintptr_t)dk) | ((uintptr_t)dv) | ((uintptr_t)ws)) & 15) return -16;
-    a.group = Hq / Hk;
+    if (!ag_aligned(p, 10, 5)) return -16;
+    a.ws = ws + ag_dsum_floats(B, Sq, Hq);
     const int splits = ag_dkv_splits(B, Sq, Sk, Hq, Hk, D, causal);
     if (!ws) return -73;
     if ((int64_t)((Sq + 31) / 32) * a.group > 0x7fffffff) return -72;

@@ -514,12 +514,21 @@ static void rn_grid(int64_t M, int H, int64_t groups, int* nbx, int64_t* gstep) 
 
 extern "C" {
 
+// What a call is about, packed by its caller (one pointer is cheaper to hand over than twenty arguments).  Rows [M, H]
+// contiguous; gate [M / rpg, H] or null; w, b, pw, pb of type wdt (dt or fp32).
+struct RnCall {
+    int64_t M, rpg;
+    int dt, wdt, layer, H;
+    float scale, eps;
+};
+static_assert(sizeof(RnCall) == 40, "packed by the caller");
+
 // fp32 workspace of the backward, in floats: groups = rows of a shared gate (1 without), narr = number of sums
-int64_t dtf_residual_norm_ws(int64_t M, int H, int64_t groups, int narr) {
+int64_t dtf_residual_norm_ws(const RnCall* c, int64_t groups, int narr) {
     int nbx;
     int64_t gstep;
-    rn_grid(M, H, groups, &nbx, &gstep);
-    return gstep * nbx * narr * H;
+    rn_grid(c->M, c->H, groups, &nbx, &gstep);
+    return gstep * nbx * narr * c->H;
 }
 
 #define RN_SHAPES_FWD(X, DTY, VECT)                                                               \
@@ -544,18 +553,18 @@ static int rn_check(int dt, int wdt, int64_t M, int H, int64_t rpg) {
     return 0;
 }
 
-// rows [M, H] contiguous; gate [M / rpg, H] or null; w, b, pw, pb of type wdt (dt or fp32)
-int dtf_residual_norm_fwd(const void* x, const void* h, const void* gate, const void* w, const void* b, const void* pw,
-                          const void* pb, void* y, void* r, float* stats, int dt, int wdt, int layer, int64_t M, int H,
-                          int64_t rpg, float scale, float eps, hipStream_t stream) {
+// p: x, h, gate, w, b, pw, pb, y, r, stats (fp32 [4, M]); h and r, gate, b, pw, pb may be null
+int dtf_residual_norm_fwd(void* const* p, const RnCall* c, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
-    int rc = rn_check(dt, wdt, M, H, rpg);
+    const int dt = c->dt, H = c->H;
+    const int64_t M = c->M;
+    int rc = rn_check(dt, c->wdt, M, H, c->rpg);
     if (rc) return rc;
     RnArgs a{};
-    a.x = x; a.h = h; a.gate = gate; a.w = w; a.b = b; a.pw = pw; a.pb = pb; a.y = y; a.r = r; a.stats = stats;
-    a.M = M; a.rpg = rpg; a.H = H; a.wdt = wdt; a.layer = layer; a.scale = scale; a.eps = eps;
-    const uintptr_t al = (uintptr_t)x | (uintptr_t)h | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)b | (uintptr_t)pw |
-                         (uintptr_t)pb | (uintptr_t)y | (uintptr_t)r;
+    a.x = p[0]; a.h = p[1]; a.gate = p[2]; a.w = p[3]; a.b = p[4]; a.pw = p[5]; a.pb = p[6]; a.y = p[7]; a.r = p[8]; a.stats = (float*)p[9];
+    a.M = M; a.rpg = c->rpg; a.H = H; a.wdt = c->wdt; a.layer = c->layer; a.scale = c->scale; a.eps = c->eps;
+    uintptr_t al = 0;
+    for (int i = 0; i < 9; ++i) al |= (uintptr_t)p[i];
     const bool vec = !(al & 15) && H % (dt == DTF_BF16 ? 8 : 4) == 0;
     const int tpr = rn_tpr(H, 16), nt = tpr < 256 ? 256 : tpr, rb = nt / tpr;
     const int64_t grid = (M + rb - 1) / rb;
@@ -569,20 +578,22 @@ int dtf_residual_norm_fwd(const void* x, const void* h, const void* gate, const 
     return 0;
 }
 
-// dgate [M, H] for a gate per element, else [M / rpg, H] through the partials; dw, db, dpw, dpb of type wdt; any of them
-// null where there is no such operand.  ws: dtf_residual_norm_ws(M, H, groups, narr) floats, groups = M / rpg for a shared
-// gate and 1 otherwise, narr = number of sums (dw, db, dpw, dpb, dgate of a shared gate) or more.
-int dtf_residual_norm_bwd(const void* x, const void* h, const void* gate, const void* w, const void* pw, const void* pb,
-                          const float* stats, const void* dy, const void* dr, void* dx, void* dh, void* dgate, void* dw,
-                          void* db, void* dpw, void* dpb, float* ws, int dt, int wdt, int layer, int64_t M, int H, int64_t rpg,
-                          float scale, hipStream_t stream) {
+// p: x, h, gate, w, pw, pb, stats, dy, dr, dx, dh, dgate, dw, db, dpw, dpb, ws.  dgate [M, H] for a gate per element, else
+// [M / rpg, H] through the partials; dw, db, dpw, dpb of type wdt; any of them null where there is no such operand.  ws:
+// dtf_residual_norm_ws(c, groups, narr) floats, groups = M / rpg for a shared gate and 1 otherwise, narr = number of sums (dw,
+// db, dpw, dpb, dgate of a shared gate) or more.
+int dtf_residual_norm_bwd(void* const* p, const RnCall* c, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
+    const int dt = c->dt, wdt = c->wdt, layer = c->layer, H = c->H;
+    const int64_t M = c->M, rpg = c->rpg;
     int rc = rn_check(dt, wdt, M, H, rpg);
     if (rc) return rc;
+    void *h = p[1], *gate = p[2], *pw = p[4], *dgate = p[11], *dw = p[12], *db = p[13], *dpw = p[14], *dpb = p[15];
+    float* ws = (float*)p[16];
     if (gate && (!dgate || !h)) return -93;
     RnArgs a{};
-    a.x = x; a.h = h; a.gate = gate; a.w = w; a.pw = pw; a.pb = pb; a.stats = const_cast<float*>(stats); a.dy = dy; a.dr = dr;
-    a.dx = dx; a.dh = dh; a.part = ws; a.M = M; a.rpg = rpg; a.H = H; a.wdt = wdt; a.layer = layer; a.scale = scale;
+    a.x = p[0]; a.h = h; a.gate = gate; a.w = p[3]; a.pw = pw; a.pb = p[5]; a.stats = (float*)p[6]; a.dy = p[7]; a.dr = p[8];
+    a.dx = p[9]; a.dh = p[10]; a.part = ws; a.M = M; a.rpg = rpg; a.H = H; a.wdt = wdt; a.layer = layer; a.scale = c->scale;
     const bool shared = gate && rpg > 1;
     a.dgate = dgate;
     const int64_t groups = shared ? (M + rpg - 1) / rpg : 1;

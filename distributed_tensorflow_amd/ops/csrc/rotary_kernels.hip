@@ -171,16 +171,28 @@ __global__ __launch_bounds__(256) void rotary_kernel(RoArgs a) {
 
 extern "C" {
 
-// st: element strides (batch, token, head) of q, then of k.  pos: null, or int32 / int64 (pos64) with strides p_bs, p_ss.
-// k may be null (Hk = 0).  sign: +1 forward, -1 backward.
-int dtf_rotary(const void* q, const void* k, void* qo, void* ko, int dt, const int64_t* st, const void* pos, int pos64,
-               int64_t p_bs, int64_t p_ss, int64_t offset, const double* inv_freq, int B, int S, int Hq, int Hk, int D, int m,
-               int interleaved, float amp, float sign, hipStream_t stream) {
+// A call, packed by its caller (one pointer is cheaper to hand over than twenty arguments).  k and ko may be null (Hk = 0).
+// pos: null, or int32 / int64 (pos64) with strides p_bs, p_ss.  st: element strides (batch, token, head) of q, then of k.
+// sign: +1 forward, -1 backward.
+struct RoCall {
+    const void *q, *k;
+    void *qo, *ko;
+    const void* pos;
+    const double* inv_freq;
+    int64_t st[6], p_bs, p_ss, offset;
+    int dt, pos64, B, S, Hq, Hk, D, m, interleaved;
+    float amp, sign;
+    int pad;
+};
+static_assert(sizeof(RoCall) == 168, "packed by the caller");
+
+int dtf_rotary(const RoCall* c, hipStream_t stream) {
     DTF_CLEAR_ERRORS();
+    const int dt = c->dt, B = c->B, S = c->S, Hq = c->Hq, Hk = c->Hk, D = c->D, m = c->m, interleaved = c->interleaved;
     if (B <= 0 || S <= 0 || Hq <= 0 || Hk < 0 || D <= 0 || m <= 0 || 2 * m > D || m > RO_PAIRS || (D & 1)) return -80;
     if (dt != DTF_F32 && dt != DTF_BF16) return -81;
-    RoArgs a{q, k, qo, ko, st[0], st[1], st[2], st[3], st[4], st[5], pos, p_bs, p_ss, offset, (int64_t)B * S,
-             inv_freq, S, Hq, Hk, D, m, 1, pos64, amp, sign};
+    RoArgs a{c->q, c->k, c->qo, c->ko, c->st[0], c->st[1], c->st[2], c->st[3], c->st[4], c->st[5], c->pos, c->p_bs, c->p_ss,
+             c->offset, (int64_t)B * S, c->inv_freq, S, Hq, Hk, D, m, 1, c->pos64, c->amp, c->sign};
     // elements a load: 16 B, or the largest half that fits the pairs (16384 tokens, 40 heads, 76 of 128 turned, bf16: 66 us; by
     // 8 B 85, by 4 B 130)
     int V = dt == DTF_BF16 ? 8 : 4;

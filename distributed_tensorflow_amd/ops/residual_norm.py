@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 import torch.nn as nn
@@ -24,11 +25,14 @@ _fns = None
 def _kernels():
     global _fns
     if _fns is None:
-        P, I, L, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-        _fns = (hip.declare("dtf_residual_norm_fwd", [P] * 10 + [I, I, I, L, I, L, Fl, Fl, P]),
-                hip.declare("dtf_residual_norm_bwd", [P] * 17 + [I, I, I, L, I, L, Fl, P]),
-                hip.declare("dtf_residual_norm_ws", [L, I, L, I], L))
+        C, P, L = ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int64
+        _fns = (hip.declare("dtf_residual_norm_fwd", [C, C, P]), hip.declare("dtf_residual_norm_bwd", [C, C, P]),
+                hip.declare("dtf_residual_norm_ws", [C, L, ctypes.c_int], L))
     return _fns
+
+
+_call = struct.Struct("<2q4i2f").pack              # RnCall of csrc/residual_norm_kernels.hip
+_fwd_tensors, _bwd_tensors = struct.Struct("<10Q").pack, struct.Struct("<17Q").pack
 
 
 def _normed(v, weight, bias, kind, eps):
@@ -105,18 +109,19 @@ def _like(t):
 
 
 def _forward(x, h, weight, bias, gate, post_weight, post_bias, rpg, scale, layer, eps):
-    """-> (y, r, the operands as the kernels read them and the statistics, the launch's sizes)."""
+    """-> (y, r, the operands as the kernels read them and the statistics, what the call is about)."""
     x, h, weight, bias, gate, post_weight, post_bias = [
         t if t is None or t.is_contiguous() else t.contiguous() for t in (x, h, weight, bias, gate, post_weight, post_bias)]
     H = x.shape[-1]
     M = x.numel() // H
     y, r = torch.empty_like(x), _like(h)
     stats = x.new_empty(4 * M, dtype=torch.float32)
-    how = hip.dt(x), hip.dt(weight), layer, M, H, rpg, scale
-    rc = hip.launch(x, _kernels()[0], x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(bias),
-                    hip.ptr(post_weight), hip.ptr(post_bias), y.data_ptr(), hip.ptr(r), stats.data_ptr(), *how, eps)
+    how = _call(M, rpg, hip.dt(x), hip.dt(weight), layer, H, scale, eps)
+    rc = hip.launch(x, _kernels()[0], _fwd_tensors(
+        x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(bias), hip.ptr(post_weight), hip.ptr(post_bias),
+        y.data_ptr(), hip.ptr(r), stats.data_ptr()), how)
     hip.check(rc, "dtf_residual_norm_fwd")
-    return y, r, (x, h, weight, bias, gate, post_weight, post_bias, stats), how
+    return y, r, (x, h, weight, bias, gate, post_weight, post_bias, stats), (how, M, rpg, scale)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -132,8 +137,8 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dy, dr):
         if dy is None and dr is None:
             return (None,) * 11
-        x, h, weight, bias, gate, post_weight, post_bias, stats = ctx.saved_tensors
-        _, _, _, M, H, rpg, scale = how = ctx.how
+        x, h, weight, bias, gate, post_weight, post_bias, stats = map(_dense, ctx.saved_tensors)
+        how, M, rpg, scale = ctx.how
         dy, dr = _dense(dy), _dense(dr)
         dx = torch.empty_like(x)
         same = post_weight is None and gate is None and scale == 1.0      # then dh = dx, written once
@@ -142,10 +147,11 @@ class _ResidualNorm(torch.autograd.Function):
         groups = M // rpg if gate is not None and rpg > 1 else 0          # rows of a gate that is shared
         narr = 1 + (bias is not None) + (post_weight is not None) + (post_bias is not None) + (groups > 0)
         _, bwd, ws_floats = _kernels()
-        ws = stats.new_empty(ws_floats(M, H, groups or 1, narr))
-        rc = hip.launch(x, bwd, x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(post_weight),
-                        hip.ptr(post_bias), stats.data_ptr(), hip.ptr(dy), hip.ptr(dr), dx.data_ptr(), hip.ptr(dh), hip.ptr(dgate),
-                        dw.data_ptr(), hip.ptr(db), hip.ptr(dpw), hip.ptr(dpb), ws.data_ptr(), *how)
+        ws = stats.new_empty(ws_floats(how, groups or 1, narr))
+        rc = hip.launch(x, bwd, _bwd_tensors(
+            x.data_ptr(), hip.ptr(h), hip.ptr(gate), weight.data_ptr(), hip.ptr(post_weight), hip.ptr(post_bias), stats.data_ptr(),
+            hip.ptr(dy), hip.ptr(dr), dx.data_ptr(), hip.ptr(dh), hip.ptr(dgate), dw.data_ptr(), hip.ptr(db), hip.ptr(dpw),
+            hip.ptr(dpb), ws.data_ptr()), how)
         hip.check(rc, "dtf_residual_norm_bwd")
         return dx, dx if same and h is not None else dh, dw, db, dgate, dpw, dpb, None, None, None, None
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 import operator
+import struct
 
 import torch
 
@@ -21,8 +22,7 @@ _fn = None
 def _kernel():
     global _fn
     if _fn is None:
-        P, I, L, Fl = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-        _fn = hip.declare("dtf_rotary", [P, P, P, P, I, P, P, I, L, L, L, P, I, I, I, I, I, I, I, Fl, Fl, P])
+        _fn = hip.declare("dtf_rotary", [ctypes.c_char_p, ctypes.c_void_p])
     return _fn
 
 
@@ -104,7 +104,7 @@ def rotary_reference(q, k, inv_freq, positions=None, *, interleaved=False, ampli
     return tuple(None if t is None else _turn(t.float(), cos, sin, interleaved).to(t.dtype) for t in (q, k))
 
 
-_Strides = ctypes.c_int64 * 6
+_call = struct.Struct("<6Q9q9i2f4x").pack          # RoCall of csrc/rotary_kernels.hip
 
 
 def _operand(t):
@@ -119,18 +119,18 @@ def _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, sign):
     B, S, Hq, D = q.shape
     qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     if k is None:
-        k_at, ko, ko_at, Hk, sk = None, None, None, 0, (0, 0, 0)
+        k_at, ko, ko_at, Hk, sk = 0, None, 0, 0, (0, 0, 0)
     else:
         k, sk = _operand(k)
         ko = torch.empty_like(k, memory_format=torch.contiguous_format)
         k_at, ko_at, Hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
-    p_at, p_64, p_bs, p_ss = None, 0, 0, 0
+    p_at = p_64 = p_bs = p_ss = 0
     if positions is not None:
         p_at, p_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
         *p_bs, p_ss = positions.stride()
         p_bs = p_bs[0] if p_bs and positions.shape[0] > 1 else 0
-    rc = hip.launch(q, _kernel(), q.data_ptr(), k_at, qo.data_ptr(), ko_at, hip.dt(q), _Strides(*sq, *sk), p_at, p_64, p_bs, p_ss,
-                    offset, inv_freq.data_ptr(), B, S, Hq, Hk, D, inv_freq.numel(), interleaved, amplitude, sign)
+    rc = hip.launch(q, _kernel(), _call(q.data_ptr(), k_at, qo.data_ptr(), ko_at, p_at, inv_freq.data_ptr(), *sq, *sk, p_bs, p_ss,
+                                        offset, hip.dt(q), p_64, B, S, Hq, Hk, D, inv_freq.numel(), interleaved, amplitude, sign))
     hip.check(rc, "dtf_rotary")
     return qo, ko
 
@@ -146,6 +146,7 @@ class _Rotary(torch.autograd.Function):
     @hip.first_order
     def backward(ctx, dq, dk):
         inv_freq, positions = ctx.saved_tensors
+        inv_freq = inv_freq.contiguous()                                  # (hooks on saved tensors may have changed that)
         # the transpose of a rotation is the rotation by the negative angle
         gq, gk = _launch(dq, dk, inv_freq, positions, *ctx.how, -1.0)
         return gq, gk, None, None, None, None, None

@@ -307,6 +307,41 @@ def test_residual_norm_unaligned_rows_equal_aligned_ones(dev):
 # ---------------------------------------------------------------------------------------------------------------------
 # how they are called: offsets past 32 bits, the same tensor twice, streams, graphs, refusals
 # ---------------------------------------------------------------------------------------------------------------------
+def test_saved_tensors_that_come_back_in_another_layout(dev):
+    """Hooks on saved tensors (moved to the host and back, or laid out anew) change addresses and strides under the backward."""
+    r = _randn(dev, 21)
+    q, k, v = r(2, 70, 8, 64).to(BF).split([4, 2, 2], 2)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    lens = torch.tensor([70, 31], dtype=torch.int32, device=dev)
+    f, _ = rotary_frequencies(64, device=dev)
+    x, h, w, pw = (t.to(BF).requires_grad_() for t in (r(2, 70, 256), r(2, 70, 256), 1 + 0.1 * r(256), 1 + 0.1 * r(256)))
+    gate = r(2, 1, 256).to(BF).requires_grad_()
+    every = leaves + [x, h, w, pw, gate]
+    pos = (3 + torch.arange(70, device=dev)).expand(2, 70)
+
+    def run():
+        a, b = rotary(leaves[0], leaves[1], f, pos)
+        o = attention(a, b, leaves[2], causal=True, kv_len=lens) + attention(*leaves, kv_len=lens)
+        y, s = residual_norm(x, h + o.flatten(2), w, gate=gate, post_weight=pw)
+        return y, s
+
+    dy, ds = r(2, 70, 256).to(BF), r(2, 70, 256).to(BF)
+    want = torch.autograd.grad(run(), every, (dy, ds))
+
+    def apart(t):                                         # every second element of a buffer, last dimension first
+        buf = t.new_zeros(tuple(reversed(t.shape)) + (2,))[..., 0].permute(*reversed(range(t.dim())))
+        return buf.copy_(t)
+
+    hooks = (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: apart(t.detach()), lambda t: t))
+    for hook in hooks:
+        with hook:
+            outs = run()
+        junk = [torch.full_like(t, 7) for t in every for _ in range(3)]                 # memory given back is in other hands
+        for a, b in zip(torch.autograd.grad(outs, every, (dy, ds)), want):
+            assert torch.equal(a, b)
+        del junk
+
+
 def test_attention_offsets_past_32_bits(dev):
     r = _randn(dev, 11)
     B, S, H, D = 2, 130, 2, 64

@@ -589,3 +589,28 @@ def test_bert_options_match_the_plain_fp32_model(dev, kw):
     worst.sort(reverse=True)
     assert worst[0][0] < 6e-2, worst[:5]
     assert sum(w for w, _ in worst) / len(worst) < 2.5e-2, worst[:5]
+
+
+def test_bert_options_in_a_captured_step_equal_the_eager_loop(dev):
+    """The training loop behind a job with these options, eager and with its step captured and replayed: the same parameters."""
+    import copy
+
+    from distributed_tensorflow_amd.models import get_model_module
+    from distributed_tensorflow_amd.parallel.ps_runtime import ShardedPS
+    from distributed_tensorflow_amd.train.trainer import train_loop
+
+    mod = get_model_module("bert_base")
+    torch.manual_seed(0)
+    opts = dict(layers=2, hidden=256, heads=4, intermediate=512, vocab=2000, seq_len=150, positions="rotary", kv_heads=2, norm="pre_rms")
+    m1 = mod.prepare(mod.build(**opts), dev).train()
+    m2 = copy.deepcopy(m1)
+    batch = mod.synthetic_batch(4, device=dev, seed=3, seq_len=150, vocab=2000)
+    out = []
+    for m, graph in ((m1, False), (m2, True)):
+        ps = ShardedPS(list(m.named_parameters()), None, mod.default_optimizer())
+        ps.set_lr(1e-3)
+        last, _, n = train_loop(m, mod, ps, batch, 9, log_every=0, graph=graph)
+        assert n == 9 and last == last
+        out.append((ps.master.clone(), last))
+        ps.remove_hooks()
+    assert out[0][1] == out[1][1] and torch.equal(out[0][0], out[1][0])

@@ -47,19 +47,36 @@ class _SplitQKV(torch.autograd.Function):
         return torch.stack([dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2)], dim=2)
 
 
-class RotaryPositions:
-    """The frequencies of ``positions=rotary``, made once per device (in 64 bits, so they are no buffer of the model, whose
-    buffers follow its dtype)."""
+class RotaryPositions(nn.Module):
+    """The frequencies of ``positions=rotary``, on every device that the model has been moved to.  They are in 64 bits and the
+    model's buffers follow its dtype, so they are no buffer: a table is made, once per device, where the model is built or moved
+    -- not by the call that first needs it, which may run under ``inference_mode`` (no training step could save the table) or
+    inside a graph capture (a copy from the host must not)."""
 
     def __init__(self, dim, base, scaling, factor, original_length):
+        super().__init__()
         self.spec = dict(dim=dim, base=base, scaling=scaling, factor=factor, original_length=original_length)
         _, self.amplitude = rotary_frequencies(**self.spec)               # checks the options where the model is built
-        self._on = {}
+        self._on, self._at = {}, torch.device("cpu")
+        self._table(self._at)
 
-    def __call__(self, q, k):
-        if q.device not in self._on:
-            self._on[q.device] = rotary_frequencies(**self.spec, device=q.device)[0]
-        return rotary(q, k, self._on[q.device], amplitude=self.amplitude)
+    def _table(self, device):
+        if device not in self._on:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("rotary positions: no frequencies on %s yet; move the model there before capturing its step" % device)
+            with torch.inference_mode(False):
+                self._on[device] = rotary_frequencies(**self.spec, device=device)[0]
+        return self._on[device]
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._at = fn(torch.empty(0, device=self._at)).device             # (what is moved has no tensor of its own to tell where)
+        if self._at.type != "meta":
+            self._table(self._at)
+        return self
+
+    def forward(self, q, k):
+        return rotary(q, k, self._table(q.device), amplitude=self.amplitude)
 
 
 def _general_attention(qkv, A, KV, kv_len, positions):

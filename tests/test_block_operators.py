@@ -279,3 +279,29 @@ def test_bert_option_refusals():
                dict(hidden=48, kv_heads=2), dict(hidden=1024, norm="pre_rms")):
         with pytest.raises(ValueError):
             bert.build(**{**BERT, **kw})
+
+
+def test_rotary_positions_belong_to_the_model_not_to_its_first_call(monkeypatch):
+    """A model evaluated under inference_mode first trains afterwards: its frequencies are made where it is built or moved, never
+    inside a call.  (Only the GPU's backward saves them, so what the operator is handed is looked at.)"""
+    bert, m, batch = _bert(positions="rotary")
+    seen = []
+    plain = bert.rotary
+
+    def spy(q, k, inv_freq, **kw):
+        seen.append(inv_freq)
+        return plain(q, k, inv_freq, **kw)
+
+    monkeypatch.setattr(bert, "rotary", spy)
+    with torch.inference_mode():
+        m(*batch[:4])
+    bert.loss_fn(m, batch).backward()
+    assert len(seen) == 4 and not any(f.is_inference() for f in seen) and all(f is seen[0] for f in seen)
+    assert seen[0].dtype == F64 and torch.equal(seen[0], rotary_frequencies(16)[0])
+    turn = m.layers[0].positions
+    before = set(m.state_dict())
+    m.to(torch.bfloat16)
+    assert turn._table(torch.device("cpu")) is seen[0] and seen[0].dtype == F64           # the model's dtype leaves them alone
+    assert set(m.state_dict()) == before and not any("positions" in n for n in before)
+    m.to("meta").to_empty(device="cpu")
+    assert torch.equal(turn._table(torch.device("cpu")), rotary_frequencies(16)[0])

@@ -614,3 +614,35 @@ def test_bert_options_in_a_captured_step_equal_the_eager_loop(dev):
         out.append((ps.master.clone(), last))
         ps.remove_hooks()
     assert out[0][1] == out[1][1] and torch.equal(out[0][0], out[1][0])
+
+
+def test_bert_with_rotary_positions_evaluated_first_then_trained(dev):
+    import copy
+
+    from distributed_tensorflow_amd.models import bert
+
+    torch.manual_seed(0)
+    m = bert.prepare(bert.build(layers=2, hidden=128, heads=2, intermediate=256, vocab=2000, seq_len=40, positions="rotary"), dev)
+    fresh = copy.deepcopy(m)
+    batch = bert.synthetic_batch(2, device=dev, seed=1, seq_len=40, vocab=2000)
+    with torch.inference_mode():
+        m.eval()(*batch[:4])
+    for model in (m, fresh):
+        bert.loss_fn(model.train(), batch).backward()
+    for (n, p), (_, q) in zip(m.named_parameters(), fresh.named_parameters()):
+        assert torch.equal(p.grad, q.grad), n
+    # the model's first call of all inside a capture: nothing is copied from the host there
+    first = bert.build(layers=1, hidden=128, heads=2, intermediate=256, vocab=2000, positions="rotary").to(dev).layers[0].positions
+    r = _randn(dev, 52)
+    q, k = r(2, 40, 2, 64).to(BF), r(2, 40, 2, 64).to(BF)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = first(q, k)
+    want = rotary(q, k, rotary_frequencies(64, device=dev)[0])
+    for _ in range(3):
+        for t in out:
+            t.fill_(7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])

@@ -169,7 +169,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_len, causal, scale):
         q, k, v, o, lse = _general_forward(q, k, v, kv_len, causal, scale)
-        ctx.save_for_backward(q, k, v, o, lse, kv_len)
+        ctx.save_for_backward(q, k, v, o, lse, hip.savable(kv_len))
         ctx.how = causal, scale
         return o
 

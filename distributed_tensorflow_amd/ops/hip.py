@@ -113,6 +113,11 @@ def recorded(*tensors):
     return False
 
 
+def savable(t):
+    """A constant of a recorded call as the backward can keep it: autograd refuses tensors that ``inference_mode`` made."""
+    return t.clone() if t is not None and t.is_inference() else t
+
+
 def first_order(backward):
     """A custom backward that is no graph itself: differentiating its result again raises (``once_differentiable``, whose
     bookkeeping is skipped in the usual case that no second graph is being recorded)."""

@@ -138,7 +138,7 @@ def _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, sign):
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, inv_freq, positions, interleaved, amplitude, offset):
-        ctx.save_for_backward(inv_freq, positions)
+        ctx.save_for_backward(hip.savable(inv_freq), hip.savable(positions))
         ctx.how = interleaved, amplitude, offset
         return _launch(q, k, inv_freq, positions, interleaved, amplitude, offset, 1.0)
 

@@ -305,3 +305,13 @@ def test_rotary_positions_belong_to_the_model_not_to_its_first_call(monkeypatch)
     assert set(m.state_dict()) == before and not any("positions" in n for n in before)
     m.to("meta").to_empty(device="cpu")
     assert torch.equal(turn._table(torch.device("cpu")), rotary_frequencies(16)[0])
+
+
+def test_constants_of_a_recorded_call_can_be_saved():
+    from distributed_tensorflow_amd.ops import hip
+
+    with torch.inference_mode():
+        a = torch.arange(3)
+    b = torch.arange(3)
+    assert hip.savable(b) is b and hip.savable(None) is None
+    assert not hip.savable(a).is_inference() and torch.equal(hip.savable(a), b)

@@ -616,6 +616,23 @@ def test_bert_options_in_a_captured_step_equal_the_eager_loop(dev):
     assert out[0][1] == out[1][1] and torch.equal(out[0][0], out[1][0])
 
 
+def test_constants_made_under_inference_mode_train(dev):
+    """Frequencies, positions and lengths that inference_mode made: a recorded call keeps copies of its own."""
+    r = _randn(dev, 51)
+    q, k, v, do = (r(2, 40, 2, 64).to(BF) for _ in range(4))
+    with torch.inference_mode():
+        f, _ = rotary_frequencies(64, device=dev)
+        pos, lens = torch.arange(5, 45, device=dev), torch.tensor([40, 13], dtype=torch.int32, device=dev)
+    res = []
+    for how in ((f, pos, lens), (f.clone(), pos.clone(), lens.clone())):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        a, b = rotary(leaves[0], leaves[1], how[0], how[1])
+        out = attention(a, b, leaves[2], kv_len=how[2])
+        res.append((out.detach(),) + torch.autograd.grad(out, leaves, do))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+
+
 def test_bert_with_rotary_positions_evaluated_first_then_trained(dev):
     import copy
 

@@ -9,6 +9,8 @@ Every ``csrc/*.hip`` translation unit is compiled with
 torch headers, so a unit compiles in seconds and the library does not depend on
 the torch ABI).  The ``.so`` is git-ignored but travels with ``gpurun``
 snapshots; nothing is JIT-compiled at job submit time.
+An object is compiled again where its source, a header or its command has
+changed (the command is recorded beside it).
 """
 from __future__ import annotations
 
@@ -42,6 +44,30 @@ def _newer(src, dst, extra=()):
     return any(os.path.getmtime(s) > t for s in (src,) + tuple(extra))
 
 
+def _record(made):
+    return made + ".cmd"
+
+
+def _command_differs(cmd, made):
+    """Whether ``made`` came from another command (other flags or another compiler) than ``cmd``, which its record tells."""
+    try:
+        with open(_record(made)) as f:
+            return f.read() != " ".join(cmd)
+    except OSError:
+        return True
+
+
+def _run(cmd, made, what, more=()):
+    if os.path.exists(_record(made)):
+        os.remove(_record(made))           # (a compiler that ends early may leave half a file behind)
+    r = subprocess.run(cmd + list(more), capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("%s:\n%s\n%s" % (what, r.stdout, r.stderr))
+    with open(_record(made), "w") as f:
+        f.write(" ".join(cmd))
+    return r
+
+
 def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
 
@@ -61,20 +87,16 @@ def build(force=False, verbose=True, save_temps=False, debug_bounds=False):
     jobs = []
     for src in sources():
         obj = os.path.join(OBJ, os.path.basename(src)[:-4] + ".o")
-        if force or _newer(src, obj, hdrs):
-            cmd = [HIPCC] + FLAGS + (["-DDTF_DEBUG_BOUNDS"] if debug_bounds else []) + \
-                EXTRA_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
-            if save_temps:
-                cmd += ["-save-temps=obj"]
-            jobs.append((src, cmd))
+        cmd = [HIPCC] + FLAGS + (["-DDTF_DEBUG_BOUNDS"] if debug_bounds else []) + \
+            EXTRA_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
+        if force or _newer(src, obj, hdrs) or _command_differs(cmd, obj):
+            jobs.append((src, obj, cmd))
 
     def run(job):
-        src, cmd = job
+        src, obj, cmd = job
         if verbose:
             print("[dtf build] hipcc", os.path.basename(src), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
+        r = _run(cmd, obj, "hipcc failed for " + src, ["-save-temps=obj"] if save_temps else [])
         if verbose and r.stderr.strip():
             print(r.stderr, file=sys.stderr)
 
@@ -82,11 +104,11 @@ def build(force=False, verbose=True, save_temps=False, debug_bounds=False):
         with ThreadPoolExecutor(max_workers=min(4, len(jobs))) as ex:
             list(ex.map(run, jobs))
     objs = [os.path.join(OBJ, os.path.basename(s)[:-4] + ".o") for s in sources()]
-    if jobs or not os.path.exists(LIB):
-        cmd = [HIPCC, "-shared", "-fPIC", "--offload-arch=" + ARCH, "-o", LIB] + objs
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+    cmd = [HIPCC, "-shared", "-fPIC", "--offload-arch=" + ARCH, "-o", LIB] + objs
+    # (the record lies beside the objects; an earlier call that ended between compiling and linking left newer objects)
+    linked = os.path.join(OBJ, os.path.basename(LIB))
+    if jobs or any(_newer(o, LIB) for o in objs) or _command_differs(cmd, linked):
+        _run(cmd, linked, "link failed")
         if verbose:
             print("[dtf build] linked", LIB, flush=True)
     return LIB

@@ -536,22 +536,17 @@ __global__ __launch_bounds__(256, 2) void ag_dkv_kernel(AgArgs a) {
     const int off = a.Sk - a.Sq;
     const int begin = a.causal ? max(0, t * BM - off) / BQ * BQ : 0;
 
-    // K rows in registers; V rows too for DP = 64, in LDS for DP = 128 (32 registers more would leave one wave a SIMD)
+    // K rows in registers; V rows too for DP = 64, in LDS for DP = 128 (32 registers more would leave one wave a SIMD).
+    // Padded keys: rows of no columns, so nothing is read and zeros take part
     const bool seen = j < klen;
+    const int width = seen ? a.D : 0;
     s16x8 kf[KS], vf[DP == 128 ? 1 : KS];
-    ag_frags<DC>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, a.D);
+    ag_frags<DC>(kf, a.k + b * a.k_bs + jc * a.k_ss + hk * a.k_hs, g, width);
     if constexpr (DP == 128) {
         AgTile<DP, DC, BM, 256> vt;
         vt.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ss, wave, lane);
         vt.load(Vimg, t * BM, klen, a.D, wave);
-    } else ag_frags<DC>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, a.D);
-    if (!seen) {                                       // padded keys: whatever they hold takes no part
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            kf[ks] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
-            if constexpr (DP == 64) vf[ks] = kf[ks];
-        }
-    }
+    } else ag_frags<DC>(vf, a.v + b * a.v_bs + jc * a.v_ss + hk * a.v_hs, g, width);
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {

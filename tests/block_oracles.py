@@ -150,3 +150,89 @@ def residual_norm(x, h, w, b=None, gate=None, scale=1.0, pw=None, pb=None, kind=
         own = up if k in ("dw", "db", "dpw", "dpb") else u
         tol[k] = (own * t.abs() if own > U32 else 0) * 1.01 + U32 * mag[k] + 1e-35
     return want, tol
+
+
+def attention_noise(q, k, v, do, causal=False, lens=None, few=256, tile=128):
+    """-> the norm that the error of out, dq, dk, dv may have where exactly the documented roundings are made: P, dS and the results
+    to bf16, D from the rounded out except in tiles of ``tile`` queries that see up to ``few`` keys (fp32 there).
+
+    A rounding is off by up to half a step, evenly spread: in the mean square U16^2 / 3 times the value's square just above a power of
+    two, and 3 / (8 ln 2) = 0.541 of that over mantissas as they occur (density 1 / (m ln 2) on 1 <= m < 2).  Roundings are
+    independent of each other, so the squares add up over the sums that they go through; fp32's part is a thousandth of them.
+    A tenth more than that norm is allowed: it is a sum over thousands of elements, and scatters by one or two parts in a hundred."""
+    W = U16 ** 2 / 3 * 3 / (8 * math.log(2))
+    q, k, v, do = q.double(), k.double(), v.double(), do.double()
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    G, c = Hq // Hk, D ** -0.5
+    val = {n: torch.zeros(s, dtype=torch.float64, device=q.device) for n, s in (("out", q.shape), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape))}
+    var = {n: torch.zeros_like(t) for n, t in val.items()}
+    i, j = torch.arange(Sq, device=q.device)[:, None], torch.arange(Sk, device=q.device)[None, :]
+    last = ((i // tile + 1) * tile).clamp_max(Sq) - 1
+    for b in range(B):
+        n = Sk if lens is None else max(0, min(Sk, int(lens[b])))
+        seen = (j < n) & (i >= 0)
+        sees = torch.full_like(last, n)
+        if causal:
+            seen = seen & (j <= i + Sk - Sq)
+            sees = torch.minimum(sees, last + 1 + Sk - Sq)
+        for h in range(Hq):
+            Q, K, V, g = q[b, :, h], k[b, :, h // G].clone(), v[b, :, h // G].clone(), do[b, :, h]
+            K[n:], V[n:] = 0, 0
+            s = (c * (Q @ K.T.contiguous())).masked_fill(~seen, -math.inf)
+            e = torch.exp(s - s.amax(1, keepdim=True).clamp_min(-1e300))
+            z = e.sum(1, keepdim=True)
+            P = e / torch.where(z == 0, torch.ones_like(z), z)
+            P2 = P ** 2
+            val["out"][b, :, h] = P @ V
+            var["out"][b, :, h] = W * (P2 @ V ** 2)
+            dP = g @ V.T.contiguous()
+            dS = P * (dP - (P * dP).sum(1, keepdim=True))
+            D2 = (g ** 2 * (var["out"][b, :, h] + W * val["out"][b, :, h] ** 2)).sum(1, keepdim=True)
+            D2 = torch.where(sees <= few, torch.zeros_like(D2), D2)
+            val["dq"][b, :, h] = c * dS @ K
+            var["dq"][b, :, h] = c * c * (W * dS ** 2 @ K ** 2 + D2 * (P @ K) ** 2)
+            val["dk"][b, :, h // G] += c * dS.T.contiguous() @ Q
+            var["dk"][b, :, h // G] += c * c * (W * dS ** 2 + P2 * D2).T.contiguous() @ Q ** 2
+            val["dv"][b, :, h // G] += P.T.contiguous() @ g
+            var["dv"][b, :, h // G] += W * P2.T.contiguous() @ g ** 2
+    return val, {n: 1.1 * math.sqrt((t + W * val[n] ** 2).sum().item()) for n, t in var.items()}
+
+
+def attention_rounded(q, k, v, do, causal=False, lens=None, few=256, tile=128, rounded_d=False, rounded_s=False, lost_key=None):
+    """The backward's and forward's arithmetic with exactly the documented roundings; ``rounded_d``, ``rounded_s``, ``lost_key`` plant a
+    mistake (D or the scores in bf16, one key left out of the sums)."""
+    def r(t):
+        return t.to(torch.bfloat16).double()
+
+    q, k, v, do = q.double(), k.double(), v.double(), do.double()
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    G, c = Hq // Hk, D ** -0.5
+    got = {n: torch.zeros(s, dtype=torch.float64) for n, s in (("out", q.shape), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape))}
+    i, j = torch.arange(Sq)[:, None], torch.arange(Sk)[None, :]
+    last = ((i // tile + 1) * tile).clamp_max(Sq) - 1
+    for b in range(B):
+        n = Sk if lens is None else max(0, min(Sk, int(lens[b])))
+        seen = (j < n) & (i >= 0) & (j != (-1 if lost_key is None else lost_key))
+        sees = torch.full_like(last, n)
+        if causal:
+            seen = seen & (j <= i + Sk - Sq)
+            sees = torch.minimum(sees, last + 1 + Sk - Sq)
+        for h in range(Hq):
+            Q, K, V, g = q[b, :, h], k[b, :, h // G], v[b, :, h // G], do[b, :, h]
+            s = c * (Q @ K.T)
+            s = (r(s) if rounded_s else s).masked_fill(~seen, -math.inf)
+            m = s.amax(1, keepdim=True).clamp_min(-1e300)
+            e = torch.exp(s - m)
+            z = e.sum(1, keepdim=True)
+            z = torch.where(z == 0, torch.ones_like(z), z)
+            O = r((r(e) @ V) / z)
+            P, dP = e / z, g @ V.T
+            d = torch.where(sees <= few, (P * dP).sum(1, keepdim=True), (g * O).sum(1, keepdim=True))
+            dS = r(P * (dP - (r(d) if rounded_d else d)))
+            got["out"][b, :, h] = O
+            got["dq"][b, :, h] = c * dS @ K
+            got["dk"][b, :, h // G] += c * dS.T @ Q
+            got["dv"][b, :, h // G] += r(P).T @ g
+    return {n: r(t) for n, t in got.items()}

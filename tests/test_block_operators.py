@@ -315,3 +315,34 @@ def test_constants_of_a_recorded_call_can_be_saved():
     b = torch.arange(3)
     assert hip.savable(b) is b and hip.savable(None) is None
     assert not hip.savable(a).is_inference() and torch.equal(hip.savable(a), b)
+
+
+NOISE = [(2, 16, 16, 4, 2, 64, True, None), (1, 64, 64, 2, 2, 128, True, None), (2, 129, 129, 2, 1, 64, True, (129, 70)),
+         (1, 31, 700, 4, 2, 128, True, None), (2, 60, 320, 2, 1, 64, False, (320, 111))]
+
+
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D,causal,lens", NOISE)
+def test_attention_noise_tells_the_documented_roundings_from_others(B, Sq, Sk, Hq, Hk, D, causal, lens):
+    """The norms that the kernels' errors are held to: the documented roundings stay under them; a D or scores in bf16, where such
+    roundings are not lost among the others, and a key left out do not."""
+    r = _g(Sq + Sk)
+    q, k, v, do = (t.to(BF) for t in (r(B, Sq, Hq, D), r(B, Sk, Hk, D), r(B, Sk, Hk, D), r(B, Sq, Hq, D)))
+    want, most = oracle.attention_noise(q, k, v, do, causal, lens)
+    plain, _ = oracle.attention(q, k, v, do, causal, lens)
+    for n in want:
+        torch.testing.assert_close(want[n], plain[n], rtol=1e-12, atol=1e-12)
+
+    def over(**kw):
+        got = oracle.attention_rounded(q, k, v, do, causal, lens, **kw)
+        return {n: (got[n] - want[n]).norm().item() / most[n] for n in want}
+
+    right = over()
+    assert max(right.values()) < 1, right
+    lost = over(lost_key=Sk // 3)
+    assert min(lost.values()) > 3, lost
+    if Sk <= 64:                                       # few keys: dS is a difference of like terms
+        d = over(rounded_d=True)
+        assert min(d["dq"], d["dk"]) > 1, d
+    if Sk > 128:
+        scores = over(rounded_s=True)
+        assert min(scores.values()) > 1, scores

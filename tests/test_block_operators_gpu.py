@@ -72,6 +72,26 @@ def test_attention_matches_the_definition(dev, B, Sq, Sk, Hq, Hk, D, causal, len
         assert not grads[0].any() and not grads[1].any()               # one key: the probabilities are constant
 
 
+NOISE = [
+    (8, 16, 16, 4, 2, 64, True, None), (2, 37, 37, 12, 12, 64, False, (18, 37)), (2, 64, 64, 4, 4, 128, True, None), (2, 129, 129, 4, 1, 64, True, (129, 70)),
+    (1, 300, 300, 4, 2, 80, True, None), (1, 640, 640, 5, 1, 128, True, (513,)), (3, 1000, 1000, 12, 12, 64, False, (333, 666, 1000)),
+    (1, 2048, 2048, 8, 2, 128, True, None), (2, 257, 1500, 8, 2, 128, True, None), (4, 1, 1100, 32, 8, 128, False, (275, 550, 825, 1100)), (2, 200, 200, 6, 2, 32, True, None),
+]
+
+
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D,causal,lens", NOISE)
+def test_attention_rounds_only_where_it_says(dev, B, Sq, Sk, Hq, Hk, D, causal, lens):
+    """The norms of the errors: far sharper than the bounds of single elements, they would show D or scores held in bf16."""
+    q, k, v, do = _att_inputs(dev, B, Sq, Sk, Hq, Hk, D, True)
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*leaves, causal=causal, kv_len=n)
+    got = (out.detach(),) + torch.autograd.grad(out, leaves, do)
+    want, most = oracle.attention_noise(q, k, v, do, causal, lens)
+    over = {m: ((g.double() - want[m]).norm().item() / most[m]) for m, g in zip(("out", "dq", "dk", "dv"), got)}
+    assert max(over.values()) < 1, over
+
+
 @pytest.mark.parametrize("scale", [0.01, 1.0])
 def test_attention_scale_and_large_scores(dev, scale):
     q, k, v, do = _att_inputs(dev, 1, 150, 150, 2, 2, 64, False)

@@ -226,7 +226,9 @@ def attention(q, k, v, causal=False, kv_len=None, scale=None):
     key that only causality hides may reach queries before it, as in any product with a probability of 0.)
 
     Scores, softmax statistics and sums are fp32; probabilities and their gradients are rounded to bf16 for the second products.
-    Gradients are sums in a fixed order (no atomics) and do not depend on what else is in the batch."""
+    Sums run in a fixed order (no atomics): calls of the same shapes give the same bits, and a sequence's do not depend on what
+    the other sequences hold or how long they are.  They may depend on how many there are: long sums are split into as many parts
+    as it takes to fill the card with the whole call."""
     scale = 1.0 / math.sqrt(max(1, q.shape[-1])) if scale is None else hip.number(scale, "attention: scale")
     _check_general(q, k, v, kv_len, scale)
     if not q.is_cuda:

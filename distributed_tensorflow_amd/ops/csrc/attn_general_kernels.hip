@@ -681,7 +681,8 @@ static int ag_grid(int64_t n, int* out) {
     return 0;
 }
 
-// Workgroups that share a tile: enough for `fill` workgroups, no fewer than `least` steps each.  512 are resident.  257 queries
+// Workgroups that share a tile (by the whole call's size, so a sequence's sums are grouped by how many others there are, not by
+// what they hold): enough for `fill` workgroups, no fewer than `least` steps each.  512 are resident.  257 queries
 // on 7000 keys, 32 / 8 heads of 128, forward and join: fill 1 141 us, 512 84 + 12, 1024 85 + 19; one token on 8192 keys: fill 1
 // 147 us, 512 11 + 5.  dQ, 512 tokens, 12 heads of 64: fill 1 14 us, 512 11 + 2.
 static int ag_splits(int64_t grid, int64_t steps, int least, int fill) {

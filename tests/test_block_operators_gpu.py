@@ -173,6 +173,33 @@ def test_attention_of_a_query_does_not_depend_on_the_others(dev, Hk):
     assert torch.equal(attention(q[1:], k[1:], v[1:]), out[1:])
 
 
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D,causal", [(2, 1000, 1000, 12, 12, 64, False), (2, 257, 1500, 8, 2, 128, True), (3, 700, 700, 4, 1, 96, True)])
+def test_attention_of_a_sequence_does_not_depend_on_what_the_others_hold(dev, B, Sq, Sk, Hq, Hk, D, causal):
+    """Sums split over workgroups: one sequence's results have the same bits whatever the others hold and however long they are, in a
+    call of the same shapes.  (In a batch of another size the parts may be others, and the bits with them.)"""
+    from distributed_tensorflow_amd.ops import attention as A
+
+    q, k, v, do = _att_inputs(dev, B, Sq, Sk, Hq, Hk, D, False)
+
+    def parts(rows):
+        how = A._general_operands(*(t.expand(rows, -1, -1, -1) for t in (q[:1], k[:1], v[:1])), None, int(causal), 1.0)[3]
+        return A._general_kernels()[2](how)
+
+    assert parts(B) > 0 and parts(64) == 0
+    got = []
+    for other, n in ((1.0, Sk), (1.0, Sk), (-3.0, Sk // 3), (100.0, 0)):
+        t = [x.clone() for x in (q, k, v, do)]
+        for x in t:
+            x[1:] *= other
+        lens = torch.tensor([Sk - 9] + [n] * (B - 1), dtype=torch.int32, device=dev)
+        leaves = [x.requires_grad_() for x in t[:3]]
+        out = attention(*leaves, causal=causal, kv_len=lens)
+        got.append([x[0] for x in (out.detach(),) + torch.autograd.grad(out, leaves, t[3])])
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+
+
 def test_attention_nan_reaches_its_query(dev):
     q, k, v, _ = _att_inputs(dev, 1, 70, 70, 1, 1, 64, False)
     clean = attention(q, k, v, causal=True)

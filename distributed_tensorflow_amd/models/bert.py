@@ -13,8 +13,8 @@ as such in the checkpoint index).
 
 Job options beside the published model: ``positions=rotary`` (K23 on queries and keys instead of the learned table, so the
 sequence length has no bound; ``rotary_scaling``, ``rotary_factor``, ``rotary_original`` stretch it), ``kv_heads=N`` (fewer key and value heads)
-and ``norm=pre_rms`` (RMS norms in front of attention and MLP, every block boundary one K24 pass).  The first two take their
-attention from K22, which has no limit on length.
+and ``norm=pre_rms`` (RMS norms in front of attention and MLP, every block boundary one K24 pass).  With any of them attention
+is K22, which has no limit on length and takes bf16 on the GPU (as :func:`prepare` makes the model there; fp32 on the CPU).
 """
 import math
 
@@ -155,7 +155,7 @@ class Bert(nn.Module):
                  rotary_scaling="none", rotary_factor=1.0, rotary_original=512):
         super().__init__()
         kv_heads = kv_heads or heads
-        if hidden % heads or heads % kv_heads:
+        if kv_heads < 0 or hidden % heads or heads % kv_heads:
             raise ValueError("hidden %d must divide over %d heads, and these over %d kv_heads" % (hidden, heads, kv_heads))
         if positions not in ("learned", "rotary") or norm not in ("post_ln", "pre_rms"):
             raise ValueError("positions is learned or rotary, norm post_ln or pre_rms; got %r, %r" % (positions, norm))

@@ -281,6 +281,14 @@ def test_bert_option_refusals():
             bert.build(**{**BERT, **kw})
 
 
+@pytest.mark.parametrize("kv_heads", [-1, -2, -4])
+def test_bert_refuses_negative_key_heads(kv_heads):
+    from distributed_tensorflow_amd.models import bert
+
+    with pytest.raises(ValueError, match="kv_heads"):
+        bert.build(**{**BERT, "kv_heads": kv_heads})
+
+
 def test_rotary_positions_belong_to_the_model_not_to_its_first_call(monkeypatch):
     """A model evaluated under inference_mode first trains afterwards: its frequencies are made where it is built or moved, never
     inside a call.  (Only the GPU's backward saves them, so what the operator is handed is looked at.)"""

@@ -17,8 +17,9 @@
 // Two waves a SIMD carry it: with 64 queries a wave (half the LDS reads, one wave a SIMD) the forward took 918 us, with
 // 32-key steps (three waves) 556, the next step's scores issued under this one's exponentials 640.  LDS reads are one operand
 // of every product, 33..46 % of its cycles.
-// P and dS are rounded to bf16 for the second products (their operands' type: half a step, 2^-9 of each term, random in
-// sign, so the sums keep the accuracy of the bf16 results); scores, maxima, sums, L, D and all accumulators are fp32.
+// P and dS are rounded to bf16 for the second products (their operands' type: off by half a step, up to 2^-8 of each term and
+// 1.65e-3 of it in the mean square, random in sign, so the sums keep the accuracy of the bf16 results, whose own rounding is as
+// large: 2.4e-3 of the norm in all); scores, maxima, sums, L, D and all accumulators are fp32.
 #include "dtf_common.h"
 
 typedef __attribute__((ext_vector_type(4))) short ag_s16x4;

@@ -27,8 +27,9 @@ ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-ffp-contract=fast",
          "-Wall", "-Wno-unused-function",
-         # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware without an error (the
-         # host pass warns that it does not know the feature, which is harmless)
+         # no packed fp32 arithmetic (v_pk_add / mul / fma_f32, which the compiler makes of ordinary float code): some of its
+         # forms have given wrong results on this hardware now and then, without an error.  What it costs: counts and times in
+         # profiles/packed_fp32.txt.  (The host pass warns that it does not know the feature, which is harmless.)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -14,9 +14,9 @@
 // Bound by the matrix pipe and by power: 4 x 4096 tokens, 16 heads of 128, not causal: forward 555 us (990 TF/s), dQ 757 us
 // (1090 in its three products), dK/dV 1060 us (1040 in its four), where a large library product makes 1400..1600; the card
 // lowers its clock under them (1.8 of 2.4 GHz; on zeros instead of random values the same kernels take a fifth less).
-// Two waves a SIMD carry it: with 64 queries a wave (half the LDS reads, one wave a SIMD) the forward took 918 us, with
-// 32-key steps (three waves) 556, the next step's scores issued under this one's exponentials 640.  LDS reads are one operand
-// of every product, 33..46 % of its cycles.
+// Two waves a SIMD carry it (heads to 64: four in the forward, three in the backward): with 64 queries a wave (half the LDS
+// reads, one wave a SIMD) the forward took 918 us, with 32-key steps (three waves) 556, the next step's scores issued under this
+// one's exponentials 640.  LDS reads are one operand of every product, 33..46 % of its cycles.
 // P and dS are rounded to bf16 for the second products (their operands' type: off by half a step, up to 2^-8 of each term and
 // 1.65e-3 of it in the mean square, random in sign, so the sums keep the accuracy of the bf16 results, whose own rounding is as
 // large: 2.4e-3 of the norm in all); scores, maxima, sums, L, D and all accumulators are fp32.
@@ -683,17 +683,18 @@ static int ag_grid(int64_t n, int* out) {
 }
 
 // Workgroups that share a tile (by the whole call's size, so a sequence's sums are grouped by how many others there are, not by
-// what they hold): enough for `fill` workgroups, no fewer than `least` steps each.  512 are resident.  257 queries
-// on 7000 keys, 32 / 8 heads of 128, forward and join: fill 1 141 us, 512 84 + 12, 1024 85 + 19; one token on 8192 keys: fill 1
-// 147 us, 512 11 + 5.  dQ, 512 tokens, 12 heads of 64: fill 1 14 us, 512 11 + 2.
+// what they hold): enough for `fill` workgroups, no fewer than `least` steps each.  512 are resident (768 to 1024 of heads to
+// 64).  2 x 257 queries on 7000 keys, 32 / 8 heads of 128, forward and join: fill 1 151 us, 512 90 + 12, 1024 90 + 20; one token
+// on 8192 keys: fill 1 147 us, 512 9 + 6.  512 tokens, 12 heads of 64, dQ and the sum of its parts: fill 1 14.6 us, 512
+// 11.7 + 3.6; forward and join 12.2, 9.9 + 4.4.
 static int ag_splits(int64_t grid, int64_t steps, int least, int fill) {
     int64_t n = fill / grid, most = steps / least;
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
 
-// PACK where a 128-row tile of one head's queries would be part empty and the group's rows fill fewer tiles: 64 tokens on 2048
-// keys each, 32 / 8 heads: 94 us (5.7 TB/s of K and V), head by head 366; 257 queries on 7000 keys 84 + 12, 104 + 8.
+// PACK where a 128-row tile of one head's queries would be part empty and the group's rows fill fewer tiles: 64 x 1 token on
+// 2048 keys, 32 / 8 heads: 98 us (5.5 TB/s of K and V), head by head 361; 2 x 257 queries on 7000 keys 90 + 12, 109 + 9.
 static bool ag_pack_rows(int Sq, int group) {
     return group > 1 && Sq <= 512 && ((int64_t)group * Sq + 127) / 128 < (int64_t)group * ((Sq + 127) / 128);
 }
@@ -707,7 +708,7 @@ static int ag_fwd_splits(int B, int Sq, int Sk, int Hq, int Hk) {
 }
 
 // Causal tiles differ in length, so the longest should be no more than what a slot gets in all: 8192 tokens, 16 / 4 heads of
-// 128, dK/dV and the sum of the parts: fill 512 882 + 13 us, 1024 640 + 22, 2048 658 + 48; unshared 1423.
+// 128, dK/dV and the sum of the parts: fill 512 895 + 13 us, 1024 581 + 22, 2048 591 + 49; unshared 1404.
 static int ag_dkv_splits(int B, int Sq, int Sk, int Hq, int Hk, int D, int causal) {
     const int bq = D > 64 ? 32 : 64;
     const int64_t steps = (int64_t)((Sq + bq - 1) / bq) * (Hq / Hk);

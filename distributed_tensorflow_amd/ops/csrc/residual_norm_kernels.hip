@@ -504,6 +504,9 @@ static int rn_tpr(int H, int ne) {
 // Workgroups of the backward: nbx share a group's rows, gstep groups go into a launch.  8 waves a CU.  Backward and the sum
 // of the parts behind it at 16384 rows, 8 against 16 waves a CU: width 4096 (rms, both norms) 157 + 6 against 164 + 9 us,
 // 2048 105 + 5 / 119 + 8; layer norms at 768 (65536 rows) 162 + 5 / 156 + 8.
+// More groups than a launch takes go one workgroup a group, launch after launch, and the last launch may be far from full: width
+// 4096, both norms, 256 gate rows over 64 rows each 174 us, 257 288 (one workgroup walks 64 rows in a launch of its own); width
+// 2048, 512 over 32 rows each 84, 513 142, 2048 over 8 each 125.
 static void rn_grid(int64_t M, int H, int64_t groups, int* nbx, int64_t* gstep) {
     const int tpr = rn_tpr(H, 8), rb = tpr < 256 ? 256 / tpr : 1;
     const int64_t target = tpr <= 256 ? 512 : 256;

@@ -7,8 +7,7 @@ Every ``csrc/*.hip`` translation unit is compiled with
 ``hipcc --offload-arch=gfx950`` into ``ops/_build/*.o`` and linked into
 ``ops/libdtf_hip.so`` (a plain C-ABI shared library loaded through ctypes: no
 torch headers, so a unit compiles in seconds and the library does not depend on
-the torch ABI).  The ``.so`` is git-ignored but travels with ``gpurun``
-snapshots; nothing is JIT-compiled at job submit time.
+the torch ABI).  Nothing is JIT-compiled at job submit time.
 An object is compiled again where its source, a header or its command has
 changed (the command is recorded beside it).
 """

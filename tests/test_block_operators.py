@@ -315,6 +315,13 @@ def test_rotary_positions_belong_to_the_model_not_to_its_first_call(monkeypatch)
     assert torch.equal(turn._table(torch.device("cpu")), rotary_frequencies(16)[0])
 
 
+def test_rotary_positions_refuse_a_capture_on_a_device_they_were_not_moved_to(monkeypatch):
+    _, m, _ = _bert(positions="rotary")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="move the model"):
+        m.layers[0].positions._table(torch.device("cuda", 0))
+
+
 def test_constants_of_a_recorded_call_can_be_saved():
     from distributed_tensorflow_amd.ops import hip
 
